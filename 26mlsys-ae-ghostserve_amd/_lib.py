@@ -82,6 +82,73 @@ class KvBhtd(C.Structure):
 
 _kbp = C.POINTER(KvBhtd)
 
+
+class Step(C.Structure):
+    """struct kvec_step of include/kvec.h."""
+    _fields_ = [
+        ("page_table", C.c_void_p),
+        ("batch", C.c_int),
+        ("pages_per_seq", C.c_int),
+        ("page_tokens", C.c_int),
+        ("pool_pages", C.c_int64),
+        ("cached", C.c_void_p),
+        ("new_tokens", C.c_void_p),
+        ("free_pages", C.c_void_p),
+        ("n_free", C.c_int64),
+        ("slots", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("max_tokens", C.c_int64),
+        ("cu_new", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("taken", C.c_void_p),
+    ]
+
+
+class NormRotate(C.Structure):
+    """struct kvec_norm_rotate of include/kvec.h."""
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("heads", C.c_int),
+        ("kv_heads", C.c_int),
+        ("dim", C.c_int),
+        ("dtype", C.c_int),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("q_out", C.c_void_p),
+        ("o_stride", C.c_int64),
+        ("o_head_stride", C.c_int64),
+        ("norm", C.c_int),
+        ("eps", C.c_float),
+        ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p),
+        ("rot", C.c_int),
+        ("interleaved", C.c_int),
+        ("axes", C.c_int),
+        ("positions", C.c_void_p),
+        ("axis_stride", C.c_int64),
+        ("axis_of", C.c_void_p),
+        ("freqs", C.c_void_p),
+        ("factor", C.c_float),
+        ("pool", C.c_void_p),
+        ("pool_dtype", C.c_int),
+        ("n_slots", C.c_int64),
+        ("slots", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("n_tokens", C.c_void_p),
+    ]
+
+
+_sp = C.POINTER(Step)
+_nrp = C.POINTER(NormRotate)
+
 # name -> (restype, argtypes); mirrors include/kvec.h
 SIGNATURES = {
     "kvec_version": (_i, []),
@@ -126,6 +193,8 @@ SIGNATURES = {
     "kvec_rs16_recover_kv": (_i, [_vp, _vp, _vp, _i64, _i, _i, _i, _vp, _i, _vp]),
     "kvec_rs16_reconstruct": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
     "kvec_gf16_tables": (_i, [_vp, _vp]),
+    "kvec_step_tables": (_i, [_sp, _vp]),
+    "kvec_norm_rotate_write": (_i, [_nrp, _vp]),
 }
 
 # major number of the include/kvec.h these signatures mirror (KVEC_VERSION / 10000)
@@ -163,6 +232,15 @@ def call(name: str, *args) -> int:
         msg = lib().kvec_last_error().decode(errors="replace")
         raise KvecError(f"{name} failed ({lib().kvec_strerror(rc).decode()}): {msg}")
     return rc
+
+
+def call_on(device, name: str, *args) -> int:
+    """`call` with ``device`` as the current device: a kernel is launched on the
+    device that its stream belongs to."""
+    if device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
 
 
 EUNSUPPORTED = -2
@@ -213,3 +291,10 @@ def require_cuda(*tensors, what: str = "tensor") -> None:
             raise ValueError(f"{what} must be a GPU (HIP) tensor")
         if not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous")
+
+
+def require_same_device(device, *tensors, what: str = "tensor") -> None:
+    """Every tensor given (None: left out) lies on the GPU ``device``."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise ValueError(f"{what}s must be GPU (HIP) tensors of one device")

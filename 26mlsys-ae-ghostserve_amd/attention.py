@@ -1,0 +1,142 @@
+"""A serving step's work on the paged K/V pool that the codes protect.
+
+No reference counterpart: the reference's plugin hooks an engine that brings its
+own cache writes and attention (bench_ghostserve_rdp.py:396-481).
+
+  norm_rotate_write   queries and keys normed by head and turned to their
+                      positions, keys and values written to their slots
+
+Pool tensor: [layers, pool_pages, page_tokens, 2 (K,V), kv_heads, head_dim], of
+the queries' type or float8_e4m3fn with a scale for K and for V, as in
+:mod:`.paged`; slots and page tables as :func:`.paged.step_tables` makes them.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+
+
+def rotary_frequencies(rot: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """theta^(-2i/rot) for the rot/2 pairs of a rotation, in 64 bits (radians a
+    position); a program with frequencies of its own passes those instead."""
+    if rot < 2 or rot % 2:
+        raise ValueError("rot must be even and positive")
+    i = torch.arange(rot // 2, dtype=torch.float64)
+    return (float(theta) ** (-2.0 * i / rot)).to(device)
+
+
+def rotary_axes(sections, device="cuda") -> torch.Tensor:
+    """axis_of for positions with several axes (time, height, width): the first
+    sections[0] pairs turn with axis 0, the next sections[1] with axis 1, ..."""
+    if not sections or any(int(n) < 0 for n in sections) or len(sections) > 8:
+        raise ValueError("sections are 1 to 8 counts of pairs")
+    n = torch.tensor([int(x) for x in sections])
+    return torch.repeat_interleave(torch.arange(len(sections), dtype=torch.uint8), n).to(device)
+
+
+def _layer(pool: torch.Tensor, layer: int) -> tuple[int, int, int, int]:
+    """(address of the layer, slots, kv_heads, head_dim) of a pool."""
+    if pool.dim() != 6 or pool.shape[3] != 2:
+        raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
+    if not pool.is_cuda or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous GPU (HIP) tensor")
+    L, pages, pt, _, H, D = pool.shape
+    if not 0 <= layer < L:
+        raise ValueError(f"layer {layer} not in [0, {L})")
+    n = pages * pt
+    return pool.data_ptr() + layer * n * 2 * H * D * pool.element_size(), n, H, D
+
+
+def _scale(t, device, what: str):
+    """Address of a scale: a float32 tensor of one value on the GPU, or None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        raise ValueError(f"{what} must be one float32 value on the pool's device")
+    return t.data_ptr()
+
+
+def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None,
+                      freqs: torch.Tensor | None, pool: torch.Tensor, slots: torch.Tensor, *, layer: int = 0,
+                      norm: bool = True, q_weight: torch.Tensor | None = None,
+                      k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                      axis_of: torch.Tensor | None = None, interleaved: bool = False, factor: float = 1.0,
+                      k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                      tokens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Queries and keys normed by head and rotated; K and V written to the pool.
+
+    ``q`` [tokens, heads, dim], ``k`` and ``v`` [tokens, kv_heads, dim], float32,
+    bfloat16 or float16: tensors or views of a packed projection (each head's
+    values adjacent, any other strides).  With ``norm`` each head of q and k is
+    divided by the root of its mean square (+ ``eps``) and multiplied by the
+    weight [dim].  Then its first 2 len(``freqs``) values are turned: pair i by the
+    angle positions * freqs[i], pairs (i, i + len) or, ``interleaved``, (2i, 2i+1),
+    cos and sin times ``factor``.  ``positions``: int32 [tokens], or [axes, tokens]
+    with ``axis_of`` (uint8 [len(freqs)], see :func:`rotary_axes`) naming each
+    pair's axis.  ``freqs``: float64, or None: no rotation.
+
+    Token t's K and V go to slot ``slots[t]`` (int32, page * page_tokens + place;
+    negative or past the pool: none) of the pool's ``layer``, in the queries' type
+    or, float8_e4m3fn, as value / scale.  The slots of a call must be distinct.
+    ``tokens`` (int32 [1] on the GPU, e.g. ``cu_new[-1:]``): tokens from that
+    number on are left as they were, here and in the result.
+
+    Returns the queries (``out``: contiguous like q, or q itself)."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError("q must be [tokens, heads, dim], k and v [tokens, kv_heads, dim]")
+    dev, dt = q.device, q.dtype
+    if dt not in (torch.float32, torch.bfloat16, torch.float16) or k.dtype != dt or v.dtype != dt:
+        raise ValueError("q, k and v must be of one type: float32, bfloat16 or float16")
+    _lib.require_same_device(dev, q, k, v, positions, freqs, pool, slots, q_weight, k_weight, axis_of, tokens, out,
+                             what="norm_rotate_write tensor")
+    N, Hq, D = q.shape
+    base, n_slots, Hk, Dp = _layer(pool, layer)
+    if (Hk, Dp) != (k.shape[1], D):
+        raise ValueError(f"pool holds {Hk} heads of {Dp}, k has {k.shape[1]} of {D}")
+    if pool.dtype != dt and pool.dtype != torch.float8_e4m3fn:
+        raise ValueError("pool must be of q's type or float8_e4m3fn")
+    for t in (q, k, v):
+        if D > 1 and t.shape[0] and t.shape[1] and t.stride(2) != 1:
+            raise ValueError("a head's values must be adjacent")
+    if slots.dtype != torch.int32 or slots.shape != (N,) or not slots.is_contiguous():
+        raise ValueError(f"slots must be contiguous int32 [{N}]")
+    half = 0 if freqs is None else freqs.shape[0]
+    axes, axis_stride = 1, N
+    if half:
+        if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or 2 * half > D:
+            raise ValueError("freqs must be contiguous float64 with at most dim/2 values")
+        if positions is None or positions.dtype != torch.int32 or positions.dim() not in (1, 2) \
+                or positions.shape[-1] != N or (N > 1 and positions.stride(-1) != 1):
+            raise ValueError(f"positions must be int32 [{N}] or [axes, {N}], adjacent by token")
+        if positions.dim() == 2:
+            axes = positions.shape[0]
+            if axes > 1:
+                axis_stride = positions.stride(0)
+                if axis_of is None:
+                    raise ValueError("positions with several axes need axis_of")
+        if axis_of is not None and (axis_of.dtype != torch.uint8 or axis_of.shape != (half,)
+                                    or not axis_of.is_contiguous()):
+            raise ValueError(f"axis_of must be contiguous uint8 [{half}]")
+    for w in (q_weight, k_weight):
+        if w is not None and (not norm or w.dtype != dt or w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f"weights belong to the norm and must be contiguous [{D}] of q's type")
+    if tokens is not None and (tokens.dtype != torch.int32 or tokens.numel() != 1):
+        raise ValueError("tokens must be one int32 value")
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=dt, device=dev)
+    elif out.shape != q.shape or out.dtype != dt or not (out.is_contiguous() or out is q):
+        raise ValueError("out must be contiguous and like q, or q itself")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    s = _lib.NormRotate(
+        N, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
+        k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), int(bool(norm)), eps,
+        ptr(q_weight), ptr(k_weight), 2 * half, int(bool(interleaved)), axes, ptr(positions), axis_stride,
+        ptr(axis_of), ptr(freqs), factor, base, _DTYPES[pool.dtype], n_slots, slots.data_ptr(),
+        _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), ptr(tokens))
+    _lib.call_on(dev, "kvec_norm_rotate_write", ctypes.byref(s), _lib.stream_handle(dev))
+    return out

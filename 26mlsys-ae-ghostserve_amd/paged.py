@@ -8,10 +8,15 @@ pool page indices.  Stream of a chunk of ``tokens`` positions starting at
 ``tok_off``: the chunk's token records in order,
 [layers, batch, tokens, 2 (K,V), kv_heads, head_dim], so each pool page
 contributes contiguous runs of records.
+
+``step_tables`` makes a serving step's page table rows and slots on the GPU from
+the lengths of its requests (no reference counterpart: the reference's plugin
+takes both from the engine that it hooks, bench_ghostserve_rdp.py:440-458).
 """
 from __future__ import annotations
 
-from typing import Sequence
+import ctypes
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -83,6 +88,64 @@ class PagedKV:
         _lib.require_cuda(stream, what="scatter input")
         _lib.call("kvec_kv_scatter", self._c, self.pool.data_ptr(), stream.data_ptr(),
                   _lib.stream_handle(stream.device))
+
+
+class StepTables(NamedTuple):
+    """What a step needs beside its page table: int32 tensors on the GPU."""
+    slots: torch.Tensor       # [max_tokens], -1 where a token has none
+    positions: torch.Tensor   # [max_tokens], each token's position in its request
+    cu_new: torch.Tensor      # [batch + 1], the tokens before each request
+    seq_lens: torch.Tensor    # [batch], cached + new
+    taken: torch.Tensor       # [1], pages the step needs of the free list
+
+
+def step_tables(page_table: torch.Tensor, cached: torch.Tensor, new: torch.Tensor, free_pages: torch.Tensor,
+                pool_pages: int, page_tokens: int, max_tokens: int,
+                out: StepTables | None = None) -> StepTables:
+    """Page table rows and slots of a step, from its requests' lengths, on the GPU.
+
+    Request b holds ``cached[b]`` tokens in the pages that its row of
+    ``page_table`` names, and gets ``new[b]`` more this step (0: idle).  The pages
+    that it needs beyond those are taken from ``free_pages`` in the order of the
+    requests and written into its row (in place; -1 once the list is used up,
+    and behind its last page).  The step's tokens are the requests' new tokens
+    one after another; ``max_tokens`` is the room for them, and what is left of
+    it gets slot -1 and position 0 (the hook's ``slot_mapping``).  A token whose
+    page is missing has slot -1.  ``taken`` above ``free_pages.numel()`` says that the
+    list was too short.
+
+    All tensors int32, contiguous, on one GPU; ``page_table`` [batch,
+    pages_per_seq].  ``out``: an earlier result of the same sizes, written again.
+    Nothing is read back to the host, so the call can be captured in a graph."""
+    if page_table.dim() != 2 or cached.dim() != 1 or new.dim() != 1 or free_pages.dim() != 1:
+        raise ValueError("page_table must be [batch, pages_per_seq], cached, new and free_pages one-dimensional")
+    B, width = page_table.shape
+    if cached.shape[0] != B or new.shape[0] != B:
+        raise ValueError(f"cached and new must have one entry for each of {B} requests")
+    for t in (page_table, cached, new, free_pages):
+        if t.dtype != torch.int32:
+            raise ValueError("page_table, cached, new and free_pages must be int32")
+    dev = page_table.device
+    _lib.require_cuda(page_table, cached, new, free_pages, what="step table")
+    _lib.require_same_device(dev, cached, new, free_pages, what="step table")
+    T = int(max_tokens)
+    if T < 0:
+        raise ValueError("max_tokens must not be negative")
+    if out is None:
+        buf = torch.empty(2 * T + 2 * B + 2, dtype=torch.int32, device=dev)
+        out = StepTables(*buf.split_with_sizes([T, T, B + 1, B, 1]))
+    else:
+        for t, n in zip(out, (T, T, B + 1, B, 1)):
+            if t.dtype != torch.int32 or t.shape != (n,):
+                raise ValueError("out is not of this step's sizes")
+        _lib.require_cuda(*out, what="step table")
+        _lib.require_same_device(dev, *out, what="step table")
+    s = _lib.Step(page_table.data_ptr(), B, width, int(page_tokens), int(pool_pages), cached.data_ptr(),
+                  new.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], out.slots.data_ptr(),
+                  out.positions.data_ptr(), T, out.cu_new.data_ptr(), out.seq_lens.data_ptr(),
+                  out.taken.data_ptr())
+    _lib.call_on(dev, "kvec_step_tables", ctypes.byref(s), _lib.stream_handle(dev))
+    return out
 
 
 def rdp_row_bytes_for(kv: PagedKV, k: int, p: int) -> int:

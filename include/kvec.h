@@ -41,8 +41,8 @@ extern "C" {
  * 1.0.0: kvec_rdp_encode / kvec_rdp_decode / kvec_rdp_encode_paged take
  * unit_bytes, kvec_chunk_stripe has region_off and unit_bytes (0.1.0 had
  * neither).  1.1.0: kvec_hook_step added.  1.2.0: the *_kv entry points over
- * kvec_kv_bhtd added. */
-#define KVEC_VERSION 10200
+ * kvec_kv_bhtd added.  1.3.0: kvec_step_tables, kvec_norm_rotate_write added. */
+#define KVEC_VERSION 10300
 int kvec_version(void);
 /* Static description of a KVEC_E* code. */
 const char* kvec_strerror(int code);
@@ -369,6 +369,91 @@ int kvec_rs16_recover_kv(void* shards, void* key_output, void* value_output, int
 /* init_gf_tables, benchmark/rs/main.py:39-54, into host arrays (exp: 131070
  * entries, log: 65536). */
 int kvec_gf16_tables(uint16_t* gf_exp, uint16_t* gf_log);
+
+/* ==================== a serving step over the paged pool ==================== */
+/* No reference counterparts: the reference's plugin hooks a serving engine that
+ * brings its own page tables, cache writes and attention
+ * (bench_ghostserve_rdp.py:396-481).  These are the parts of a step that make,
+ * fill and read the paged pool which the calls above code and rebuild. */
+
+#define KVEC_F32 0
+#define KVEC_BF16 1
+#define KVEC_F16 2
+#define KVEC_FP8_E4M3 3 /* the finite-only e4m3 of the OCP 8-bit formats */
+
+/* Page table rows and slots of a step, from the requests' lengths.  Request b
+ * holds `cached[b]` tokens and gets `new_tokens[b]` more (negative: none).  Its
+ * pages ceil(cached/page_tokens) .. ceil((cached + new)/page_tokens) - 1 are
+ * taken from free_pages in the order of the requests (entries past the list,
+ * and every entry behind the request's last page, become -1; entries before
+ * are kept).  Token t of the step (the requests' new tokens one after another)
+ * gets its position in its request and its slot page*page_tokens + position %
+ * page_tokens, -1 where the page is not in [0, pool_pages) or past the row;
+ * t >= the step's tokens: slot -1, position 0.  cu_new [batch + 1]: the tokens
+ * before each request; seq_lens [batch] = cached + new; taken [1]: the pages
+ * that the step needs, which is more than n_free if the list was too short.
+ * Sums past 2^31 - 1 stay there.  page_tokens is a power of two; pool_pages *
+ * page_tokens <= 2^31.  All arrays are device int32. */
+typedef struct kvec_step {
+    int32_t* page_table;        /* [batch][pages_per_seq], rewritten */
+    int batch;
+    int pages_per_seq;
+    int page_tokens;
+    int64_t pool_pages;
+    const int32_t* cached;      /* [batch] */
+    const int32_t* new_tokens;  /* [batch] */
+    const int32_t* free_pages;  /* [n_free] */
+    int64_t n_free;
+    int32_t* slots;             /* [max_tokens] */
+    int32_t* positions;         /* [max_tokens] */
+    int64_t max_tokens;
+    int32_t* cu_new;
+    int32_t* seq_lens;
+    int32_t* taken;
+} kvec_step;
+int kvec_step_tables(const kvec_step* step, void* stream);
+
+/* Queries and keys of a step normed by head and turned to their positions, and
+ * keys and values written to their slots of one layer of the pool, in one pass:
+ *   x = x * rsqrt(mean(x^2) + eps) * weight     (norm != 0; weight NULL: 1)
+ *   pair i of the first `rot` values: (a c - b s, a s + b c), with c, s =
+ *   factor * cos, factor * sin of positions[axis_of[i]][t] * freqs[i]
+ * Pair i is (x[i], x[i + rot/2]), or (x[2i], x[2i+1]) if interleaved; values
+ * from rot on are not turned.  Angles in 64 bits, the rest in 32, one rounding
+ * at the end.  An fp8 pool gets x / scale, values past +-448 as +-448.
+ * Queries go to q_out (q itself with q's strides: in place).  A slot outside
+ * [0, n_slots) is skipped; the slots of a call must be distinct.  Tokens from
+ * *n_tokens on (if given) are left as they were.  Strides in elements, each
+ * head's values adjacent.  dim <= 512, rot even and <= dim, axes <= 8. */
+typedef struct kvec_norm_rotate {
+    int64_t tokens;
+    int heads, kv_heads, dim;
+    int dtype;                  /* of q, k, v, q_out: KVEC_F32, KVEC_BF16, KVEC_F16 */
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    void* q_out;
+    int64_t o_stride, o_head_stride;
+    int norm;
+    float eps;
+    const void* q_weight;       /* [dim] of `dtype`, or NULL */
+    const void* k_weight;
+    int rot, interleaved, axes;
+    const int32_t* positions;   /* [tokens] for each axis, axis_stride apart (0: one for all) */
+    int64_t axis_stride;
+    const uint8_t* axis_of;     /* [rot/2], or NULL: axis 0 (entries past the last axis: the last) */
+    const double* freqs;        /* [rot/2] radians a position */
+    float factor;
+    void* pool;                 /* the layer: [n_slots][2 (K,V)][kv_heads][dim] */
+    int pool_dtype;             /* dtype, or KVEC_FP8_E4M3 */
+    int64_t n_slots;
+    const int32_t* slots;       /* [tokens] */
+    const float* k_scale;       /* [1] each, device, or NULL: 1 */
+    const float* v_scale;
+    const int32_t* n_tokens;    /* [1], device, or NULL: all */
+} kvec_norm_rotate;
+int kvec_norm_rotate_write(const kvec_norm_rotate* step, void* stream);
 
 #ifdef __cplusplus
 }
