@@ -146,7 +146,41 @@ class NormRotate(C.Structure):
     ]
 
 
+class Attention(C.Structure):
+    """struct kvec_attention of include/kvec.h."""
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("batch", C.c_int),
+        ("heads", C.c_int),
+        ("kv_heads", C.c_int),
+        ("dim", C.c_int),
+        ("dtype", C.c_int),
+        ("q", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("out", C.c_void_p),
+        ("o_stride", C.c_int64),
+        ("o_head_stride", C.c_int64),
+        ("pool", C.c_void_p),
+        ("pool_dtype", C.c_int),
+        ("pool_pages", C.c_int64),
+        ("page_tokens", C.c_int),
+        ("page_table", C.c_void_p),
+        ("pages_per_seq", C.c_int),
+        ("seq_lens", C.c_void_p),
+        ("cu_q", C.c_void_p),
+        ("max_q", C.c_int),
+        ("max_len", C.c_int64),
+        ("prefix", C.c_int64),
+        ("prefix_pages", C.c_void_p),
+        ("scale", C.c_float),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+    ]
+
+
 _sp = C.POINTER(Step)
+_ap = C.POINTER(Attention)
 _nrp = C.POINTER(NormRotate)
 
 # name -> (restype, argtypes); mirrors include/kvec.h
@@ -195,6 +229,8 @@ SIGNATURES = {
     "kvec_gf16_tables": (_i, [_vp, _vp]),
     "kvec_step_tables": (_i, [_sp, _vp]),
     "kvec_norm_rotate_write": (_i, [_nrp, _vp]),
+    "kvec_prefix_attention_workspace": (_i64, [_ap]),
+    "kvec_prefix_attention": (_i, [_ap, _vp, _i64, _vp]),
 }
 
 # major number of the include/kvec.h these signatures mirror (KVEC_VERSION / 10000)

@@ -5,6 +5,8 @@ own cache writes and attention (bench_ghostserve_rdp.py:396-481).
 
   norm_rotate_write   queries and keys normed by head and turned to their
                       positions, keys and values written to their slots
+  prefix_attention    attention over the pool for a batch whose requests share
+                      a prefix, which is computed once for all of them
 
 Pool tensor: [layers, pool_pages, page_tokens, 2 (K,V), kv_heads, head_dim], of
 the queries' type or float8_e4m3fn with a scale for K and for V, as in
@@ -139,4 +141,78 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
         ptr(axis_of), ptr(freqs), factor, base, _DTYPES[pool.dtype], n_slots, slots.data_ptr(),
         _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), ptr(tokens))
     _lib.call_on(dev, "kvec_norm_rotate_write", ctypes.byref(s), _lib.stream_handle(dev))
+    return out
+
+
+def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                     prefix: int = 0, *, layer: int = 0, cu_q: torch.Tensor | None = None,
+                     max_q: int | None = None, max_len: int | None = None,
+                     prefix_pages: torch.Tensor | None = None, scale: float | None = None,
+                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a step's queries over the pool's ``layer``.
+
+    ``q`` [tokens, heads, dim] (bfloat16 or float16; each head's values adjacent):
+    the requests' new tokens one after another, request b's from ``cu_q[b]`` to
+    ``cu_q[b+1]`` - 1, or without ``cu_q`` one token a request.  Request b holds
+    ``seq_lens[b]`` tokens, its new ones included (their K and V are in the pool
+    already, see :func:`norm_rotate_write`), on the pages of its row of
+    ``page_table``; each query sees the positions up to its own.  Query heads
+    share K/V heads in order.  dim: a multiple of 8 (fp8 pool: 16) up to 256.
+
+    The first ``prefix`` positions are the same for all requests; they are read
+    from ``prefix_pages`` (default: the first row of ``page_table``) once for all
+    queries.  ``prefix`` need not be whole pages.  0 is ordinary paged attention.
+
+    Keys on pages outside the pool are left out; a query that sees no key (an idle
+    row: ``seq_lens`` 0) gives zeros.  Rows from ``cu_q[-1]`` on are left as they
+    were.  ``max_q``: the most tokens of a request (default: all tokens), ``max_len``:
+    about the longest of ``seq_lens`` (default: what a table row can hold); closer
+    values split the work better.  ``scale``: default 1/sqrt(dim).  ``k_scale``,
+    ``v_scale``: an fp8 pool's, as in :func:`norm_rotate_write`.  Nothing is read
+    back to the host, so the call can be captured in a graph."""
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, heads, dim]")
+    dev, dt = q.device, q.dtype
+    if dt not in (torch.bfloat16, torch.float16):
+        raise ValueError("q must be bfloat16 or float16")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise ValueError("page_table must be int32 [batch, pages_per_seq], seq_lens int32")
+    N, Hq, D = q.shape
+    B, width = page_table.shape
+    if seq_lens.shape != (B,) or (cu_q is not None and (cu_q.shape != (B + 1,) or cu_q.dtype != torch.int32)):
+        raise ValueError(f"seq_lens must be [{B}] and cu_q int32 [{B + 1}]")
+    if cu_q is None and N != B:
+        raise ValueError("without cu_q there is one query token a request")
+    _lib.require_same_device(dev, q, pool, page_table, seq_lens, cu_q, prefix_pages, out,
+                             what="prefix_attention tensor")
+    base, _, Hk, Dp = _layer(pool, layer)
+    if Dp != D or Hq % Hk:
+        raise ValueError(f"q has {Hq} heads of {D}, the pool {Hk} of {Dp}")
+    if pool.dtype != dt and pool.dtype != torch.float8_e4m3fn:
+        raise ValueError("pool must be of q's type or float8_e4m3fn")
+    for t in (page_table, seq_lens, cu_q, prefix_pages):
+        if t is not None and not t.is_contiguous():
+            raise ValueError("page_table, seq_lens, cu_q and prefix_pages must be contiguous")
+    if N and D > 1 and q.stride(2) != 1:
+        raise ValueError("a head's values must be adjacent")
+    pt, prefix = pool.shape[2], int(prefix)
+    pages = page_table if prefix_pages is None else prefix_pages
+    if prefix_pages is not None and (prefix_pages.dtype != torch.int32 or prefix_pages.numel() * pt < prefix):
+        raise ValueError("prefix_pages must be int32 and hold the prefix")
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=dt, device=dev)
+    elif out.shape != q.shape or out.dtype != dt or not out.is_contiguous():
+        raise ValueError("out must be contiguous and like q")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    s = _lib.Attention(
+        N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
+        out.stride(1), base, _DTYPES[pool.dtype], pool.shape[1], pt, page_table.data_ptr(), width,
+        seq_lens.data_ptr(), ptr(cu_q), int(max_q if max_q is not None else max(N, 1)), int(max_len or 0), prefix,
+        pages.data_ptr(), D ** -0.5 if scale is None else float(scale), _scale(k_scale, dev, "k_scale"),
+        _scale(v_scale, dev, "v_scale"))
+    ref = ctypes.byref(s)
+    need = _lib.lib().kvec_prefix_attention_workspace(ref)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    _lib.call_on(dev, "kvec_prefix_attention", ref, ptr(ws), max(need, 0), _lib.stream_handle(dev))
     return out

@@ -1,0 +1,990 @@
+// attention.hip -- attention over the paged pool for a batch that shares a prefix.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m)
+//
+// over the keys j that the query sees: positions up to its own, on pages inside
+// the pool.  Positions below `prefix` are the same for all requests and are read
+// from one list of pages; their part of the sum is computed for the rows of all
+// requests together (a row: one query head of one token), so that a tile of keys
+// is read once for as many rows as fill a matrix instruction, not once a
+// request.  Each request's own keys are a second part; parts are joined by
+// their maxima and sums, which are linear once both are brought to one maximum.
+//
+// Both kernels form S^T = K Q^T and O^T += V^T P^T, keys along the rows of the
+// matrix instructions and query rows along their columns: a lane then holds
+// scores of one query row only, so the softmax needs one exchange between lane
+// halves (or quarters) for the maximum and none for the sum, and the scores
+// that a lane holds are, rounded to 16 bits, just what the second product wants
+// from it (the instruction sums over keys in any order, so long as V^T comes
+// in the same one: rows 4h .. and 8 + 4h .. of each 16).  V lies [key][value]
+// and is needed transposed, which ds_read_b64_tr_b16 does on the way from LDS.
+//
+// Scores, maxima, sums and outputs are 32-bit; P is rounded to 16 bits for the
+// second product (its largest value is near 1, the rounding is half a step of
+// the inputs' own type), and the output once at the end.
+//
+// Masked keys: a key past a row's last one or on a page outside the pool has
+// p = 0 by selection; keys that no row of a tile sees are read as zeros, so what
+// a page holds behind its last token (NaN, say) has no part.  Where some rows of
+// a tile see a key and others do not, a V value that is not finite would reach
+// the others as 0 * NaN: such values are taken out of the product and added to
+// the rows that see them (add_not_finite).
+#include "lm_types.h"
+#include "paged_geom.h"
+
+namespace kvec {
+
+constexpr int kAB = 256;                       // threads of a block: 4 waves
+constexpr int kTileRows = 128;                 // rows of a tile block, 32 a wave
+constexpr int kTileKeys = 64;
+constexpr int kStreamRows = 16;                // rows of a stream block
+constexpr int kStreamKeys = 32;                // keys a wave takes at a time
+constexpr float kLog2e = 1.44269504088896340736f;
+// The running maximum moves only when a score passes it by this much (in
+// powers of two): p stays under 2^8, and most tiles rescale nothing.
+constexpr float kLazy = 8.0f;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c, __bf16*) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c, _Float16*) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c, __bf16*) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c, _Float16*) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Transposed read of 16-bit values: within 16 lanes, lane i gives the address
+// of columns 4 (i % 4) .. + 3 of row i / 4 and gets column i of the four rows.
+__device__ __forceinline__ u32x2 lds_tr(const uint8_t* p) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p));
+}
+
+// Four e4m3 values to four 16-bit ones: exact in both types.
+__device__ __forceinline__ u32x2 fp8_widen(uint32_t v, __bf16*) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, true))};
+}
+__device__ __forceinline__ u32x2 fp8_widen(uint32_t v, _Float16*) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true))};
+}
+
+// Whether a 16-bit value is infinite or NaN: all its exponent bits are set.
+__device__ __forceinline__ uint32_t exponent_bits(__bf16*) { return 0x7F80u; }
+__device__ __forceinline__ uint32_t exponent_bits(_Float16*) { return 0x7C00u; }
+
+// The values of four that are not finite, zeros for the others; v: 16-bit pairs.
+template <class T>
+__device__ __forceinline__ f32x4 not_finite(u32x2 v, T*) {
+    f32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t w = j < 2 ? v.x : v.y;
+        const float f = float(__builtin_bit_cast(T, uint16_t(j & 1 ? w >> 16 : w & 0xFFFFu)));
+        x[j] = __builtin_fabsf(f) < INFINITY ? 0.0f : f;
+    }
+    return x;
+}
+
+// The lowest n bits, n clamped to 0 .. 32.
+__device__ __forceinline__ uint32_t low_bits(int32_t n) {
+    return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+// A value that the compiler takes for a new one: what is compared
+// with it is compared again each time, instead of once with a register pair
+// held for each lane mask over a whole loop.
+__device__ __forceinline__ uint32_t anew(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+struct AttnArgs {
+    const uint8_t* q;
+    uint8_t* out;
+    int64_t qs, qh, os, oh;                    // elements
+    const uint8_t* pool;                       // the layer
+    const int32_t* table;
+    const int32_t* prefix_pages;
+    const int32_t* seq_lens;
+    const int32_t* cu;                         // null: one token a request
+    const float *k_scale, *v_scale;
+    float* ws_o;                               // [parts][rows][dim]
+    f32x2* ws_ml;                              // [parts][rows]: maximum (powers of two), sum
+    uint64_t rec;                              // bytes of a token record
+    uint32_t token_bytes;
+    uint32_t tokens, batch, heads, kv_heads, group, dim;
+    uint32_t width, shift, pool_pages, cap;    // cap: positions that a table row covers
+    uint32_t prefix;                           // keys of the shared part (0: none)
+    uint32_t first;                            // first own key: prefix, or 0 with the prefix's pages read there
+    uint32_t parts_flat, parts_own;            // splits of the keys of each part
+    uint32_t tiles;                            // row tiles (upper bound) of this launch
+    uint32_t req_tiles;                        // stream kernel, own keys: row tiles of a request
+    int flat;                                  // this launch: rows of all requests on the prefix
+    int direct;                                // one part in all: outputs are final
+    int wide_q, wide_o;                        // 16-byte rows
+    float scale;
+};
+
+__device__ __forceinline__ uint32_t first_token(const AttnArgs& a, uint32_t b) {
+    return a.cu ? uint32_t(a.cu[b]) : b;
+}
+__device__ __forceinline__ uint32_t live_tokens(const AttnArgs& a) {
+    return a.cu ? min(uint32_t(max(a.cu[a.batch], 0)), a.tokens) : a.tokens;
+}
+// The request that token t (a live one) belongs to.
+__device__ __forceinline__ uint32_t request_of(const AttnArgs& a, uint32_t t) {
+    if (!a.cu) return t;
+    uint32_t lo = 0, hi = a.batch;             // cu[lo] <= t < cu[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (uint32_t(a.cu[mid]) <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// Keys that token t of request b sees.
+__device__ __forceinline__ uint32_t seen_by(const AttnArgs& a, uint32_t b, uint32_t t) {
+    const int64_t n = int64_t(a.seq_lens[b]) - int64_t(first_token(a, b + 1)) + int64_t(t) + 1;
+    return uint32_t(n < 0 ? 0 : n > int64_t(a.cap) ? int64_t(a.cap) : n);
+}
+
+// What a block works on: rows row0 .. of a segment's rows, keys k0 .. k1 - 1.
+struct Item {
+    bool live;
+    uint32_t b;                                // request (own keys)
+    uint32_t t0;                               // its first token (0: all requests' rows)
+    uint32_t rows;                             // rows of the segment
+    uint32_t row0;
+    uint32_t head;                             // K/V head
+    uint32_t part;                             // where its partial result goes
+    uint32_t k0, k1;
+};
+
+template <bool STREAM>
+__device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
+    constexpr uint32_t BM = STREAM ? kStreamRows : kTileRows;
+    constexpr uint32_t KEYS = STREAM ? 4 * kStreamKeys : kTileKeys;
+    Item it{};
+    const uint32_t parts = a.flat ? a.parts_flat : a.parts_own;
+    const uint32_t tile = id % a.tiles, rest = id / a.tiles;
+    const uint32_t split = rest % parts;
+    it.head = rest / parts;
+    it.part = a.flat ? split : a.parts_flat + split;
+    uint32_t first = 0, last;
+    if (a.flat) {
+        it.rows = live_tokens(a) * a.group;
+        it.row0 = tile * BM;
+        it.live = it.row0 < it.rows;
+        last = a.prefix;
+    } else {
+        uint32_t local;
+        if (STREAM) {
+            it.b = tile / a.req_tiles;
+            local = tile % a.req_tiles;
+        } else {
+            // request b's tiles start at floor(cu_b G / BM) + b, at least as far
+            // apart as it has tiles
+            uint32_t lo = 0, hi = a.batch;
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (uint32_t((uint64_t(first_token(a, mid)) * a.group) / BM) + mid <= tile) lo = mid;
+                else hi = mid;
+            }
+            it.b = lo;
+            local = tile - uint32_t((uint64_t(first_token(a, lo)) * a.group) / BM) - lo;
+        }
+        it.t0 = first_token(a, it.b);
+        const uint32_t t1 = min(first_token(a, it.b + 1), a.tokens);
+        it.rows = t1 > it.t0 ? (t1 - it.t0) * a.group : 0u;
+        it.row0 = local * BM;
+        it.live = it.row0 < it.rows;
+        first = a.first;
+        last = 0;
+        if (it.live) {
+            const uint32_t end_row = min(it.row0 + BM, it.rows) - 1;
+            last = seen_by(a, it.b, it.t0 + end_row / a.group);
+        }
+    }
+    // equal shares of the keys, in whole steps
+    const uint32_t n = last > first ? last - first : 0u;
+    const uint32_t steps = (n + KEYS - 1) / KEYS, each = (steps + parts - 1) / parts;
+    it.k0 = first + min(uint64_t(split) * each * KEYS, uint64_t(n));
+    it.k1 = first + min(uint64_t(split + 1) * each * KEYS, uint64_t(n));
+    return it;
+}
+
+// The slot of a key, or kNoCell where there is none.
+__device__ __forceinline__ uint32_t key_slot(const AttnArgs& a, const Item& it, uint32_t pos) {
+    if (pos >= it.k1) return kNoCell;
+    const uint32_t j = pos >> a.shift;
+    const int32_t* row = a.flat || pos < a.prefix ? a.prefix_pages : a.table + uint64_t(it.b) * a.width;
+    const uint32_t page = uint32_t(row[j]);
+    return page < a.pool_pages ? (page << a.shift) | (pos & ((1u << a.shift) - 1)) : kNoCell;
+}
+
+// A 16-byte chunk of a key's K (or V) row, zeros where there is no key.
+__device__ __forceinline__ const uint8_t* chunk_at(const AttnArgs& a, uint32_t slot, uint32_t off, bool inside) {
+    return slot != kNoCell && inside ? a.pool + uint64_t(slot) * a.rec + off : reinterpret_cast<const uint8_t*>(kZeroCell);
+}
+
+// What a product of a query and a key is multiplied by, in powers of two.
+__device__ __forceinline__ float score_factor(const AttnArgs& a) {
+    const float c = a.scale * kLog2e * (a.k_scale ? *a.k_scale : 1.0f);
+    return c == 0.0f ? 1e-30f : c;
+}
+
+// A row's maximum and sum at the end: none for one that sees nothing, and a
+// maximum for a sum that is NaN (all its scores were), so that it is not taken
+// for a row without keys when parts are joined.
+__device__ __forceinline__ void settle(float& m, float& l, bool sees) {
+    if (!sees) m = -INFINITY, l = 0.0f;
+    else if (l != l && m == -INFINITY) m = 0.0f;
+}
+
+// Four values of a key's V row from value d on, zeros where there are none.
+template <class T, bool FP8>
+__device__ __forceinline__ u32x2 value4(const AttnArgs& a, uint32_t slot, uint32_t head_off, uint32_t d) {
+    const uint8_t* p = chunk_at(a, slot, a.token_bytes + head_off + d * (FP8 ? 1 : 2), d < anew(a.dim));
+    if constexpr (FP8) return fp8_widen(*as_global(reinterpret_cast<const uint32_t*>(p)), (T*)nullptr);
+    else return *as_global(reinterpret_cast<const u32x2*>(p));
+}
+
+// Eight values of a query row (zeros past the head's end).
+template <class T>
+__device__ __forceinline__ u32x4 load_q(const AttnArgs& a, const T* row, uint32_t d) {
+    u32x4 v = {0, 0, 0, 0};
+    if (!row || d >= a.dim) return v;
+    if (a.wide_q) return ld16(reinterpret_cast<const uint8_t*>(row + d));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        v[j] = uint32_t(__builtin_bit_cast(uint16_t, *as_global(row + d + 2 * j))) |
+               uint32_t(__builtin_bit_cast(uint16_t, *as_global(row + d + 2 * j + 1))) << 16;
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, f32x4 v, bool wide) {
+    T* t = nullptr;
+    if (wide) {
+        *as_global(reinterpret_cast<u32x2*>(p)) = u32x2{pack2(v.x, v.y, t), pack2(v.z, v.w, t)};
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put1(p + j, v[j]);
+    }
+}
+
+// A finished quarter of a row: into the workspace, or the output.
+template <class T>
+__device__ __forceinline__ void emit4(const AttnArgs& a, const Item& it, uint32_t token, uint32_t head, uint32_t d,
+                                      f32x4 o, float inv_l) {
+    if (d >= anew(a.dim)) return;
+    if (a.direct) {
+        store4(reinterpret_cast<T*>(a.out) + int64_t(token) * a.os + int64_t(head) * a.oh + d,
+               f32x4{o.x * inv_l, o.y * inv_l, o.z * inv_l, o.w * inv_l}, a.wide_o);
+    } else {
+        const uint64_t row = uint64_t(it.part) * a.tokens * a.heads + uint64_t(token) * a.heads + head;
+        *as_global(reinterpret_cast<f32x4*>(a.ws_o + row * a.dim + d)) = o;
+    }
+}
+
+// ------------------------------------------------------------- tile kernel
+// 128 rows against tiles of 64 keys: for rows enough to be bound by the matrix
+// units.  Each wave owns 32 rows (Q in registers); the four waves share the K
+// and V tiles in LDS, read one tile ahead through registers.  Row strides of K
+// and V in LDS are 16 and 32 bytes past a multiple of the banks, so the 16
+// rows (8 rows of 32 bytes, transposed) that a phase reads lie on all banks.
+template <class T, bool FP8, int DP>
+__global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
+    constexpr int KS = DP / 16, DB = DP / 32;
+    constexpr int KROW = DP * 2 + 16, VROW = DP * 2 + 32;
+    constexpr int CH = DP / (FP8 ? 16 : 8);               // 16-byte chunks of a row in the pool
+    constexpr int PER = (kTileKeys * CH + kAB - 1) / kAB;  // chunks a thread
+    __shared__ __attribute__((aligned(16))) uint8_t lk[2][kTileKeys * KROW];
+    __shared__ __attribute__((aligned(16))) uint8_t lv[2][kTileKeys * VROW];
+    __shared__ uint32_t odd;                              // V values that are not finite were taken out
+
+    const Item it = make_item<false>(a, blockIdx.x);
+    if (!it.live) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t r = lane & 31, h = lane >> 5;
+    T* const ty = nullptr;
+
+    // the lane's row
+    const uint32_t row = it.row0 + wave * 32 + r;
+    const bool has = row < it.rows;
+    const uint32_t token = it.t0 + (has ? row / a.group : 0u);
+    const uint32_t head = it.head * a.group + (has ? row % a.group : 0u);
+    // rows that are not there, and rows that see nothing, ask for no mask
+    const uint32_t seen = has ? seen_by(a, a.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
+    // 0 would make NaN of a masked score; a negative one goes to the query
+    const float c0 = score_factor(a);
+    const uint32_t sign = c0 < 0.0f ? 0x80008000u : 0u;
+    u32x4 qf[KS];
+    {
+        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, uint32_t(s * 16) + h * 8) ^ sign;
+    }
+    // the fewest keys that a row of the wave, and of the block, sees
+    uint32_t low = limit;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
+    low = __builtin_amdgcn_readfirstlane(low);
+    __shared__ uint32_t lows[4];
+    if (lane == 0) lows[wave] = low;
+    if (tid == 0) odd = 0;
+    __syncthreads();
+    const uint32_t block_low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
+
+    const float c = fabsf(c0);
+    float m = -INFINITY, l = 0.0f;
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+
+    const uint32_t head_off = it.head * (a.token_bytes / a.kv_heads);
+    const uint32_t row_bytes = a.token_bytes / a.kv_heads;
+    u32x4 xk[PER], xv[PER];
+    auto fetch = [&](uint32_t slot) {                     // slot: of the tile's key `lane`
+        const uint32_t inside = anew(row_bytes);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t idx = i * kAB + tid, key = idx / CH, ch = idx % CH;
+            const uint32_t s = uint32_t(__shfl(int(slot), int(key & 63), 64));
+            const bool in = ch * 16 < inside && key < uint32_t(kTileKeys);
+            xk[i] = ld16(chunk_at(a, s, head_off + ch * 16, in));
+            xv[i] = ld16(chunk_at(a, s, a.token_bytes + head_off + ch * 16, in));
+        }
+    };
+    auto put16 = [&](uint8_t* p, u32x4 v) { *reinterpret_cast<u32x4*>(p) = v; };
+    // V values that are not finite become 0
+    auto scrub = [&](u32x4 v) {
+        const uint32_t e = exponent_bits(ty);
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t w = v[j];
+            if ((w & e) == e) w &= 0xFFFF0000u, bad = true;
+            if (((w >> 16) & e) == e) w &= 0x0000FFFFu, bad = true;
+            v[j] = w;
+        }
+        if (bad) odd = 1;
+        return v;
+    };
+    auto stage = [&](int buf, bool careful) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t idx = i * kAB + tid, key = idx / CH, ch = idx % CH;
+            if (kTileKeys * CH % kAB && key >= uint32_t(kTileKeys)) break;
+            uint8_t* pk = lk[buf] + key * KROW;
+            uint8_t* pv = lv[buf] + key * VROW;
+            if constexpr (FP8) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const u32x2 k0 = fp8_widen(xk[i][2 * j], ty), k1 = fp8_widen(xk[i][2 * j + 1], ty);
+                    const u32x2 v0 = fp8_widen(xv[i][2 * j], ty), v1 = fp8_widen(xv[i][2 * j + 1], ty);
+                    u32x4 v = {v0.x, v0.y, v1.x, v1.y};
+                    if (careful) v = scrub(v);
+                    put16(pk + ch * 32 + j * 16, u32x4{k0.x, k0.y, k1.x, k1.y});
+                    put16(pv + ch * 32 + j * 16, v);
+                }
+            } else {
+                u32x4 v = xv[i];
+                if (careful) v = scrub(v);
+                put16(pk + ch * 16, xk[i]);
+                put16(pv + ch * 16, v);
+            }
+        }
+    };
+
+    const uint32_t ntiles = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
+    uint32_t slot = 0, slot_next = 0;                     // the lane's key of this tile and the next
+    if (ntiles) {
+        slot = key_slot(a, it, it.k0 + lane);
+        fetch(slot);
+        slot_next = key_slot(a, it, it.k0 + kTileKeys + lane);
+        stage(0, it.k0 + kTileKeys > block_low);
+    }
+    __syncthreads();
+    for (uint32_t n = 0; n < ntiles; ++n) {
+        const int buf = n & 1;
+        const uint32_t base = it.k0 + n * kTileKeys;
+        const uint64_t valid = __ballot(slot != kNoCell);
+        const bool more = n + 1 < ntiles;
+        if (more) {
+            fetch(slot_next);
+            slot = slot_next;
+            slot_next = key_slot(a, it, base + 2 * kTileKeys + lane);
+        }
+        // S^T: 64 keys x 32 rows
+        f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(lk[buf] + (kb * 32 + r) * KROW + ks * 32 + h * 16);
+                s[kb] = mma32(kf, qf[ks], s[kb], ty);
+            }
+        // keys: 32 kb + 8 (i / 4) + 4 h + i % 4
+        if (valid != ~0ull || base + kTileKeys > low) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const uint32_t see = (uint32_t(valid >> (32 * kb)) & low_bits(int32_t(min(limit, 0x7FFFFFFFu) - base) - 32 * kb)) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[kb][i] = see & (1u << (8 * (i / 4) + i % 4)) ? s[kb][i] : -INFINITY;
+            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__any((top - m) * c > kLazy || m == -INFINITY)) {
+            const float to = fmaxf(m, top);
+            const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -mc));
+                l += s[kb][i];
+            }
+        // O^T += V^T P^T, 16 keys at a time
+        const uint32_t i16 = lane & 15, gd = (lane >> 4) & 1;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const f32x16& x = s[t / 2];
+            const int i0 = 8 * (t % 2);
+            const u32x4 p = {pack2(x[i0], x[i0 + 1], ty), pack2(x[i0 + 2], x[i0 + 3], ty),
+                             pack2(x[i0 + 4], x[i0 + 5], ty), pack2(x[i0 + 6], x[i0 + 7], ty)};
+            const uint8_t* v = lv[buf] + (16 * t + 4 * h + i16 / 4) * VROW + gd * 32 + (i16 % 4) * 8;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const u32x2 v0 = lds_tr(v + d * 64), v1 = lds_tr(v + 8 * VROW + d * 64);
+                o[d] = mma32(u32x4{v0.x, v0.y, v1.x, v1.y}, p, o[d], ty);
+            }
+        }
+        if (more) stage(buf ^ 1, base + 2 * kTileKeys > block_low);
+        __syncthreads();
+    }
+
+    // V values that were taken out, to the rows that see them
+    if (odd) {
+        const uint32_t skip = block_low > it.k0 ? (block_low - it.k0) / kTileKeys * kTileKeys : 0u;
+        for (uint32_t key = it.k0 + skip; key < it.k1; ++key) {
+            const uint32_t sl = key < limit ? key_slot(a, it, key) : kNoCell;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 x = not_finite(value4<T, FP8>(a, sl, head_off, uint32_t(d * 32 + 8 * i) + 4 * h), ty);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[d][4 * i + j] += x[j];
+                }
+        }
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    settle(m, l, seen != 0);
+    if (!has) return;
+    const float vs = a.v_scale ? *a.v_scale : 1.0f;
+    const float inv = l > 0.0f ? vs / l : l == l ? 0.0f : l;
+    if (!a.direct && h == 0) {
+        const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(token) * a.heads + head;
+        *as_global(a.ws_ml + at) = f32x2{m == -INFINITY ? -INFINITY : m * c, l};
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f32x4 x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            if (l == 0.0f) x = f32x4{0, 0, 0, 0};
+            emit4<T>(a, it, token, head, uint32_t(d * 32 + 8 * i) + 4 * h, x, inv);
+        }
+}
+
+// ------------------------------------------------------------- stream kernel
+// 16 rows against a run of keys that the block's four waves share out, 32 keys
+// at a time: for the few rows of a request that decodes, bound by reading K and
+// V.  A wave works alone until the end (its V in a part of LDS of its own, its
+// maximum and sum its own), then the four results are joined.
+template <class T, bool FP8, int DP>
+__global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
+    constexpr int KS = DP / 32, DB = DP / 16;
+    constexpr int VROW = DP * 2 + 32;
+    constexpr int CH = DP / (FP8 ? 16 : 8);
+    constexpr int PER = (kStreamKeys * CH + 63) / 64;
+    constexpr int VBYTES = kStreamKeys * VROW, OBYTES = kStreamRows * DP * 4;
+    constexpr int WBYTES = VBYTES > OBYTES ? VBYTES : OBYTES;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4][WBYTES];
+    __shared__ float lm[4][kStreamRows], ll[4][kStreamRows];
+
+    const Item it = make_item<true>(a, blockIdx.x);
+    if (!it.live) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t r = lane & 15, g = lane >> 4;
+    T* const ty = nullptr;
+    uint8_t* const lv = lds[wave];
+
+    const uint32_t row = it.row0 + r;
+    const bool has = row < it.rows;
+    const uint32_t token = it.t0 + (has ? row / a.group : 0u);
+    const uint32_t head = it.head * a.group + (has ? row % a.group : 0u);
+    // rows that are not there, and rows that see nothing, ask for no mask
+    const uint32_t seen = has ? seen_by(a, a.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
+    // 0 would make NaN of a masked score; a negative one goes to the query
+    const float c0 = score_factor(a);
+    const uint32_t sign = c0 < 0.0f ? 0x80008000u : 0u;
+    u32x4 qf[KS];
+    {
+        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, uint32_t(s * 32) + g * 8) ^ sign;
+    }
+    uint32_t low = limit;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
+    low = __builtin_amdgcn_readfirstlane(low);
+
+    const float c = fabsf(c0);
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
+
+    const uint32_t row_bytes = a.token_bytes / a.kv_heads, head_off = it.head * row_bytes;
+    u32x4 xv[PER];
+    u32x4 xk[2][KS];                                      // fp8: 8 bytes of each
+    auto fetch = [&](uint32_t slot) {                     // slot: of the keys lane % 32
+        const uint32_t inside = anew(row_bytes);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const uint32_t s = uint32_t(__shfl(int(slot), int(kb * 16 + r), 64));
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t d = ks * 32 + g * 8;
+                if constexpr (FP8) {
+                    const u32x2 v = *as_global(reinterpret_cast<const u32x2*>(chunk_at(a, s, head_off + d, d < inside)));
+                    xk[kb][ks].x = v.x;
+                    xk[kb][ks].y = v.y;
+                } else {
+                    xk[kb][ks] = ld16(chunk_at(a, s, head_off + d * 2, d * 2 < inside));
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t idx = i * 64 + lane, key = idx / CH, ch = idx % CH;
+            const uint32_t s = uint32_t(__shfl(int(slot), int(key & 31), 64));
+            const bool in = ch * 16 < inside && key < uint32_t(kStreamKeys);
+            xv[i] = ld16(chunk_at(a, s, a.token_bytes + head_off + ch * 16, in));
+        }
+    };
+    auto scrub = [&](u32x4& v) {
+        const uint32_t e = exponent_bits(ty);
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t w = v[j];
+            if ((w & e) == e) w &= 0xFFFF0000u, bad = true;
+            if (((w >> 16) & e) == e) w &= 0x0000FFFFu, bad = true;
+            v[j] = w;
+        }
+        return bad;
+    };
+
+    const uint32_t nblk = (it.k1 - it.k0 + kStreamKeys - 1) / kStreamKeys;
+    bool odd = false;
+    uint32_t slot = kNoCell, slot_next = kNoCell;
+    if (wave < nblk) {
+        slot = key_slot(a, it, it.k0 + wave * kStreamKeys + (lane & 31));
+        fetch(slot);
+        slot_next = key_slot(a, it, it.k0 + (wave + 4) * kStreamKeys + (lane & 31));
+    }
+    for (uint32_t n = wave; n < nblk; n += 4) {
+        const uint32_t base = it.k0 + n * kStreamKeys;
+        const uint32_t valid = uint32_t(__ballot(slot != kNoCell));
+        const bool careful = base + kStreamKeys > low;
+        // V to LDS; the reads of the block before have all been waited for by
+        // its products, and a wave's LDS operations keep their order
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t idx = i * 64 + lane, key = idx / CH, ch = idx % CH;
+            if (kStreamKeys * CH % 64 && key >= uint32_t(kStreamKeys)) break;
+            uint8_t* pv = lv + key * VROW;
+            if constexpr (FP8) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const u32x2 v0 = fp8_widen(xv[i][2 * j], ty), v1 = fp8_widen(xv[i][2 * j + 1], ty);
+                    u32x4 v = {v0.x, v0.y, v1.x, v1.y};
+                    if (careful) odd |= scrub(v);
+                    *reinterpret_cast<u32x4*>(pv + ch * 32 + j * 16) = v;
+                }
+            } else {
+                u32x4 v = xv[i];
+                if (careful) odd |= scrub(v);
+                *reinterpret_cast<u32x4*>(pv + ch * 16) = v;
+            }
+        }
+        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                u32x4 kf = xk[kb][ks];
+                if constexpr (FP8) {
+                    const u32x2 k0 = fp8_widen(kf.x, ty), k1 = fp8_widen(kf.y, ty);
+                    kf = u32x4{k0.x, k0.y, k1.x, k1.y};
+                }
+                s[kb] = mma16(kf, qf[ks], s[kb], ty);
+            }
+        if (n + 4 < nblk) {
+            fetch(slot_next);
+            slot = slot_next;
+            slot_next = key_slot(a, it, base + 8 * kStreamKeys + (lane & 31));
+        }
+        // keys: 16 kb + 4 g + i
+        if (valid != 0xFFFFFFFFu || careful) {
+            const uint32_t see = (valid & low_bits(int32_t(min(limit, 0x7FFFFFFFu) - base))) >> (4 * g);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[kb][i] = see & (1u << (kb * 16 + i)) ? s[kb][i] : -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__any((top - m) * c > kLazy || m == -INFINITY)) {
+            const float to = fmaxf(m, top);
+            const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= f;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], c, -mc));
+            l += s[i / 4][i % 4];
+        }
+        // sum over keys 4 g .. and 16 + 4 g .. : what the lane's scores are of
+        const u32x4 p = {pack2(s[0][0], s[0][1], ty), pack2(s[0][2], s[0][3], ty), pack2(s[1][0], s[1][1], ty),
+                         pack2(s[1][2], s[1][3], ty)};
+        const uint8_t* v = lv + (4 * g + r / 4) * VROW + (r % 4) * 8;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const u32x2 v0 = lds_tr(v + d * 32), v1 = lds_tr(v + 16 * VROW + d * 32);
+            o[d] = mma16(u32x4{v0.x, v0.y, v1.x, v1.y}, p, o[d], ty);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // V values that were taken out, to the rows that see them
+    if (__any(odd)) {
+        for (uint32_t n = wave; n < nblk; n += 4) {
+            const uint32_t base = it.k0 + n * kStreamKeys;
+            if (base + kStreamKeys <= low) continue;
+            for (uint32_t key = base; key < min(base + kStreamKeys, it.k1); ++key) {
+                const uint32_t sl = key < limit ? key_slot(a, it, key) : kNoCell;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    o[d] += not_finite(value4<T, FP8>(a, sl, head_off, uint32_t(d * 16) + 4 * g), ty);
+            }
+        }
+    }
+
+    // the four waves' results: brought to one maximum, summed over LDS
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    settle(m, l, seen != 0);
+    if (g == 0) {
+        lm[wave][r] = m;
+        ll[wave][r] = l;
+    }
+    __syncthreads();
+    const float top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
+    auto factor = [&](float x) { return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x - top) * c); };
+    const float f = factor(m);
+    float* lo = reinterpret_cast<float*>(lds[wave]);      // [row][dim]
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        f32x4 x = o[d] * f;
+        if (m == -INFINITY) x = f32x4{0, 0, 0, 0};
+        *reinterpret_cast<f32x4*>(lo + r * DP + d * 16 + 4 * g) = x;
+    }
+    __syncthreads();
+    const float vs = a.v_scale ? *a.v_scale : 1.0f;
+    for (uint32_t e = tid; e < uint32_t(kStreamRows) * (DP / 4); e += kAB) {
+        const uint32_t rr = e / (DP / 4), d = e % (DP / 4) * 4;
+        const uint32_t rw = it.row0 + rr;
+        if (rw >= it.rows) continue;
+        f32x4 x = {0, 0, 0, 0};
+        float sum = 0.0f, mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) + rr * DP + d);
+            mx = fmaxf(mx, lm[w][rr]);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            sum += lm[w][rr] == -INFINITY ? 0.0f : ll[w][rr] * __builtin_amdgcn_exp2f((lm[w][rr] - mx) * c);
+        const uint32_t tk = it.t0 + rw / a.group, hd = it.head * a.group + rw % a.group;
+        if (!a.direct && d == 0) {
+            const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(tk) * a.heads + hd;
+            *as_global(a.ws_ml + at) = f32x2{mx == -INFINITY ? -INFINITY : mx * c, sum};
+        }
+        emit4<T>(a, it, tk, hd, d, x, sum > 0.0f ? vs / sum : sum == sum ? 0.0f : sum);
+    }
+}
+
+// Partial results of a row brought to one maximum, summed, divided and rounded.
+template <class T>
+__global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lanes) {
+    const uint32_t row = (blockIdx.x * kAB + threadIdx.x) / lanes, d = (threadIdx.x % lanes) * 4;
+    const uint32_t rows = a.tokens * a.heads;
+    if (row >= rows || row / a.heads >= live_tokens(a) || d >= a.dim) return;
+    const uint32_t parts = a.parts_flat + a.parts_own;
+    float top = -INFINITY;
+    for (uint32_t p = 0; p < parts; ++p) top = fmaxf(top, as_global(a.ws_ml)[uint64_t(p) * rows + row].x);
+    f32x4 o = {0, 0, 0, 0};
+    float l = 0.0f;
+    for (uint32_t p = 0; p < parts; ++p) {
+        const uint64_t at = uint64_t(p) * rows + row;
+        const f32x2 ml = as_global(a.ws_ml)[at];
+        if (ml.x == -INFINITY) continue;                  // nothing seen there
+        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        l += ml.y * f;
+        o += *as_global(reinterpret_cast<const f32x4*>(a.ws_o + at * a.dim + d)) * f;
+    }
+    const float vs = a.v_scale ? *a.v_scale : 1.0f;
+    const float inv = l > 0.0f ? vs / l : l == l ? 0.0f : l;
+    store4(reinterpret_cast<T*>(a.out) + int64_t(row / a.heads) * a.os + int64_t(row % a.heads) * a.oh + d, o * inv,
+           a.wide_o);
+}
+
+typedef void (*AttnFn)(AttnArgs);
+
+template <class T, bool FP8>
+AttnFn pick_attn(bool stream, int dim) {
+    if (stream)
+        return dim <= 64    ? &attn_stream_kernel<T, FP8, 64>
+               : dim <= 96  ? &attn_stream_kernel<T, FP8, 96>
+               : dim <= 128 ? &attn_stream_kernel<T, FP8, 128>
+                            : &attn_stream_kernel<T, FP8, 256>;
+    return dim <= 64    ? &attn_tile_kernel<T, FP8, 64>
+           : dim <= 96  ? &attn_tile_kernel<T, FP8, 96>
+           : dim <= 128 ? &attn_tile_kernel<T, FP8, 128>
+                        : &attn_tile_kernel<T, FP8, 256>;
+}
+
+struct AttnPlan {
+    bool flat, flat_stream, own_stream;
+    uint32_t parts_flat, parts_own, flat_tiles, own_tiles, req_tiles, first;
+    uint64_t rows;
+    bool direct() const { return parts_flat + parts_own == 1; }
+    int64_t bytes(int64_t dim) const {
+        return direct() ? 0 : int64_t(uint64_t(parts_flat + parts_own) * rows * (uint64_t(dim) * 4 + 8)) + 16;
+    }
+};
+
+// Which kernel takes which part, and in how many splits of the keys.
+inline AttnPlan plan_attention(const kvec_attention* s) {
+    AttnPlan p{};
+    const uint64_t group = uint64_t(s->heads / s->kv_heads), N = uint64_t(s->tokens);
+    const uint64_t max_q = s->cu_q ? uint64_t(s->max_q) : 1;
+    p.rows = N * uint64_t(s->heads);
+    const uint64_t req_rows = max_q * group, all_rows = N * group;
+    const uint64_t prefix = uint64_t(s->prefix);
+    // Requests that fill tiles by themselves read the prefix with their own
+    // keys: no partial results to write and join.
+    p.own_stream = req_rows <= 4 * kStreamRows;
+    p.flat = prefix > 0 && req_rows < uint64_t(kTileRows);
+    p.first = p.flat ? uint32_t(prefix) : 0;
+    p.flat_stream = all_rows <= 2 * kStreamRows;
+    auto splits = [](uint64_t blocks, uint64_t want, uint64_t keys, uint64_t least) {
+        uint64_t n = (want + blocks - 1) / (blocks ? blocks : 1);
+        const uint64_t most = (keys + least - 1) / least;
+        if (n > most) n = most;
+        return uint32_t(n < 1 ? 1 : n > 256 ? 256 : n);
+    };
+    if (p.flat) {
+        const uint64_t bm = p.flat_stream ? kStreamRows : kTileRows;
+        p.flat_tiles = uint32_t((all_rows + bm - 1) / bm);
+        p.parts_flat = splits(uint64_t(p.flat_tiles) * s->kv_heads, 512, prefix, 256);
+    }
+    if (p.own_stream) {
+        p.req_tiles = uint32_t((req_rows + kStreamRows - 1) / kStreamRows);
+        p.own_tiles = uint32_t(s->batch) * p.req_tiles;
+    } else {
+        p.own_tiles = uint32_t(all_rows / kTileRows) + uint32_t(s->batch);
+    }
+    const int64_t cap = int64_t(s->pages_per_seq) * s->page_tokens;
+    const int64_t len = s->max_len > 0 && s->max_len < cap ? s->max_len : cap;
+    const uint64_t own_keys = len > int64_t(p.first) ? uint64_t(len) - p.first : 1;
+    p.parts_own = splits(uint64_t(p.own_tiles) * s->kv_heads, p.own_stream ? 768 : 512, own_keys, 256);
+    return p;
+}
+
+inline int check_attention(const kvec_attention* s, const char* fn) {
+    if (!s) return set_error(KVEC_EINVAL, "%s: null descriptor", fn);
+    if (s->tokens < 0 || s->batch < 0 || s->heads < 1 || s->kv_heads < 1 || s->heads % s->kv_heads || s->dim < 1 ||
+        s->pages_per_seq < 1 || s->pool_pages < 0 || s->prefix < 0)
+        return set_error(KVEC_EINVAL, "%s: bad sizes", fn);
+    if (s->dtype != KVEC_BF16 && s->dtype != KVEC_F16) return set_error(KVEC_EINVAL, "%s: dtype %d", fn, s->dtype);
+    if (s->pool_dtype != s->dtype && s->pool_dtype != KVEC_FP8_E4M3)
+        return set_error(KVEC_EINVAL, "%s: pool_dtype %d is neither dtype nor fp8", fn, s->pool_dtype);
+    if (s->pool_dtype == s->dtype && (s->k_scale || s->v_scale))
+        return set_error(KVEC_EINVAL, "%s: scales are an fp8 pool's", fn);
+    const int unit = s->pool_dtype == KVEC_FP8_E4M3 ? 16 : 8;
+    if (s->dim > 256 || s->dim % unit)
+        return set_error(KVEC_EUNSUPPORTED, "%s: dim=%d must be a multiple of %d up to 256", fn, s->dim, unit);
+    if (s->page_tokens < 1 || (s->page_tokens & (s->page_tokens - 1)))
+        return set_error(KVEC_EINVAL, "%s: page_tokens=%d must be a power of two", fn, s->page_tokens);
+    if (s->pool_pages > (int64_t(1) << 31) / s->page_tokens ||
+        int64_t(s->pages_per_seq) * s->page_tokens >= (int64_t(1) << 31) - 1024)
+        return set_error(KVEC_EUNSUPPORTED, "%s: positions or slots past 2^31", fn);
+    if (s->prefix > int64_t(s->pages_per_seq) * s->page_tokens)
+        return set_error(KVEC_EINVAL, "%s: prefix=%lld past the page table", fn, (long long)s->prefix);
+    if (s->cu_q ? s->max_q < 1 && s->tokens > 0 : s->tokens != s->batch)
+        return set_error(KVEC_EINVAL, "%s: max_q=%d tokens=%lld batch=%d", fn, s->max_q, (long long)s->tokens, s->batch);
+    if (!(s->scale >= 0.0f) || s->scale > 3e38f) return set_error(KVEC_EINVAL, "%s: scale must be finite and not negative", fn);
+    if (s->tokens * s->heads >= (int64_t(1) << 31) / 64 || int64_t(s->batch) * s->pages_per_seq >= (int64_t(1) << 31))
+        return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
+    return KVEC_OK;
+}
+
+}  // namespace kvec
+
+using namespace kvec;
+
+extern "C" int64_t kvec_prefix_attention_workspace(const kvec_attention* s) {
+    if (check_attention(s, "kvec_prefix_attention_workspace")) return -1;
+    if (s->tokens == 0 || s->batch == 0) return 0;
+    return plan_attention(s).bytes(s->dim);
+}
+
+extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, int64_t workspace_bytes, void* stream) {
+    static const char* fn = "kvec_prefix_attention";
+    int rc = check_attention(s, fn);
+    if (rc) return rc;
+    if (s->tokens == 0 || s->batch == 0) return KVEC_OK;
+    if (!s->q || !s->out || !s->pool || !s->page_table || !s->seq_lens || (s->prefix && !s->prefix_pages))
+        return set_error(KVEC_EINVAL, "%s: null array", fn);
+    if (!aligned16(s->pool)) return set_error(KVEC_EINVAL, "%s: pool not 16-byte aligned", fn);
+    const int64_t str[4] = {s->q_stride, s->q_head_stride, s->o_stride, s->o_head_stride};
+    for (int64_t x : str)
+        if (x < 0 || x > (int64_t(1) << 40)) return set_error(KVEC_EINVAL, "%s: stride %lld", fn, (long long)x);
+    if ((s->heads > 1 && s->o_head_stride < s->dim) || (s->tokens > 1 && s->o_stride < s->dim))
+        return set_error(KVEC_EINVAL, "%s: rows of out overlap", fn);
+    const AttnPlan p = plan_attention(s);
+    const int64_t need = p.bytes(s->dim);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return set_error(KVEC_EINVAL, "%s: workspace of %lld bytes, 16-byte aligned, wanted", fn, (long long)need);
+    const int64_t ps = type_bytes(s->pool_dtype);
+    const uint64_t rec = 2 * uint64_t(s->kv_heads) * uint64_t(s->dim) * uint64_t(ps);
+    if (rec / 2 >= (uint64_t(1) << 30)) return set_error(KVEC_EUNSUPPORTED, "%s: token record too large", fn);
+    {
+        auto span = [&](const void* q, int64_t st, int64_t hs, const char* name) {
+            return Span{q, uint64_t((s->tokens - 1) * st + (s->heads - 1) * hs + s->dim) * 2, name, -1};
+        };
+        const Span w[2] = {span(s->out, s->o_stride, s->o_head_stride, "out"),
+                           {workspace, uint64_t(need), "workspace", -1}};
+        const Span r[6] = {span(s->q, s->q_stride, s->q_head_stride, "q"),
+                           {s->pool, uint64_t(s->pool_pages) * uint64_t(s->page_tokens) * rec, "pool", -1},
+                           {s->page_table, uint64_t(s->batch) * uint64_t(s->pages_per_seq) * 4, "page_table", -1},
+                           {s->seq_lens, uint64_t(s->batch) * 4, "seq_lens", -1},
+                           {s->cu_q, s->cu_q ? uint64_t(s->batch + 1) * 4 : 0, "cu_q", -1},
+                           {s->prefix_pages,
+                            s->prefix ? uint64_t((s->prefix + s->page_tokens - 1) / s->page_tokens) * 4 : 0,
+                            "prefix_pages", -1}};
+        if ((rc = check_no_alias(w, 2, r, 6, fn))) return rc;
+    }
+    AttnArgs a{};
+    a.q = (const uint8_t*)s->q;
+    a.out = (uint8_t*)s->out;
+    a.qs = s->q_stride, a.qh = s->q_head_stride, a.os = s->o_stride, a.oh = s->o_head_stride;
+    a.pool = (const uint8_t*)s->pool;
+    a.table = s->page_table;
+    a.prefix_pages = s->prefix_pages;
+    a.seq_lens = s->seq_lens;
+    a.cu = s->cu_q;
+    a.k_scale = s->k_scale;
+    a.v_scale = s->v_scale;
+    a.rec = rec;
+    a.token_bytes = uint32_t(rec / 2);
+    a.tokens = uint32_t(s->tokens);
+    a.batch = uint32_t(s->batch);
+    a.heads = uint32_t(s->heads);
+    a.kv_heads = uint32_t(s->kv_heads);
+    a.group = a.heads / a.kv_heads;
+    a.dim = uint32_t(s->dim);
+    a.width = uint32_t(s->pages_per_seq);
+    while ((1 << a.shift) < s->page_tokens) ++a.shift;
+    a.pool_pages = uint32_t(s->pool_pages);
+    a.cap = a.width << a.shift;
+    a.prefix = uint32_t(s->prefix);
+    a.first = p.first;
+    a.parts_flat = p.parts_flat;
+    a.parts_own = p.parts_own;
+    a.req_tiles = p.req_tiles;
+    a.direct = p.direct();
+    a.scale = s->scale;
+    a.wide_q = aligned16(s->q) && s->q_stride % 8 == 0 && s->q_head_stride % 8 == 0;
+    a.wide_o = aligned16(s->out) && s->o_stride % 8 == 0 && s->o_head_stride % 8 == 0;
+    if (need) {
+        a.ws_o = (float*)workspace;
+        a.ws_ml = (f32x2*)((uint8_t*)workspace + uint64_t(p.parts_flat + p.parts_own) * p.rows * uint64_t(s->dim) * 4);
+    }
+    const bool fp8 = s->pool_dtype == KVEC_FP8_E4M3, bf = s->dtype == KVEC_BF16;
+    auto pick = [&](bool st) {
+        return bf ? (fp8 ? pick_attn<__bf16, true>(st, s->dim) : pick_attn<__bf16, false>(st, s->dim))
+                  : (fp8 ? pick_attn<_Float16, true>(st, s->dim) : pick_attn<_Float16, false>(st, s->dim));
+    };
+    auto launch = [&](bool flat) {
+        AttnArgs x = a;
+        x.flat = flat;
+        x.tiles = flat ? p.flat_tiles : p.own_tiles;
+        const uint64_t blocks = uint64_t(x.tiles) * x.kv_heads * (flat ? x.parts_flat : x.parts_own);
+        if (blocks >= (uint64_t(1) << 31)) return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks", fn);
+        hipLaunchKernelGGL(pick(flat ? p.flat_stream : p.own_stream), dim3(unsigned(blocks)), dim3(kAB), 0,
+                           as_stream(stream), x);
+        return check_launch(fn);
+    };
+    if (p.flat && (rc = launch(true))) return rc;
+    if ((rc = launch(false))) return rc;
+    if (p.direct()) return KVEC_OK;
+    uint32_t lanes = 16;
+    while (lanes * 4 < a.dim) lanes *= 2;
+    const uint64_t threads = uint64_t(a.tokens) * a.heads * lanes;
+    if (bf) hipLaunchKernelGGL(attn_join_kernel<__bf16>, dim3(blocks_for(int64_t(threads), kAB)), dim3(kAB), 0, as_stream(stream), a, lanes);
+    else hipLaunchKernelGGL(attn_join_kernel<_Float16>, dim3(blocks_for(int64_t(threads), kAB)), dim3(kAB), 0, as_stream(stream), a, lanes);
+    return check_launch(fn);
+}

@@ -41,7 +41,8 @@ extern "C" {
  * 1.0.0: kvec_rdp_encode / kvec_rdp_decode / kvec_rdp_encode_paged take
  * unit_bytes, kvec_chunk_stripe has region_off and unit_bytes (0.1.0 had
  * neither).  1.1.0: kvec_hook_step added.  1.2.0: the *_kv entry points over
- * kvec_kv_bhtd added.  1.3.0: kvec_step_tables, kvec_norm_rotate_write added. */
+ * kvec_kv_bhtd added.  1.3.0: kvec_step_tables, kvec_norm_rotate_write,
+ * kvec_prefix_attention added. */
 #define KVEC_VERSION 10300
 int kvec_version(void);
 /* Static description of a KVEC_E* code. */
@@ -454,6 +455,47 @@ typedef struct kvec_norm_rotate {
     const int32_t* n_tokens;    /* [1], device, or NULL: all */
 } kvec_norm_rotate;
 int kvec_norm_rotate_write(const kvec_norm_rotate* step, void* stream);
+
+/* Attention of a step's queries over one layer of the pool, for requests that
+ * share their first `prefix` positions (0: none).  Token i of request b's n_b
+ * (cu_q[b] .. cu_q[b+1] - 1; cu_q NULL: one token a request) is at position
+ * seq_lens[b] - n_b + i and sees the positions up to its own: below `prefix` on
+ * the pages of prefix_pages, from there on those of its page table row.  Keys on
+ * pages outside [0, pool_pages) and past the row are left out; a query that
+ * sees none gives zeros.  Tokens from cu_q[batch] on are left as they were.
+ * out = softmax(scale * q.k) v by query head; head h reads K/V head
+ * h / (heads / kv_heads).  fp8 K and V stand for value * scale.
+ * max_q: the most tokens that a request has (more of them are not computed);
+ * max_len: about the longest seq_lens (0: pages_per_seq * page_tokens), which
+ * only decides how the work is split.  dim: a multiple of 8 (fp8 pool: 16) up to
+ * 256.  workspace: kvec_prefix_attention_workspace bytes, 16-byte aligned (0:
+ * may be NULL), not to be used by another call at the same time. */
+typedef struct kvec_attention {
+    int64_t tokens;
+    int batch, heads, kv_heads, dim;
+    int dtype;                  /* of q and out: KVEC_BF16, KVEC_F16 */
+    const void* q;              /* strides in elements, each head's values adjacent */
+    int64_t q_stride, q_head_stride;
+    void* out;
+    int64_t o_stride, o_head_stride;
+    const void* pool;           /* the layer: [pool_pages][page_tokens][2 (K,V)][kv_heads][dim] */
+    int pool_dtype;             /* dtype, or KVEC_FP8_E4M3 */
+    int64_t pool_pages;
+    int page_tokens;            /* a power of two */
+    const int32_t* page_table;  /* device [batch][pages_per_seq] */
+    int pages_per_seq;
+    const int32_t* seq_lens;    /* device [batch] */
+    const int32_t* cu_q;        /* device [batch + 1], or NULL */
+    int max_q;
+    int64_t max_len;
+    int64_t prefix;
+    const int32_t* prefix_pages; /* device [ceil(prefix / page_tokens)] */
+    float scale;                /* not negative */
+    const float* k_scale;       /* [1] each, device, or NULL: 1 */
+    const float* v_scale;
+} kvec_attention;
+int64_t kvec_prefix_attention_workspace(const kvec_attention* call);
+int kvec_prefix_attention(const kvec_attention* call, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

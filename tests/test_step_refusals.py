@@ -119,3 +119,83 @@ def test_rotary_helpers(pkg):
             pkg.attention.rotary_frequencies(bad, device="cpu")
     with pytest.raises(ValueError):
         pkg.attention.rotary_axes([1, -1], device="cpu")
+
+
+def at(pkg, **kw):
+    f = dict(tokens=4, batch=4, heads=8, kv_heads=2, dim=64, dtype=1, q=1 << 20, q_stride=512, q_head_stride=64,
+             out=1 << 21, o_stride=512, o_head_stride=64, pool=1 << 22, pool_dtype=1, pool_pages=50, page_tokens=16,
+             page_table=1 << 23, pages_per_seq=8, seq_lens=1 << 24, max_q=1, prefix=20, prefix_pages=1 << 25,
+             scale=0.125)
+    f.update(kw)
+    return pkg._lib.Attention(**f)
+
+
+@pytest.mark.parametrize("bad,code,word", [
+    ({"tokens": -1}, -1, b"sizes"),
+    ({"heads": 7}, -1, b"sizes"),
+    ({"prefix": -1}, -1, b"sizes"),
+    ({"dtype": 0}, -1, b"dtype"),
+    ({"pool_dtype": 2}, -1, b"pool_dtype"),
+    ({"v_scale": 1 << 28}, -1, b"scales"),
+    ({"dim": 264}, -2, b"dim"),
+    ({"dim": 60}, -2, b"dim"),
+    ({"dim": 72, "pool_dtype": 3}, -2, b"dim"),
+    ({"page_tokens": 24}, -1, b"power of two"),
+    ({"pool_pages": 1 << 28}, -2, b"2^31"),
+    ({"pages_per_seq": 1 << 27}, -2, b"2^31"),
+    ({"prefix": 129}, -1, b"prefix"),
+    ({"tokens": 5}, -1, b"max_q"),
+    ({"cu_q": 1 << 26, "max_q": 0}, -1, b"max_q"),
+    ({"scale": -0.5}, -1, b"scale"),
+    ({"scale": float("nan")}, -1, b"scale"),
+    ({"scale": float("inf")}, -1, b"scale"),
+    ({"tokens": 1 << 23, "batch": 1 << 23}, -2, b"rows"),
+])
+def test_attention_refuses(pkg, bad, code, word):
+    L = pkg._lib.lib()
+    assert L.kvec_prefix_attention(C.byref(at(pkg, **bad)), 1 << 30, 1 << 30, None) == code
+    assert word in L.kvec_last_error()
+    assert L.kvec_prefix_attention_workspace(C.byref(at(pkg, **bad))) == -1
+
+
+@pytest.mark.parametrize("bad,word", [
+    ({"q": None}, b"null"),
+    ({"prefix_pages": None}, b"null"),
+    ({"seq_lens": None}, b"null"),
+    ({"pool": (1 << 22) + 8}, b"aligned"),
+    ({"q_stride": -1}, b"stride"),
+    ({"o_head_stride": 32}, b"overlap"),
+    ({"out": 1 << 20}, b"overlaps"),
+    ({"out": 1 << 22}, b"overlaps"),
+])
+def test_attention_refuses_arrays(pkg, bad, word):
+    L = pkg._lib.lib()
+    assert L.kvec_prefix_attention(C.byref(at(pkg, **bad)), 1 << 30, 1 << 30, None) == -1
+    assert word in L.kvec_last_error()
+
+
+def test_attention_workspace(pkg):
+    L = pkg._lib.lib()
+    call = at(pkg)
+    need = L.kvec_prefix_attention_workspace(C.byref(call))
+    assert need >= 2 * 32 * (64 * 4 + 8)               # two parts of 32 rows at least
+    for ws, n in ((None, need), (1 << 30, need - 1), ((1 << 30) + 8, need)):
+        assert L.kvec_prefix_attention(C.byref(call), ws, n, None) == -1
+        assert b"workspace" in L.kvec_last_error()
+    assert L.kvec_prefix_attention_workspace(C.byref(at(pkg, tokens=0, batch=0))) == 0
+    assert L.kvec_prefix_attention(C.byref(at(pkg, tokens=0, batch=0, q=None)), None, 0, None) == 0
+
+
+def test_attention_python_refusals(pkg):
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    q, pool = torch.zeros(4, 8, 64, dtype=torch.half), torch.zeros(1, 8, 16, 2, 2, 64, dtype=torch.half)
+    with pytest.raises(ValueError, match="GPU"):
+        pkg.attention.prefix_attention(q, pool, i(4, 3), i(4))
+    with pytest.raises(ValueError, match="bfloat16 or float16"):
+        pkg.attention.prefix_attention(q.float(), pool, i(4, 3), i(4))
+    with pytest.raises(ValueError, match="seq_lens"):
+        pkg.attention.prefix_attention(q, pool, i(4, 3), i(3))
+    with pytest.raises(ValueError, match="one query token"):
+        pkg.attention.prefix_attention(q[:3], pool, i(4, 3), i(4))
+    with pytest.raises(ValueError, match="int32"):
+        pkg.attention.prefix_attention(q, pool, i(4, 3).long(), i(4))
