@@ -36,7 +36,7 @@ namespace kvec {
 
 constexpr int kAB = 256;                       // threads of a block: 4 waves
 constexpr int kTileRows = 128;                 // rows of a tile block, 32 a wave
-constexpr int kTileKeys = 64;
+constexpr int kTileKeys = 32;
 constexpr int kStreamRows = 16;                // rows of a stream block
 constexpr int kStreamKeys = 32;                // keys a wave takes at a time
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -78,6 +78,20 @@ __device__ __forceinline__ u32x2 fp8_widen(uint32_t v, __bf16*) {
 __device__ __forceinline__ u32x2 fp8_widen(uint32_t v, _Float16*) {
     return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true))};
+}
+
+// The larger of the two lane halves' values, in both.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// c plus the sum of two 16-bit values.
+__device__ __forceinline__ float add2(uint32_t v, float c, __bf16*) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{__bf16(1.0f), __bf16(1.0f)}, c, false);
+}
+__device__ __forceinline__ float add2(uint32_t v, float c, _Float16*) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), f16x2{_Float16(1.0f), _Float16(1.0f)}, c, false);
 }
 
 // Whether a 16-bit value is infinite or NaN: all its exponent bits are set.
@@ -122,8 +136,7 @@ struct AttnArgs {
     const float *k_scale, *v_scale;
     float* ws_o;                               // [parts][rows][dim]
     f32x2* ws_ml;                              // [parts][rows]: maximum (powers of two), sum
-    uint64_t rec;                              // bytes of a token record
-    uint32_t token_bytes;
+    uint32_t rec, token_bytes;                 // bytes of a token record, of its K
     uint32_t tokens, batch, heads, kv_heads, group, dim;
     uint32_t width, shift, pool_pages, cap;    // cap: positions that a table row covers
     uint32_t prefix;                           // keys of the shared part (0: none)
@@ -172,13 +185,58 @@ struct Item {
     uint32_t k0, k1;
 };
 
+// Row tiles of the requests before each, for the tile kernel's own keys: the
+// request of tile `tile` and the first of its tiles; past the last one, the number
+// of all tiles in `first` and batch in `b`.  A wave sums 64 requests at a time.
+struct TileAt {
+    uint32_t b, first;
+};
+__device__ __forceinline__ uint32_t tiles_of(const AttnArgs& a, uint32_t b) {
+    const uint32_t t0 = first_token(a, b), t1 = min(first_token(a, b + 1), a.tokens);
+    return t1 > t0 ? uint32_t((uint64_t(t1 - t0) * a.group + kTileRows - 1) / kTileRows) : 0u;
+}
+__device__ __forceinline__ TileAt tile_at(const AttnArgs& a, uint32_t tile) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        const uint32_t b = b0 + lane, n = b < a.batch ? tiles_of(a, b) : 0u;
+        uint32_t x = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t y = uint32_t(__shfl_up(int(x), d, 64));
+            if (lane >= uint32_t(d)) x += y;
+        }
+        const uint64_t past = __ballot(before + x > tile);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            return TileAt{b0 + uint32_t(at), before + uint32_t(__shfl(int(x - n), at, 64))};
+        }
+        before += uint32_t(__shfl(int(x), 63, 64));
+    }
+    return TileAt{a.batch, before};
+}
+
 template <bool STREAM>
 __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     constexpr uint32_t BM = STREAM ? kStreamRows : kTileRows;
     constexpr uint32_t KEYS = STREAM ? 4 * kStreamKeys : kTileKeys;
     Item it{};
     const uint32_t parts = a.flat ? a.parts_flat : a.parts_own;
-    const uint32_t tile = id % a.tiles, rest = id / a.tiles;
+    uint32_t tiles = a.tiles;
+    if (!STREAM && !a.flat) {
+        // as many tiles as there are, not the launch's bound: blocks without
+        // work come last then, and no compute unit gets a third block for them
+        tiles = __builtin_amdgcn_readfirstlane(tile_at(a, 0xFFFFFFFFu).first);
+        if (id >= tiles * parts * a.kv_heads) return it;
+    }
+    // Blocks go to the eight XCDs in turn: heads and splits first, so that with
+    // eight K/V heads (and any eighth of the sizes that serve) an XCD's blocks
+    // share their keys in its L2; and the tiles with the most keys, a request's
+    // last ones, before the others (both: 1375 -> 1272 us for 8192 tokens behind
+    // 8192 in four requests).
+    const uint32_t hp = parts * a.kv_heads, rest = id % hp;
+    uint32_t tile = id / hp;
+    if (!STREAM && !a.flat) tile = tiles - 1 - tile;
     const uint32_t split = rest % parts;
     it.head = rest / parts;
     it.part = a.flat ? split : a.parts_flat + split;
@@ -194,16 +252,9 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
             it.b = tile / a.req_tiles;
             local = tile % a.req_tiles;
         } else {
-            // request b's tiles start at floor(cu_b G / BM) + b, at least as far
-            // apart as it has tiles
-            uint32_t lo = 0, hi = a.batch;
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (uint32_t((uint64_t(first_token(a, mid)) * a.group) / BM) + mid <= tile) lo = mid;
-                else hi = mid;
-            }
-            it.b = lo;
-            local = tile - uint32_t((uint64_t(first_token(a, lo)) * a.group) / BM) - lo;
+            const TileAt t = tile_at(a, tile);
+            it.b = __builtin_amdgcn_readfirstlane(t.b);
+            local = tile - __builtin_amdgcn_readfirstlane(t.first);
         }
         it.t0 = first_token(a, it.b);
         const uint32_t t1 = min(first_token(a, it.b + 1), a.tokens);
@@ -225,13 +276,20 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     return it;
 }
 
-// The slot of a key, or kNoCell where there is none.
-__device__ __forceinline__ uint32_t key_slot(const AttnArgs& a, const Item& it, uint32_t pos) {
-    if (pos >= it.k1) return kNoCell;
-    const uint32_t j = pos >> a.shift;
+// The page of a key, as the table has it (of the last key past that: its place
+// is looked at before it is used), and its slot, or kNoCell where there is none.
+// In two steps, so that the table's entry can be on its way for a while.
+__device__ __forceinline__ uint32_t key_page(const AttnArgs& a, const Item& it, uint32_t pos) {
+    pos = min(pos, it.k1 - 1);
     const int32_t* row = a.flat || pos < a.prefix ? a.prefix_pages : a.table + uint64_t(it.b) * a.width;
-    const uint32_t page = uint32_t(row[j]);
-    return page < a.pool_pages ? (page << a.shift) | (pos & ((1u << a.shift) - 1)) : kNoCell;
+    return uint32_t(*as_global(row + (pos >> a.shift)));
+}
+__device__ __forceinline__ uint32_t page_slot(const AttnArgs& a, const Item& it, uint32_t pos, uint32_t page) {
+    const uint32_t slot = (page << a.shift) | (pos & ((1u << a.shift) - 1));
+    return pos < it.k1 && page < a.pool_pages ? slot : kNoCell;
+}
+__device__ __forceinline__ uint32_t key_slot(const AttnArgs& a, const Item& it, uint32_t pos) {
+    return page_slot(a, it, pos, key_page(a, it, pos));
 }
 
 // A 16-byte chunk of a key's K (or V) row, zeros where there is no key.
@@ -248,9 +306,9 @@ __device__ __forceinline__ float score_factor(const AttnArgs& a) {
 // A row's maximum and sum at the end: none for one that sees nothing, and a
 // maximum for a sum that is NaN (all its scores were), so that it is not taken
 // for a row without keys when parts are joined.
-__device__ __forceinline__ void settle(float& m, float& l, bool sees) {
-    if (!sees) m = -INFINITY, l = 0.0f;
-    else if (l != l && m == -INFINITY) m = 0.0f;
+__device__ __forceinline__ f32x2 settle(float m, float l, bool sees) {
+    const float top = l != l && m == -INFINITY ? 0.0f : m;
+    return f32x2{sees ? top : -INFINITY, sees ? l : 0.0f};
 }
 
 // Four values of a key's V row from value d on, zeros where there are none.
@@ -285,9 +343,19 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, bool wide) {
     }
 }
 
+// A kernel's arguments, read from memory again where they are used: what only its
+// end needs is not held in registers over its loop.  (They are the kernel's one
+// argument, so they start its argument segment.)
+typedef const __attribute__((address_space(4))) AttnArgs LateArgs;
+__device__ __forceinline__ LateArgs& late_args() {
+    auto* p = (LateArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+
 // A finished quarter of a row: into the workspace, or the output.
-template <class T>
-__device__ __forceinline__ void emit4(const AttnArgs& a, const Item& it, uint32_t token, uint32_t head, uint32_t d,
+template <class T, class Args>
+__device__ __forceinline__ void emit4(Args& a, const Item& it, uint32_t token, uint32_t head, uint32_t d,
                                       f32x4 o, float inv_l) {
     if (d >= anew(a.dim)) return;
     if (a.direct) {
@@ -300,24 +368,72 @@ __device__ __forceinline__ void emit4(const AttnArgs& a, const Item& it, uint32_
 }
 
 // ------------------------------------------------------------- tile kernel
-// 128 rows against tiles of 64 keys: for rows enough to be bound by the matrix
+// 128 rows against units of 32 keys: for rows enough to be bound by the matrix
 // units.  Each wave owns 32 rows (Q in registers); the four waves share the K
-// and V tiles in LDS, read one tile ahead through registers.  Row strides of K
-// and V in LDS are 16 and 32 bytes past a multiple of the banks, so the 16
-// rows (8 rows of 32 bytes, transposed) that a phase reads lie on all banks.
+// and V units in LDS, a ring of four of each.  A step of the loop forms the
+// scores of unit j + 1 while the vector units turn those of unit j into P, and
+// adds V of unit j; K of unit j + 3 and V of unit j + 2 are on their way from
+// memory meanwhile.  There is a barrier every two steps.  (Scores of 64 keys at a
+// time, both buffers of them, would take the registers past 256, and so one
+// wave a SIMD less.)
+//
+// K and V of the queries' type go to LDS without passing registers: a wave's
+// load puts 64 chunks of 16 bytes there one after another, so rows cannot be
+// padded against bank conflicts, and the chunks of a row are permuted instead
+// (chunk c of key r lies at c ^ swz(r); the lane that loads it picks its source
+// accordingly).  An fp8 pool's values are widened on the way, by register.
+template <int DP>
+struct TileGeom {
+    static constexpr int ROW = DP == 64 ? 128 : DP <= 128 ? 256 : 512;   // bytes of a key's row in LDS
+    static constexpr int POS = ROW / 16;                                 // chunks of it
+    static constexpr int BYTES = kTileKeys * ROW;
+    // 16 lanes read one chunk of 16 keys: all on different banks
+    static __device__ __forceinline__ uint32_t swz_k(uint32_t key) { return DP == 64 ? (key >> 1) & 7 : key & 15; }
+    // 64 lanes read two neighbours of chunks of 8 keys: moved by whole pairs
+    static __device__ __forceinline__ uint32_t swz_v(uint32_t key) {
+        return DP == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
+    }
+};
+
+// 16 bytes a lane from memory to LDS, lane after lane from `to` on (the same for
+// the wave).
+__device__ __forceinline__ void load_to_lds(const uint8_t* from, uint8_t* to) {
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// Says that a condition hardly ever holds (where SAY: at 256 values a head the
+// registers come out worse for it, past what a wave has).
+template <bool SAY>
+__device__ __forceinline__ bool rarely(bool x) {
+    return SAY ? __builtin_expect_with_probability(x, 0, 0.99) : x;
+}
+
+// A barrier of the block after which its LDS holds what was written before and
+// what loads brought.
+__device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);                   // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <class T, bool FP8, int DP>
 __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
+    using G = TileGeom<DP>;
     constexpr int KS = DP / 16, DB = DP / 32;
-    constexpr int KROW = DP * 2 + 16, VROW = DP * 2 + 32;
-    constexpr int CH = DP / (FP8 ? 16 : 8);               // 16-byte chunks of a row in the pool
-    constexpr int PER = (kTileKeys * CH + kAB - 1) / kAB;  // chunks a thread
-    __shared__ __attribute__((aligned(16))) uint8_t lk[2][kTileKeys * KROW];
-    __shared__ __attribute__((aligned(16))) uint8_t lv[2][kTileKeys * VROW];
+    constexpr int CH = FP8 ? DP / 16 : G::POS;             // chunks of a key that are loaded
+    constexpr int PER = (kTileKeys * CH + kAB - 1) / kAB;  // of them by a thread
+    // separate arrays: the compiler can tell their accesses apart, so a read of
+    // one does not wait for a load into another
+    __shared__ __attribute__((aligned(16))) uint8_t k0[G::BYTES], k1[G::BYTES], k2[G::BYTES], k3[G::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t v0[G::BYTES], v1[G::BYTES], v2[G::BYTES], v3[G::BYTES];
     __shared__ uint32_t odd;                              // V values that are not finite were taken out
+    __shared__ uint32_t lows[4];
 
     const Item it = make_item<false>(a, blockIdx.x);
     if (!it.live) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t r = lane & 31, h = lane >> 5;
     T* const ty = nullptr;
 
@@ -343,33 +459,19 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
     low = __builtin_amdgcn_readfirstlane(low);
-    __shared__ uint32_t lows[4];
     if (lane == 0) lows[wave] = low;
     if (tid == 0) odd = 0;
     __syncthreads();
     const uint32_t block_low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
 
     const float c = fabsf(c0);
-    float m = -INFINITY, l = 0.0f;
+    const float lazy = kLazy / c;
+    float m = -INFINITY, l = 0.0f, mc = 0.0f, bar = -INFINITY;   // bar: the score that moves m
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = f32x16{};
 
-    const uint32_t head_off = it.head * (a.token_bytes / a.kv_heads);
-    const uint32_t row_bytes = a.token_bytes / a.kv_heads;
-    u32x4 xk[PER], xv[PER];
-    auto fetch = [&](uint32_t slot) {                     // slot: of the tile's key `lane`
-        const uint32_t inside = anew(row_bytes);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint32_t idx = i * kAB + tid, key = idx / CH, ch = idx % CH;
-            const uint32_t s = uint32_t(__shfl(int(slot), int(key & 63), 64));
-            const bool in = ch * 16 < inside && key < uint32_t(kTileKeys);
-            xk[i] = ld16(chunk_at(a, s, head_off + ch * 16, in));
-            xv[i] = ld16(chunk_at(a, s, a.token_bytes + head_off + ch * 16, in));
-        }
-    };
-    auto put16 = [&](uint8_t* p, u32x4 v) { *reinterpret_cast<u32x4*>(p) = v; };
+    const uint32_t row_bytes = a.token_bytes / a.kv_heads, head_off = it.head * row_bytes;
     // V values that are not finite become 0
     auto scrub = [&](u32x4 v) {
         const uint32_t e = exponent_bits(ty);
@@ -384,116 +486,234 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
         if (bad) odd = 1;
         return v;
     };
-    auto stage = [&](int buf, bool careful) {
+    // A unit's K and V rows on their way; slot: of its key `lane` % 32.  A chunk
+    // past the head's end, or of a key that is not there, is read from zeros.
+    u32x4 xk[FP8 ? PER : 1], xv[FP8 ? PER : 1];
+    const uint8_t *from_k[PER], *from_v[PER];
+    uint32_t step_k[PER], step_v[PER];                    // bytes a slot
+    const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeroCell);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const uint32_t idx = FP8 ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH, pos = idx % CH;
+        const uint32_t ck = (FP8 ? pos : pos ^ G::swz_k(key)) * 16, cv = (FP8 ? pos : pos ^ G::swz_v(key)) * 16;
+        const bool in = key < uint32_t(kTileKeys);
+        step_k[i] = in && ck < row_bytes ? a.rec : 0u;
+        step_v[i] = in && cv < row_bytes ? a.rec : 0u;
+        from_k[i] = step_k[i] ? a.pool + head_off + ck : zeros;
+        from_v[i] = step_v[i] ? a.pool + a.token_bytes + head_off + cv : zeros;
+    }
+    uint32_t sl[PER];                                     // the slots that K was loaded from last
+    auto load_k = [&](uint32_t slot, uint8_t* k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t idx = FP8 ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH;
+            sl[i] = uint32_t(__shfl(int(slot), int(key & 31), 64));
+            const bool there = sl[i] != kNoCell;
+            const uint8_t* p = (there ? from_k[i] : zeros) + uint64_t(there ? sl[i] : 0u) * step_k[i];
+            if constexpr (FP8) xk[i] = ld16(p);
+            else load_to_lds(p, k + (wave * PER + i) * 1024);
+        }
+    };
+    // V of the unit whose K was loaded last
+    auto load_v = [&](uint8_t* v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const bool there = sl[i] != kNoCell;
+            const uint8_t* p = (there ? from_v[i] : zeros) + uint64_t(there ? sl[i] : 0u) * step_v[i];
+            if constexpr (FP8) xv[i] = ld16(p);
+            else load_to_lds(p, v + (wave * PER + i) * 1024);
+        }
+    };
+    // fp8: what load() holds in registers, widened into LDS
+    auto put_fp8 = [&](const u32x4* from, bool is_v, uint8_t* to, bool careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const uint32_t idx = i * kAB + tid, key = idx / CH, ch = idx % CH;
             if (kTileKeys * CH % kAB && key >= uint32_t(kTileKeys)) break;
-            uint8_t* pk = lk[buf] + key * KROW;
-            uint8_t* pv = lv[buf] + key * VROW;
-            if constexpr (FP8) {
+            const uint32_t swz = is_v ? G::swz_v(key) : G::swz_k(key);
+            const u32x4 x = from[FP8 ? i : 0];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const u32x2 k0 = fp8_widen(xk[i][2 * j], ty), k1 = fp8_widen(xk[i][2 * j + 1], ty);
-                    const u32x2 v0 = fp8_widen(xv[i][2 * j], ty), v1 = fp8_widen(xv[i][2 * j + 1], ty);
-                    u32x4 v = {v0.x, v0.y, v1.x, v1.y};
-                    if (careful) v = scrub(v);
-                    put16(pk + ch * 32 + j * 16, u32x4{k0.x, k0.y, k1.x, k1.y});
-                    put16(pv + ch * 32 + j * 16, v);
-                }
-            } else {
-                u32x4 v = xv[i];
-                if (careful) v = scrub(v);
-                put16(pk + ch * 16, xk[i]);
-                put16(pv + ch * 16, v);
+            for (int j = 0; j < 2; ++j) {
+                const u32x2 x0 = fp8_widen(x[2 * j], ty), x1 = fp8_widen(x[2 * j + 1], ty);
+                u32x4 w = {x0.x, x0.y, x1.x, x1.y};
+                if (careful) w = scrub(w);
+                *reinterpret_cast<u32x4*>(to + key * G::ROW + ((ch * 2 + j) ^ swz) * 16) = w;
             }
         }
     };
-
-    const uint32_t ntiles = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
-    uint32_t slot = 0, slot_next = 0;                     // the lane's key of this tile and the next
-    if (ntiles) {
-        slot = key_slot(a, it, it.k0 + lane);
-        fetch(slot);
-        slot_next = key_slot(a, it, it.k0 + kTileKeys + lane);
-        stage(0, it.k0 + kTileKeys > block_low);
+    // places in a unit of K and V that the lane reads
+    uint32_t at_k[KS], at_v[DB];
+    {
+        const uint32_t i16 = lane & 15, gd = (lane >> 4) & 1, kk = 4 * h + i16 / 4;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) at_k[ks] = anew(r * G::ROW + ((ks * 2 + h) ^ G::swz_k(r)) * 16);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+            at_v[d] = anew(kk * G::ROW + ((d * 4 + gd * 2 + ((i16 >> 1) & 1)) ^ G::swz_v(kk)) * 16 + (i16 & 1) * 8);
     }
-    __syncthreads();
-    for (uint32_t n = 0; n < ntiles; ++n) {
-        const int buf = n & 1;
-        const uint32_t base = it.k0 + n * kTileKeys;
-        const uint64_t valid = __ballot(slot != kNoCell);
-        const bool more = n + 1 < ntiles;
-        if (more) {
-            fetch(slot_next);
-            slot = slot_next;
-            slot_next = key_slot(a, it, base + 2 * kTileKeys + lane);
+    // S^T: 32 keys x 32 rows
+    auto scores = [&](const uint8_t* k) __attribute__((always_inline)) {
+        f32x16 s = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = mma32(*reinterpret_cast<const u32x4*>(k + at_k[ks]), qf[ks], s, ty);
+        return s;
+    };
+    // the largest score of the lane's row among the scores that it holds
+    auto largest = [&](const f32x16& s) __attribute__((always_inline)) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        return top;
+    };
+    // ... with the masks, where there are any; keys: 8 (i / 4) + 4 h + i % 4
+    auto masked = [&](f32x16& s, float top, uint32_t base, uint32_t valid) __attribute__((always_inline)) {
+        if (rarely<DP <= 128>(valid != ~0u || base + kTileKeys > low)) {
+            const uint32_t see = (valid & low_bits(int32_t(min(limit, 0x7FFFFFFFu) - base))) >> (4 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = see & (1u << (8 * (i / 4) + i % 4)) ? s[i] : -INFINITY;
+            top = largest(s);
         }
-        // S^T: 64 keys x 32 rows
-        f32x16 s[2] = {f32x16{}, f32x16{}};
+        return max_halves(top);
+    };
+
+    const uint32_t units = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
+    const int32_t* const own_row = a.table + uint64_t(it.b) * a.width;
+    // key_page of a unit's keys, by one row where they lie on one side of the prefix's end
+    auto unit_page = [&](uint32_t base, uint32_t key) __attribute__((always_inline)) {
+        if (!a.flat && base < a.prefix && base + kTileKeys > a.prefix) return key_page(a, it, base + key);
+        const int32_t* row = a.flat || base < a.prefix ? a.prefix_pages : own_row;
+        return uint32_t(as_global(row)[min(base + key, it.k1 - 1) >> a.shift]);
+    };
+    const uint32_t key = lane & 31;
+    f32x16 sa, sb;
+    float top = -INFINITY;
+    // of the lane's key: pages of units j + 3 and j + 4; and which keys of units
+    // j + 1 and j + 2 are there
+    uint32_t page3 = 0, page4 = 0, valid1 = 0, valid2 = 0;
+    if (units) {
+        const uint32_t s0 = key_slot(a, it, it.k0 + key), s1 = key_slot(a, it, it.k0 + kTileKeys + key);
+        const uint32_t s2 = key_slot(a, it, it.k0 + 2 * kTileKeys + key);
+        page3 = unit_page(it.k0 + 3 * kTileKeys, key);
+        page4 = unit_page(it.k0 + 4 * kTileKeys, key);
+        const uint32_t first[3] = {s0, s1, s2};
+        uint8_t* const ks[3] = {k0, k1, k2};
+        uint8_t* const vs[2] = {v0, v1};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(lk[buf] + (kb * 32 + r) * KROW + ks * 32 + h * 16);
-                s[kb] = mma32(kf, qf[ks], s[kb], ty);
-            }
-        // keys: 32 kb + 8 (i / 4) + 4 h + i % 4
-        if (valid != ~0ull || base + kTileKeys > low) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const uint32_t see = (uint32_t(valid >> (32 * kb)) & low_bits(int32_t(min(limit, 0x7FFFFFFFu) - base) - 32 * kb)) >> (4 * h);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[kb][i] = see & (1u << (8 * (i / 4) + i % 4)) ? s[kb][i] : -INFINITY;
+        for (int u = 0; u < 3; ++u) {
+            load_k(first[u], ks[u]);
+            if (u < 2) load_v(vs[u < 2 ? u : 0]);
+            if constexpr (FP8) {
+                put_fp8(xk, false, ks[u], false);
+                if (u < 2) put_fp8(xv, true, vs[u < 2 ? u : 0], it.k0 + (u + 1) * kTileKeys > block_low);
             }
         }
-        float top = s[0][0];
-#pragma unroll
-        for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        if (__any((top - m) * c > kLazy || m == -INFINITY)) {
+        valid1 = uint32_t(__ballot(s1 != kNoCell));
+        valid2 = uint32_t(__ballot(s2 != kNoCell));
+        meet();
+        sa = scores(k0);
+        top = masked(sa, largest(sa), it.k0, uint32_t(__ballot(s0 != kNoCell)));
+    }
+    // Step j: K of unit j + 1 and V of unit j are read, K of unit j + 3 (its
+    // lane's slot: `slot`) and V of unit j + 2 loaded.
+    auto step = [&](uint32_t base, uint32_t slot, uint32_t valid, const uint8_t* k_next, const uint8_t* v_now, uint8_t* k_to,
+                    uint8_t* v_to, f32x16& s, f32x16& s_next) __attribute__((always_inline)) {
+        if (rarely<DP <= 128>(__ballot(top > bar) != 0)) {
             const float to = fmaxf(m, top);
             const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
             m = to;
+            bar = m + lazy;
+            mc = m == -INFINITY ? 0.0f : m * c;
             l *= f;
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int d = 0; d < DB; ++d) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
-        }
-        const float mc = m == -INFINITY ? 0.0f : m * c;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -mc));
-                l += s[kb][i];
-            }
-        // O^T += V^T P^T, 16 keys at a time
-        const uint32_t i16 = lane & 15, gd = (lane >> 4) & 1;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const f32x16& x = s[t / 2];
-            const int i0 = 8 * (t % 2);
-            const u32x4 p = {pack2(x[i0], x[i0 + 1], ty), pack2(x[i0 + 2], x[i0 + 3], ty),
-                             pack2(x[i0 + 4], x[i0 + 5], ty), pack2(x[i0 + 6], x[i0 + 7], ty)};
-            const uint8_t* v = lv[buf] + (16 * t + 4 * h + i16 / 4) * VROW + gd * 32 + (i16 % 4) * 8;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const u32x2 v0 = lds_tr(v + d * 64), v1 = lds_tr(v + 8 * VROW + d * 64);
-                o[d] = mma32(u32x4{v0.x, v0.y, v1.x, v1.y}, p, o[d], ty);
             }
         }
-        if (more) stage(buf ^ 1, base + 2 * kTileKeys > block_low);
-        __syncthreads();
+        load_v(v_to);
+        // (the lane masks of both at once, at four loads each, are too many)
+        if constexpr (PER > 2) __builtin_amdgcn_sched_barrier(0);
+        load_k(slot, k_to);
+        // The next unit's scores beside this one's powers, then O^T += V^T P^T.
+        // Left to the compiler's order: barriers between a vector and a matrix
+        // part, alternating both products, fixed counts of vector instructions
+        // to a matrix one, or raised priority in the matrix part took 0 to 10 %
+        // longer (8192 tokens behind 8192, eight K/V heads).
+        constexpr int AK = DP > 128 ? 4 : KS < 8 ? KS : 8, AV = 4;   // reads ahead of their use
+        u32x4 kf[KS], vf[2 * DB];
+        auto read_k = [&](int i) __attribute__((always_inline)) {
+            kf[i] = *reinterpret_cast<const u32x4*>(k_next + at_k[i]);
+        };
+        // keys 16 t + 4 h + (lane % 16) / 4 and 8 further
+        auto read_v = [&](int i) __attribute__((always_inline)) {
+            const uint8_t* vd = v_now + at_v[i % DB] + 16 * (i / DB) * G::ROW;
+            const u32x2 x0 = lds_tr(vd), x1 = lds_tr(vd + 8 * G::ROW);
+            vf[i] = u32x4{x0.x, x0.y, x1.x, x1.y};
+        };
+#pragma unroll
+        for (int i = 0; i < AK; ++i) read_k(i);
+        s_next = f32x16{};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            s_next = mma32(kf[i], qf[i], s_next, ty);
+            if (i + AK < KS) read_k(i + AK);
+        }
+        u32x4 p[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i / 4][i % 4] = pack2(s[2 * i], s[2 * i + 1], ty);
+            l = add2(uint32_t(p[i / 4][i % 4]), l, ty);   // the sum is that of the rounded P
+        }
+#pragma unroll
+        for (int i = 0; i < AV; ++i) read_v(i);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            if (i + AV < 2 * DB) read_v(i + AV);
+            o[i % DB] = mma32(vf[i], p[i / DB], o[i % DB], ty);
+        }
+        top = masked(s_next, largest(s_next), base + kTileKeys, valid);
+        if constexpr (FP8) {
+            put_fp8(xk, false, k_to, false);
+            put_fp8(xv, true, v_to, base + 3 * kTileKeys > block_low);
+        }
+    };
+    // Two steps, with a barrier before them: what either reads has come in the
+    // pass before, and what either loads goes where nothing is read any more.
+    // (The pages, loaded a pass ahead, have come by then too.)
+    auto pass = [&](uint32_t j, const uint8_t* ka, const uint8_t* kb, uint8_t* va, uint8_t* vb, uint8_t* kc, uint8_t* vc,
+                    uint8_t* kd, uint8_t* vd) __attribute__((always_inline)) {
+        const uint32_t base = it.k0 + j * kTileKeys;
+        meet();
+        if (!FP8 && rarely<DP <= 128>(base + 2 * kTileKeys > block_low)) {
+            for (uint32_t e = tid; e < uint32_t(G::BYTES) / 16; e += kAB) {
+                const u32x4 x = reinterpret_cast<const u32x4*>(va)[e], y = reinterpret_cast<const u32x4*>(vb)[e];
+                reinterpret_cast<u32x4*>(va)[e] = scrub(x);
+                reinterpret_cast<u32x4*>(vb)[e] = scrub(y);
+            }
+            meet();
+        }
+        const uint32_t slot3 = page_slot(a, it, base + 3 * kTileKeys + key, page3);
+        const uint32_t slot4 = page_slot(a, it, base + 4 * kTileKeys + key, page4);
+        page3 = unit_page(base + 5 * kTileKeys, key);
+        page4 = unit_page(base + 6 * kTileKeys, key);
+        step(base, slot3, valid1, ka, va, kc, vc, sa, sb);
+        if (j + 1 < units) step(base + kTileKeys, slot4, valid2, kb, vb, kd, vd, sb, sa);
+        valid1 = uint32_t(__ballot(slot3 != kNoCell));
+        valid2 = uint32_t(__ballot(slot4 != kNoCell));
+    };
+    for (uint32_t j = 0; j < units; j += 4) {
+        pass(j, k1, k2, v0, v1, k3, v2, k0, v3);
+        if (j + 2 < units) pass(j + 2, k3, k0, v2, v3, k1, v0, k2, v1);
     }
+    meet();
 
     // V values that were taken out, to the rows that see them
     if (odd) {
         const uint32_t skip = block_low > it.k0 ? (block_low - it.k0) / kTileKeys * kTileKeys : 0u;
-        for (uint32_t key = it.k0 + skip; key < it.k1; ++key) {
-            const uint32_t sl = key < limit ? key_slot(a, it, key) : kNoCell;
+        for (uint32_t kk = it.k0 + skip; kk < it.k1; ++kk) {
+            const uint32_t sl = kk < limit ? key_slot(a, it, kk) : kNoCell;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -501,18 +721,26 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
                     const f32x4 x = not_finite(value4<T, FP8>(a, sl, head_off, uint32_t(d * 32 + 8 * i) + 4 * h), ty);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[d][4 * i + j] += x[j];
+                    __builtin_amdgcn_sched_barrier(0);    // a rare path: few registers, not speed
                 }
         }
     }
 
     l += __shfl_xor(l, 32, 64);
-    settle(m, l, seen != 0);
-    if (!has) return;
-    const float vs = a.v_scale ? *a.v_scale : 1.0f;
+    {
+        const f32x2 ml = settle(m, l, limit != 0xFFFFFFFFu);
+        m = ml.x, l = ml.y;
+    }
+    // where the row goes, worked out anew: not held over the loop
+    const uint32_t at_row = it.row0 + wave * 32 + (anew(lane) & 31);
+    if (at_row >= it.rows) return;
+    LateArgs& e = late_args();
+    const uint32_t to_token = it.t0 + at_row / e.group, to_head = it.head * e.group + at_row % e.group;
+    const float vs = e.v_scale ? *e.v_scale : 1.0f;
     const float inv = l > 0.0f ? vs / l : l == l ? 0.0f : l;
-    if (!a.direct && h == 0) {
-        const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(token) * a.heads + head;
-        *as_global(a.ws_ml + at) = f32x2{m == -INFINITY ? -INFINITY : m * c, l};
+    if (!e.direct && anew(h) == 0) {
+        const uint64_t at = uint64_t(it.part) * e.tokens * e.heads + uint64_t(to_token) * e.heads + to_head;
+        *as_global(e.ws_ml + at) = f32x2{m == -INFINITY ? -INFINITY : m * c, l};
     }
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -520,7 +748,7 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
         for (int i = 0; i < 4; ++i) {
             f32x4 x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             if (l == 0.0f) x = f32x4{0, 0, 0, 0};
-            emit4<T>(a, it, token, head, uint32_t(d * 32 + 8 * i) + 4 * h, x, inv);
+            emit4<T>(e, it, to_token, to_head, uint32_t(d * 32 + 8 * i) + 4 * h, x, inv);
         }
 }
 
@@ -724,7 +952,10 @@ __global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
     // the four waves' results: brought to one maximum, summed over LDS
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    settle(m, l, seen != 0);
+    {
+        const f32x2 ml = settle(m, l, seen != 0);
+        m = ml.x, l = ml.y;
+    }
     if (g == 0) {
         lm[wave][r] = m;
         ll[wave][r] = l;
@@ -938,7 +1169,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.cu = s->cu_q;
     a.k_scale = s->k_scale;
     a.v_scale = s->v_scale;
-    a.rec = rec;
+    a.rec = uint32_t(rec);
     a.token_bytes = uint32_t(rec / 2);
     a.tokens = uint32_t(s->tokens);
     a.batch = uint32_t(s->batch);
