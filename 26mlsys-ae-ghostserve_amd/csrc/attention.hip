@@ -142,9 +142,9 @@ struct AttnArgs {
     uint32_t prefix;                           // keys of the shared part (0: none)
     uint32_t first;                            // first own key: prefix, or 0 with the prefix's pages read there
     uint32_t parts_flat, parts_own;            // splits of the keys of each part
-    uint32_t tiles;                            // row tiles (upper bound) of this launch
-    uint32_t req_tiles;                        // stream kernel, own keys: row tiles of a request
-    int flat;                                  // this launch: rows of all requests on the prefix
+    uint32_t blocks_flat;                      // blocks of the shared part, before those of the own keys
+    uint32_t tiles_flat, tiles_own;            // row tiles of each (upper bound)
+    uint32_t req_tiles;                        // stream blocks, own keys: row tiles of a request
     int direct;                                // one part in all: outputs are final
     int wide_q, wide_o;                        // 16-byte rows
     float scale;
@@ -176,6 +176,7 @@ __device__ __forceinline__ uint32_t seen_by(const AttnArgs& a, uint32_t b, uint3
 // What a block works on: rows row0 .. of a segment's rows, keys k0 .. k1 - 1.
 struct Item {
     bool live;
+    bool flat;                                 // the shared part: rows of all requests
     uint32_t b;                                // request (own keys)
     uint32_t t0;                               // its first token (0: all requests' rows)
     uint32_t rows;                             // rows of the segment
@@ -221,9 +222,11 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     constexpr uint32_t BM = STREAM ? kStreamRows : kTileRows;
     constexpr uint32_t KEYS = STREAM ? 4 * kStreamKeys : kTileKeys;
     Item it{};
-    const uint32_t parts = a.flat ? a.parts_flat : a.parts_own;
-    uint32_t tiles = a.tiles;
-    if (!STREAM && !a.flat) {
+    it.flat = id < a.blocks_flat;
+    if (!it.flat) id -= a.blocks_flat;
+    const uint32_t parts = it.flat ? a.parts_flat : a.parts_own;
+    uint32_t tiles = it.flat ? a.tiles_flat : a.tiles_own;
+    if (!STREAM && !it.flat) {
         // as many tiles as there are, not the launch's bound: blocks without
         // work come last then, and no compute unit gets a third block for them
         tiles = __builtin_amdgcn_readfirstlane(tile_at(a, 0xFFFFFFFFu).first);
@@ -236,12 +239,12 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     // 8192 in four requests).
     const uint32_t hp = parts * a.kv_heads, rest = id % hp;
     uint32_t tile = id / hp;
-    if (!STREAM && !a.flat) tile = tiles - 1 - tile;
+    if (!STREAM && !it.flat) tile = tiles - 1 - tile;
     const uint32_t split = rest % parts;
     it.head = rest / parts;
-    it.part = a.flat ? split : a.parts_flat + split;
+    it.part = it.flat ? split : a.parts_flat + split;
     uint32_t first = 0, last;
-    if (a.flat) {
+    if (it.flat) {
         it.rows = live_tokens(a) * a.group;
         it.row0 = tile * BM;
         it.live = it.row0 < it.rows;
@@ -281,7 +284,7 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
 // In two steps, so that the table's entry can be on its way for a while.
 __device__ __forceinline__ uint32_t key_page(const AttnArgs& a, const Item& it, uint32_t pos) {
     pos = min(pos, it.k1 - 1);
-    const int32_t* row = a.flat || pos < a.prefix ? a.prefix_pages : a.table + uint64_t(it.b) * a.width;
+    const int32_t* row = it.flat || pos < a.prefix ? a.prefix_pages : a.table + uint64_t(it.b) * a.width;
     return uint32_t(*as_global(row + (pos >> a.shift)));
 }
 __device__ __forceinline__ uint32_t page_slot(const AttnArgs& a, const Item& it, uint32_t pos, uint32_t page) {
@@ -419,20 +422,15 @@ __device__ __forceinline__ void meet() {
 }
 
 template <class T, bool FP8, int DP>
-__global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uint8_t* k0, uint8_t* k1, uint8_t* k2, uint8_t* k3,
+                                          uint8_t* v0, uint8_t* v1, uint8_t* v2, uint8_t* v3) {
     using G = TileGeom<DP>;
     constexpr int KS = DP / 16, DB = DP / 32;
     constexpr int CH = FP8 ? DP / 16 : G::POS;             // chunks of a key that are loaded
     constexpr int PER = (kTileKeys * CH + kAB - 1) / kAB;  // of them by a thread
-    // separate arrays: the compiler can tell their accesses apart, so a read of
-    // one does not wait for a load into another
-    __shared__ __attribute__((aligned(16))) uint8_t k0[G::BYTES], k1[G::BYTES], k2[G::BYTES], k3[G::BYTES];
-    __shared__ __attribute__((aligned(16))) uint8_t v0[G::BYTES], v1[G::BYTES], v2[G::BYTES], v3[G::BYTES];
     __shared__ uint32_t odd;                              // V values that are not finite were taken out
     __shared__ uint32_t lows[4];
 
-    const Item it = make_item<false>(a, blockIdx.x);
-    if (!it.live) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t r = lane & 31, h = lane >> 5;
     T* const ty = nullptr;
@@ -443,7 +441,7 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
     const uint32_t token = it.t0 + (has ? row / a.group : 0u);
     const uint32_t head = it.head * a.group + (has ? row % a.group : 0u);
     // rows that are not there, and rows that see nothing, ask for no mask
-    const uint32_t seen = has ? seen_by(a, a.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
     const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
     // 0 would make NaN of a masked score; a negative one goes to the query
     const float c0 = score_factor(a);
@@ -580,8 +578,8 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
     const int32_t* const own_row = a.table + uint64_t(it.b) * a.width;
     // key_page of a unit's keys, by one row where they lie on one side of the prefix's end
     auto unit_page = [&](uint32_t base, uint32_t key) __attribute__((always_inline)) {
-        if (!a.flat && base < a.prefix && base + kTileKeys > a.prefix) return key_page(a, it, base + key);
-        const int32_t* row = a.flat || base < a.prefix ? a.prefix_pages : own_row;
+        if (!it.flat && base < a.prefix && base + kTileKeys > a.prefix) return key_page(a, it, base + key);
+        const int32_t* row = it.flat || base < a.prefix ? a.prefix_pages : own_row;
         return uint32_t(as_global(row)[min(base + key, it.k1 - 1) >> a.shift]);
     };
     const uint32_t key = lane & 31;
@@ -758,29 +756,26 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_tile_kernel(AttnA
 // V.  A wave works alone until the end (its V in a part of LDS of its own, its
 // maximum and sum its own), then the four results are joined.
 template <class T, bool FP8, int DP>
-__global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, uint8_t* v0, uint8_t* v1, uint8_t* v2,
+                                            uint8_t* v3) {
+    using G = TileGeom<DP>;                               // V lies as in the tile kernel
     constexpr int KS = DP / 32, DB = DP / 16;
-    constexpr int VROW = DP * 2 + 32;
     constexpr int CH = DP / (FP8 ? 16 : 8);
     constexpr int PER = (kStreamKeys * CH + 63) / 64;
-    constexpr int VBYTES = kStreamKeys * VROW, OBYTES = kStreamRows * DP * 4;
-    constexpr int WBYTES = VBYTES > OBYTES ? VBYTES : OBYTES;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4][WBYTES];
+    static_assert(kStreamKeys == kTileKeys && G::BYTES >= kStreamRows * DP * 4, "a unit of V, or the rows' results");
     __shared__ float lm[4][kStreamRows], ll[4][kStreamRows];
 
-    const Item it = make_item<true>(a, blockIdx.x);
-    if (!it.live) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t r = lane & 15, g = lane >> 4;
     T* const ty = nullptr;
-    uint8_t* const lv = lds[wave];
+    uint8_t* const lv = wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3;
 
     const uint32_t row = it.row0 + r;
     const bool has = row < it.rows;
     const uint32_t token = it.t0 + (has ? row / a.group : 0u);
     const uint32_t head = it.head * a.group + (has ? row % a.group : 0u);
     // rows that are not there, and rows that see nothing, ask for no mask
-    const uint32_t seen = has ? seen_by(a, a.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
     const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
     // 0 would make NaN of a masked score; a negative one goes to the query
     const float c0 = score_factor(a);
@@ -861,19 +856,20 @@ __global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
         for (int i = 0; i < PER; ++i) {
             const uint32_t idx = i * 64 + lane, key = idx / CH, ch = idx % CH;
             if (kStreamKeys * CH % 64 && key >= uint32_t(kStreamKeys)) break;
-            uint8_t* pv = lv + key * VROW;
+            uint8_t* pv = lv + key * G::ROW;
+            const uint32_t swz = G::swz_v(key);
             if constexpr (FP8) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const u32x2 v0 = fp8_widen(xv[i][2 * j], ty), v1 = fp8_widen(xv[i][2 * j + 1], ty);
                     u32x4 v = {v0.x, v0.y, v1.x, v1.y};
                     if (careful) odd |= scrub(v);
-                    *reinterpret_cast<u32x4*>(pv + ch * 32 + j * 16) = v;
+                    *reinterpret_cast<u32x4*>(pv + ((ch * 2 + j) ^ swz) * 16) = v;
                 }
             } else {
                 u32x4 v = xv[i];
                 if (careful) odd |= scrub(v);
-                *reinterpret_cast<u32x4*>(pv + ch * 16) = v;
+                *reinterpret_cast<u32x4*>(pv + (ch ^ swz) * 16) = v;
             }
         }
         f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
@@ -923,14 +919,16 @@ __global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
         // sum over keys 4 g .. and 16 + 4 g .. : what the lane's scores are of
         const u32x4 p = {pack2(s[0][0], s[0][1], ty), pack2(s[0][2], s[0][3], ty), pack2(s[1][0], s[1][1], ty),
                          pack2(s[1][2], s[1][3], ty)};
-        const uint8_t* v = lv + (4 * g + r / 4) * VROW + (r % 4) * 8;
+        const uint32_t kk = 4 * g + r / 4, z = G::swz_v(kk);   // keys 8 and 16 apart: the same permutation
+        const uint8_t* v = lv + kk * G::ROW + (r & 1) * 8;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            const u32x2 v0 = lds_tr(v + d * 32), v1 = lds_tr(v + 16 * VROW + d * 32);
-            o[d] = mma16(u32x4{v0.x, v0.y, v1.x, v1.y}, p, o[d], ty);
+            const uint8_t* vd = v + ((d * 2 + ((r >> 1) & 1)) ^ z) * 16;
+            const u32x2 x0 = lds_tr(vd), x1 = lds_tr(vd + 16 * G::ROW);
+            o[d] = mma16(u32x4{x0.x, x0.y, x1.x, x1.y}, p, o[d], ty);
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -964,7 +962,7 @@ __global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
     const float top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
     auto factor = [&](float x) { return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x - top) * c); };
     const float f = factor(m);
-    float* lo = reinterpret_cast<float*>(lds[wave]);      // [row][dim]
+    float* lo = reinterpret_cast<float*>(lv);             // [row][dim]
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
         f32x4 x = o[d] * f;
@@ -981,7 +979,7 @@ __global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
         float sum = 0.0f, mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) + rr * DP + d);
+            x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(w == 0 ? v0 : w == 1 ? v1 : w == 2 ? v2 : v3) + rr * DP + d);
             mx = fmaxf(mx, lm[w][rr]);
         }
 #pragma unroll
@@ -996,24 +994,60 @@ __global__ __launch_bounds__(kAB) void attn_stream_kernel(AttnArgs a) {
     }
 }
 
+// The kernels: FLAT and OWN say what takes the shared part and the own keys (0: no
+// such blocks, 1: stream blocks, 2: tile blocks).  Both parts are one launch: the
+// one is bound by the matrix units, the other by memory.
+template <class T, bool FP8, int DP, int FLAT, int OWN>
+__global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a) {
+    using G = TileGeom<DP>;
+    constexpr bool TILE = FLAT == 2 || OWN == 2;
+    // separate arrays: the compiler can tell their accesses apart, so a read of
+    // one does not wait for a load into another
+    __shared__ __attribute__((aligned(16))) uint8_t k0[TILE ? G::BYTES : 16], k1[TILE ? G::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t k2[TILE ? G::BYTES : 16], k3[TILE ? G::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t v0[G::BYTES], v1[G::BYTES], v2[G::BYTES], v3[G::BYTES];
+    const uint32_t id = blockIdx.x;
+    if (TILE && (FLAT != 2 || OWN == 2 || id < a.blocks_flat)) {
+        const Item it = make_item<false>(a, id);
+        if (it.live) attn_tile<T, FP8, DP>(a, it, k0, k1, k2, k3, v0, v1, v2, v3);
+    } else if (OWN == 1) {
+        const Item it = make_item<true>(a, id);
+        if (it.live) attn_stream<T, FP8, DP>(a, it, v0, v1, v2, v3);
+    }
+}
+
 // Partial results of a row brought to one maximum, summed, divided and rounded.
+// A block takes one row: `lanes` threads a part, the parts shared out to the
+// others, so that a row's parts are read side by side.
 template <class T>
 __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lanes) {
-    const uint32_t row = (blockIdx.x * kAB + threadIdx.x) / lanes, d = (threadIdx.x % lanes) * 4;
-    const uint32_t rows = a.tokens * a.heads;
-    if (row >= rows || row / a.heads >= live_tokens(a) || d >= a.dim) return;
+    __shared__ f32x4 lo[kAB];
+    __shared__ float ll[kAB];
+    const uint32_t tid = threadIdx.x, rows = a.tokens * a.heads, row = blockIdx.x;
+    if (row / a.heads >= live_tokens(a)) return;
+    const uint32_t each = kAB / lanes, mine = tid / lanes, d = tid % lanes * 4;
     const uint32_t parts = a.parts_flat + a.parts_own;
-    float top = -INFINITY;
-    for (uint32_t p = 0; p < parts; ++p) top = fmaxf(top, as_global(a.ws_ml)[uint64_t(p) * rows + row].x);
+    float top = -INFINITY, l = 0.0f;
     f32x4 o = {0, 0, 0, 0};
-    float l = 0.0f;
-    for (uint32_t p = 0; p < parts; ++p) {
+    for (uint32_t p = tid & 63; p < parts; p += 64) top = fmaxf(top, as_global(a.ws_ml)[uint64_t(p) * rows + row].x);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+#pragma unroll 4
+    for (uint32_t p = mine; p < parts; p += each) {
         const uint64_t at = uint64_t(p) * rows + row;
         const f32x2 ml = as_global(a.ws_ml)[at];
         if (ml.x == -INFINITY) continue;                  // nothing seen there
         const float f = __builtin_amdgcn_exp2f(ml.x - top);
         l += ml.y * f;
-        o += *as_global(reinterpret_cast<const f32x4*>(a.ws_o + at * a.dim + d)) * f;
+        if (d < a.dim) o += *as_global(reinterpret_cast<const f32x4*>(a.ws_o + at * a.dim + d)) * f;
+    }
+    lo[tid] = o;
+    ll[tid] = l;
+    __syncthreads();
+    if (mine || d >= a.dim) return;
+    for (uint32_t p = 1; p < each; ++p) {
+        o += lo[p * lanes + tid];
+        l += ll[p * lanes + tid];
     }
     const float vs = a.v_scale ? *a.v_scale : 1.0f;
     const float inv = l > 0.0f ? vs / l : l == l ? 0.0f : l;
@@ -1023,64 +1057,60 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
 
 typedef void (*AttnFn)(AttnArgs);
 
+template <class T, bool FP8, int FLAT, int OWN>
+AttnFn pick_dim(int dim) {
+    return dim <= 64    ? &attn_kernel<T, FP8, 64, FLAT, OWN>
+           : dim <= 96  ? &attn_kernel<T, FP8, 96, FLAT, OWN>
+           : dim <= 128 ? &attn_kernel<T, FP8, 128, FLAT, OWN>
+                        : &attn_kernel<T, FP8, 256, FLAT, OWN>;
+}
 template <class T, bool FP8>
-AttnFn pick_attn(bool stream, int dim) {
-    if (stream)
-        return dim <= 64    ? &attn_stream_kernel<T, FP8, 64>
-               : dim <= 96  ? &attn_stream_kernel<T, FP8, 96>
-               : dim <= 128 ? &attn_stream_kernel<T, FP8, 128>
-                            : &attn_stream_kernel<T, FP8, 256>;
-    return dim <= 64    ? &attn_tile_kernel<T, FP8, 64>
-           : dim <= 96  ? &attn_tile_kernel<T, FP8, 96>
-           : dim <= 128 ? &attn_tile_kernel<T, FP8, 128>
-                        : &attn_tile_kernel<T, FP8, 256>;
+AttnFn pick_attn(bool flat_tile, bool own_tile, int dim) {
+    return own_tile ? pick_dim<T, FP8, 0, 2>(dim) : flat_tile ? pick_dim<T, FP8, 2, 1>(dim) : pick_dim<T, FP8, 1, 1>(dim);
 }
 
 struct AttnPlan {
-    bool flat, flat_stream, own_stream;
-    uint32_t parts_flat, parts_own, flat_tiles, own_tiles, req_tiles, first;
-    uint64_t rows;
+    bool flat, flat_tile, own_tile;
+    uint32_t parts_flat, parts_own, tiles_flat, tiles_own, req_tiles, first;
+    uint64_t rows, blocks_flat, blocks;
     bool direct() const { return parts_flat + parts_own == 1; }
     int64_t bytes(int64_t dim) const {
         return direct() ? 0 : int64_t(uint64_t(parts_flat + parts_own) * rows * (uint64_t(dim) * 4 + 8)) + 16;
     }
 };
 
-// Which kernel takes which part, and in how many splits of the keys.
+// Which blocks take which part, and in how many splits of the keys.
 inline AttnPlan plan_attention(const kvec_attention* s) {
     AttnPlan p{};
-    const uint64_t group = uint64_t(s->heads / s->kv_heads), N = uint64_t(s->tokens);
-    const uint64_t max_q = s->cu_q ? uint64_t(s->max_q) : 1;
+    const uint64_t group = uint64_t(s->heads / s->kv_heads), N = uint64_t(s->tokens), B = uint64_t(s->batch);
+    const uint64_t max_q = s->cu_q ? uint64_t(s->max_q) : 1, Hk = uint64_t(s->kv_heads);
+    const uint64_t req_rows = max_q * group, all_rows = N * group, prefix = uint64_t(s->prefix);
+    const uint64_t cap = uint64_t(s->pages_per_seq) * uint64_t(s->page_tokens);
+    const uint64_t len = s->max_len > 0 && uint64_t(s->max_len) < cap ? uint64_t(s->max_len) : cap;
     p.rows = N * uint64_t(s->heads);
-    const uint64_t req_rows = max_q * group, all_rows = N * group;
-    const uint64_t prefix = uint64_t(s->prefix);
-    // Requests that fill tiles by themselves read the prefix with their own
-    // keys: no partial results to write and join.
-    p.own_stream = req_rows <= 4 * kStreamRows;
-    p.flat = prefix > 0 && req_rows < uint64_t(kTileRows);
-    p.first = p.flat ? uint32_t(prefix) : 0;
-    p.flat_stream = all_rows <= 2 * kStreamRows;
     auto splits = [](uint64_t blocks, uint64_t want, uint64_t keys, uint64_t least) {
-        uint64_t n = (want + blocks - 1) / (blocks ? blocks : 1);
-        const uint64_t most = (keys + least - 1) / least;
+        uint64_t n = want / (blocks ? blocks : 1);
+        const uint64_t most = keys / least;
         if (n > most) n = most;
         return uint32_t(n < 1 ? 1 : n > 256 ? 256 : n);
     };
+    // Requests with rows enough for tiles read the prefix with their own keys,
+    // without partial results to write and join.
+    p.own_tile = req_rows > 4 * kStreamRows;
+    p.req_tiles = uint32_t((req_rows + kStreamRows - 1) / kStreamRows);
+    p.tiles_own = p.own_tile ? uint32_t(all_rows / kTileRows) + uint32_t(B) : uint32_t(B) * p.req_tiles;
+    const uint64_t own = uint64_t(p.tiles_own) * Hk;
+    p.flat = prefix > 0 && !p.own_tile;
     if (p.flat) {
-        const uint64_t bm = p.flat_stream ? kStreamRows : kTileRows;
-        p.flat_tiles = uint32_t((all_rows + bm - 1) / bm);
-        p.parts_flat = splits(uint64_t(p.flat_tiles) * s->kv_heads, 512, prefix, 256);
+        p.first = uint32_t(prefix);
+        p.flat_tile = all_rows > 2 * kStreamRows;
+        const uint64_t bm = p.flat_tile ? kTileRows : kStreamRows;
+        p.tiles_flat = uint32_t((all_rows + bm - 1) / bm);
+        p.parts_flat = splits(uint64_t(p.tiles_flat) * Hk, 512, prefix, 256);
     }
-    if (p.own_stream) {
-        p.req_tiles = uint32_t((req_rows + kStreamRows - 1) / kStreamRows);
-        p.own_tiles = uint32_t(s->batch) * p.req_tiles;
-    } else {
-        p.own_tiles = uint32_t(all_rows / kTileRows) + uint32_t(s->batch);
-    }
-    const int64_t cap = int64_t(s->pages_per_seq) * s->page_tokens;
-    const int64_t len = s->max_len > 0 && s->max_len < cap ? s->max_len : cap;
-    const uint64_t own_keys = len > int64_t(p.first) ? uint64_t(len) - p.first : 1;
-    p.parts_own = splits(uint64_t(p.own_tiles) * s->kv_heads, p.own_stream ? 768 : 512, own_keys, 256);
+    p.parts_own = splits(own, 512, len > p.first ? len - p.first : 1, 256);
+    p.blocks_flat = p.flat ? uint64_t(p.tiles_flat) * Hk * p.parts_flat : 0;
+    p.blocks = p.blocks_flat + own * p.parts_own;
     return p;
 }
 
@@ -1185,6 +1215,9 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.first = p.first;
     a.parts_flat = p.parts_flat;
     a.parts_own = p.parts_own;
+    a.blocks_flat = uint32_t(p.blocks_flat);
+    a.tiles_flat = p.tiles_flat;
+    a.tiles_own = p.tiles_own;
     a.req_tiles = p.req_tiles;
     a.direct = p.direct();
     a.scale = s->scale;
@@ -1195,27 +1228,17 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
         a.ws_ml = (f32x2*)((uint8_t*)workspace + uint64_t(p.parts_flat + p.parts_own) * p.rows * uint64_t(s->dim) * 4);
     }
     const bool fp8 = s->pool_dtype == KVEC_FP8_E4M3, bf = s->dtype == KVEC_BF16;
-    auto pick = [&](bool st) {
-        return bf ? (fp8 ? pick_attn<__bf16, true>(st, s->dim) : pick_attn<__bf16, false>(st, s->dim))
-                  : (fp8 ? pick_attn<_Float16, true>(st, s->dim) : pick_attn<_Float16, false>(st, s->dim));
-    };
-    auto launch = [&](bool flat) {
-        AttnArgs x = a;
-        x.flat = flat;
-        x.tiles = flat ? p.flat_tiles : p.own_tiles;
-        const uint64_t blocks = uint64_t(x.tiles) * x.kv_heads * (flat ? x.parts_flat : x.parts_own);
-        if (blocks >= (uint64_t(1) << 31)) return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks", fn);
-        hipLaunchKernelGGL(pick(flat ? p.flat_stream : p.own_stream), dim3(unsigned(blocks)), dim3(kAB), 0,
-                           as_stream(stream), x);
-        return check_launch(fn);
-    };
-    if (p.flat && (rc = launch(true))) return rc;
-    if ((rc = launch(false))) return rc;
-    if (p.direct()) return KVEC_OK;
+    if (p.blocks >= (uint64_t(1) << 31)) return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks", fn);
+    AttnFn f = bf ? (fp8 ? pick_attn<__bf16, true>(p.flat_tile, p.own_tile, s->dim)
+                         : pick_attn<__bf16, false>(p.flat_tile, p.own_tile, s->dim))
+                  : (fp8 ? pick_attn<_Float16, true>(p.flat_tile, p.own_tile, s->dim)
+                         : pick_attn<_Float16, false>(p.flat_tile, p.own_tile, s->dim));
+    hipLaunchKernelGGL(f, dim3(unsigned(p.blocks)), dim3(kAB), 0, as_stream(stream), a);
+    if ((rc = check_launch(fn)) || p.direct()) return rc;
     uint32_t lanes = 16;
     while (lanes * 4 < a.dim) lanes *= 2;
-    const uint64_t threads = uint64_t(a.tokens) * a.heads * lanes;
-    if (bf) hipLaunchKernelGGL(attn_join_kernel<__bf16>, dim3(blocks_for(int64_t(threads), kAB)), dim3(kAB), 0, as_stream(stream), a, lanes);
-    else hipLaunchKernelGGL(attn_join_kernel<_Float16>, dim3(blocks_for(int64_t(threads), kAB)), dim3(kAB), 0, as_stream(stream), a, lanes);
+    const dim3 grid(unsigned(p.rows));
+    if (bf) hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, dim3(kAB), 0, as_stream(stream), a, lanes);
+    else hipLaunchKernelGGL(attn_join_kernel<_Float16>, grid, dim3(kAB), 0, as_stream(stream), a, lanes);
     return check_launch(fn);
 }
