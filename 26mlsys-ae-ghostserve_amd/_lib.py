@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch  # noqa: F401  (must precede CDLL, see module docstring)
 
@@ -20,6 +21,9 @@ LIB_PATH = os.path.join(HERE, "libkvec.so")
 
 # torch's own accessor of a stream handle; not public, so maybe not there
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# the current device, without torch.cuda.current_device()'s own checks: a GPU
+# tensor is at hand wherever it is asked for
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 _vp = C.c_void_p
 _i = C.c_int
@@ -179,8 +183,12 @@ class Attention(C.Structure):
     ]
 
 
-_sp = C.POINTER(Step)
-_ap = C.POINTER(Attention)
+# The step entry points take the structs above or the same bytes from struct.pack
+# (native layout), which is several times faster to fill than a Structure: a
+# small call is bound by its host time.  Formats in the order of the fields.
+STEP_FORMAT = struct.Struct("@PiiiqPPPqPPqPPP")
+NORM_ROTATE_FORMAT = struct.Struct("@qiiiiPPPqqqqqqPqqifPPiiiPqPPfPiqPPPP")
+ATTENTION_FORMAT = struct.Struct("@qiiiiiPqqPqqPiqiPiPPiqqPfPP")
 _nrp = C.POINTER(NormRotate)
 
 # name -> (restype, argtypes); mirrors include/kvec.h
@@ -227,10 +235,10 @@ SIGNATURES = {
     "kvec_rs16_recover_kv": (_i, [_vp, _vp, _vp, _i64, _i, _i, _i, _vp, _i, _vp]),
     "kvec_rs16_reconstruct": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
     "kvec_gf16_tables": (_i, [_vp, _vp]),
-    "kvec_step_tables": (_i, [_sp, _vp]),
-    "kvec_norm_rotate_write": (_i, [_nrp, _vp]),
-    "kvec_prefix_attention_workspace": (_i64, [_ap]),
-    "kvec_prefix_attention": (_i, [_ap, _vp, _i64, _vp]),
+    "kvec_step_tables": (_i, [_vp, _vp]),
+    "kvec_norm_rotate_write": (_i, [_vp, _vp]),
+    "kvec_prefix_attention_workspace": (_i64, [_vp]),
+    "kvec_prefix_attention": (_i, [_vp, _vp, _i64, _vp]),
 }
 
 # major number of the include/kvec.h these signatures mirror (KVEC_VERSION / 10000)
@@ -273,7 +281,7 @@ def call(name: str, *args) -> int:
 def call_on(device, name: str, *args) -> int:
     """`call` with ``device`` as the current device: a kernel is launched on the
     device that its stream belongs to."""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         return call(name, *args)
     with torch.cuda.device(device):
         return call(name, *args)
@@ -331,6 +339,8 @@ def require_cuda(*tensors, what: str = "tensor") -> None:
 
 def require_same_device(device, *tensors, what: str = "tensor") -> None:
     """Every tensor given (None: left out) lies on the GPU ``device``."""
+    if device.type != "cuda":
+        raise ValueError(f"{what}s must be GPU (HIP) tensors of one device")
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != device):
+        if t is not None and t.device != device:
             raise ValueError(f"{what}s must be GPU (HIP) tensors of one device")

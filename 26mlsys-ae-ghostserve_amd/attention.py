@@ -14,13 +14,12 @@ the queries' type or float8_e4m3fn with a scale for K and for V, as in
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+_COMPUTE = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def rotary_frequencies(rot: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -43,11 +42,12 @@ def rotary_axes(sections, device="cuda") -> torch.Tensor:
 
 def _layer(pool: torch.Tensor, layer: int) -> tuple[int, int, int, int]:
     """(address of the layer, slots, kv_heads, head_dim) of a pool."""
-    if pool.dim() != 6 or pool.shape[3] != 2:
+    shape = pool.shape
+    if len(shape) != 6 or shape[3] != 2:
         raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
-    if not pool.is_cuda or not pool.is_contiguous():
+    if not pool.is_contiguous():
         raise ValueError("pool must be a contiguous GPU (HIP) tensor")
-    L, pages, pt, _, H, D = pool.shape
+    L, pages, pt, _, H, D = shape
     if not 0 <= layer < L:
         raise ValueError(f"layer {layer} not in [0, {L})")
     n = pages * pt
@@ -55,12 +55,16 @@ def _layer(pool: torch.Tensor, layer: int) -> tuple[int, int, int, int]:
 
 
 def _scale(t, device, what: str):
-    """Address of a scale: a float32 tensor of one value on the GPU, or None."""
+    """Address of a scale: a float32 tensor of one value on the GPU, or 0."""
     if t is None:
-        return None
+        return 0
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
         raise ValueError(f"{what} must be one float32 value on the pool's device")
     return t.data_ptr()
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None,
@@ -89,22 +93,24 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     number on are left as they were, here and in the result.
 
     Returns the queries (``out``: contiguous like q, or q itself)."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("q must be [tokens, heads, dim], k and v [tokens, kv_heads, dim]")
     dev, dt = q.device, q.dtype
-    if dt not in (torch.float32, torch.bfloat16, torch.float16) or k.dtype != dt or v.dtype != dt:
+    if dt not in _COMPUTE or k.dtype != dt or v.dtype != dt:
         raise ValueError("q, k and v must be of one type: float32, bfloat16 or float16")
-    _lib.require_same_device(dev, q, k, v, positions, freqs, pool, slots, q_weight, k_weight, axis_of, tokens, out,
+    _lib.require_same_device(dev, k, v, positions, freqs, pool, slots, q_weight, k_weight, axis_of, tokens, out,
                              what="norm_rotate_write tensor")
-    N, Hq, D = q.shape
+    N, Hq, D = qs
     base, n_slots, Hk, Dp = _layer(pool, layer)
-    if (Hk, Dp) != (k.shape[1], D):
-        raise ValueError(f"pool holds {Hk} heads of {Dp}, k has {k.shape[1]} of {D}")
-    if pool.dtype != dt and pool.dtype != torch.float8_e4m3fn:
+    if Hk != ks[1] or Dp != D:
+        raise ValueError(f"pool holds {Hk} heads of {Dp}, k has {ks[1]} of {D}")
+    pool_dt = pool.dtype
+    if pool_dt != dt and pool_dt != torch.float8_e4m3fn:
         raise ValueError("pool must be of q's type or float8_e4m3fn")
-    for t in (q, k, v):
-        if D > 1 and t.shape[0] and t.shape[1] and t.stride(2) != 1:
-            raise ValueError("a head's values must be adjacent")
+    (q0, q1, q2), (k0, k1, k2), (v0, v1, v2) = q.stride(), k.stride(), v.stride()
+    if D > 1 and N and not q2 == k2 == v2 == 1:
+        raise ValueError("a head's values must be adjacent")
     if slots.dtype != torch.int32 or slots.shape != (N,) or not slots.is_contiguous():
         raise ValueError(f"slots must be contiguous int32 [{N}]")
     half = 0 if freqs is None else freqs.shape[0]
@@ -130,17 +136,18 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     if tokens is not None and (tokens.dtype != torch.int32 or tokens.numel() != 1):
         raise ValueError("tokens must be one int32 value")
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=dt, device=dev)
-    elif out.shape != q.shape or out.dtype != dt or not (out.is_contiguous() or out is q):
+        out = torch.empty(qs, dtype=dt, device=dev)
+        o0, o1 = Hq * D, D
+    elif out.shape != qs or out.dtype != dt or not (out.is_contiguous() or out is q):
         raise ValueError("out must be contiguous and like q, or q itself")
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    s = _lib.NormRotate(
-        N, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-        k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), int(bool(norm)), eps,
-        ptr(q_weight), ptr(k_weight), 2 * half, int(bool(interleaved)), axes, ptr(positions), axis_stride,
-        ptr(axis_of), ptr(freqs), factor, base, _DTYPES[pool.dtype], n_slots, slots.data_ptr(),
-        _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), ptr(tokens))
-    _lib.call_on(dev, "kvec_norm_rotate_write", ctypes.byref(s), _lib.stream_handle(dev))
+    else:
+        o0, o1, _ = out.stride()
+    s = _lib.NORM_ROTATE_FORMAT.pack(
+        N, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1, out.data_ptr(),
+        o0, o1, bool(norm), eps, _ptr(q_weight), _ptr(k_weight), 2 * half, bool(interleaved), axes, _ptr(positions),
+        axis_stride, _ptr(axis_of), _ptr(freqs), factor, base, _DTYPES[pool_dt], n_slots, slots.data_ptr(),
+        _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), _ptr(tokens))
+    _lib.call_on(dev, "kvec_norm_rotate_write", s, _lib.stream_handle(dev))
     return out
 
 
@@ -171,48 +178,51 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
     values split the work better.  ``scale``: default 1/sqrt(dim).  ``k_scale``,
     ``v_scale``: an fp8 pool's, as in :func:`norm_rotate_write`.  Nothing is read
     back to the host, so the call can be captured in a graph."""
-    if q.dim() != 3:
+    shape, tab = q.shape, page_table.shape
+    if len(shape) != 3:
         raise ValueError("q must be [tokens, heads, dim]")
-    dev, dt = q.device, q.dtype
-    if dt not in (torch.bfloat16, torch.float16):
+    dev, dt, i32 = q.device, q.dtype, torch.int32
+    if dt != torch.bfloat16 and dt != torch.float16:
         raise ValueError("q must be bfloat16 or float16")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+    if len(tab) != 2 or page_table.dtype != i32 or seq_lens.dtype != i32:
         raise ValueError("page_table must be int32 [batch, pages_per_seq], seq_lens int32")
-    N, Hq, D = q.shape
-    B, width = page_table.shape
-    if seq_lens.shape != (B,) or (cu_q is not None and (cu_q.shape != (B + 1,) or cu_q.dtype != torch.int32)):
+    N, Hq, D = shape
+    B, width = tab
+    if seq_lens.shape != (B,) or (cu_q is not None and (cu_q.shape != (B + 1,) or cu_q.dtype != i32)):
         raise ValueError(f"seq_lens must be [{B}] and cu_q int32 [{B + 1}]")
     if cu_q is None and N != B:
         raise ValueError("without cu_q there is one query token a request")
-    _lib.require_same_device(dev, q, pool, page_table, seq_lens, cu_q, prefix_pages, out,
-                             what="prefix_attention tensor")
+    _lib.require_same_device(dev, pool, page_table, seq_lens, cu_q, prefix_pages, out, what="prefix_attention tensor")
     base, _, Hk, Dp = _layer(pool, layer)
     if Dp != D or Hq % Hk:
         raise ValueError(f"q has {Hq} heads of {D}, the pool {Hk} of {Dp}")
-    if pool.dtype != dt and pool.dtype != torch.float8_e4m3fn:
+    pool_dt = pool.dtype
+    if pool_dt != dt and pool_dt != torch.float8_e4m3fn:
         raise ValueError("pool must be of q's type or float8_e4m3fn")
     for t in (page_table, seq_lens, cu_q, prefix_pages):
         if t is not None and not t.is_contiguous():
             raise ValueError("page_table, seq_lens, cu_q and prefix_pages must be contiguous")
-    if N and D > 1 and q.stride(2) != 1:
+    q0, q1, q2 = q.stride()
+    if N and D > 1 and q2 != 1:
         raise ValueError("a head's values must be adjacent")
-    pt, prefix = pool.shape[2], int(prefix)
-    pages = page_table if prefix_pages is None else prefix_pages
-    if prefix_pages is not None and (prefix_pages.dtype != torch.int32 or prefix_pages.numel() * pt < prefix):
-        raise ValueError("prefix_pages must be int32 and hold the prefix")
+    pages, pt, prefix = pool.shape[1], pool.shape[2], int(prefix)
+    if prefix_pages is None:
+        front = page_table
+    else:
+        front = prefix_pages
+        if front.dtype != i32 or front.numel() * pt < prefix:
+            raise ValueError("prefix_pages must be int32 and hold the prefix")
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=dt, device=dev)
-    elif out.shape != q.shape or out.dtype != dt or not out.is_contiguous():
+        out = torch.empty(shape, dtype=dt, device=dev)
+    elif out.shape != shape or out.dtype != dt or not out.is_contiguous():
         raise ValueError("out must be contiguous and like q")
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    s = _lib.Attention(
-        N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-        out.stride(1), base, _DTYPES[pool.dtype], pool.shape[1], pt, page_table.data_ptr(), width,
-        seq_lens.data_ptr(), ptr(cu_q), int(max_q if max_q is not None else max(N, 1)), int(max_len or 0), prefix,
-        pages.data_ptr(), D ** -0.5 if scale is None else float(scale), _scale(k_scale, dev, "k_scale"),
+    s = _lib.ATTENTION_FORMAT.pack(
+        N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q0, q1, out.data_ptr(), Hq * D, D, base, _DTYPES[pool_dt], pages,
+        pt, page_table.data_ptr(), width, seq_lens.data_ptr(), _ptr(cu_q),
+        max(N, 1) if max_q is None else int(max_q), int(max_len or 0), prefix, front.data_ptr(),
+        D ** -0.5 if scale is None else float(scale), _scale(k_scale, dev, "k_scale"),
         _scale(v_scale, dev, "v_scale"))
-    ref = ctypes.byref(s)
-    need = _lib.lib().kvec_prefix_attention_workspace(ref)
+    need = _lib.lib().kvec_prefix_attention_workspace(s)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _lib.call_on(dev, "kvec_prefix_attention", ref, ptr(ws), max(need, 0), _lib.stream_handle(dev))
+    _lib.call_on(dev, "kvec_prefix_attention", s, _ptr(ws), max(need, 0), _lib.stream_handle(dev))
     return out

@@ -1088,10 +1088,16 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     const uint64_t cap = uint64_t(s->pages_per_seq) * uint64_t(s->page_tokens);
     const uint64_t len = s->max_len > 0 && uint64_t(s->max_len) < cap ? uint64_t(s->max_len) : cap;
     p.rows = N * uint64_t(s->heads);
-    auto splits = [](uint64_t blocks, uint64_t want, uint64_t keys, uint64_t least) {
-        uint64_t n = want / (blocks ? blocks : 1);
-        const uint64_t most = keys / least;
-        if (n > most) n = most;
+    // Splits of `keys` keys: a block's time falls with them, the writing and
+    // joining of partial results (rows * dim) grows with them, so about the root
+    // of the quotient; no more than two blocks a compute unit, and 128 keys each.
+    // Measured, bf16, us: 2048 rows behind 8192 keys 49 (32 splits), 42 (16);
+    // 512 rows behind 4096 22 (32), 19 (16); 128 rows behind 512 16.6 (1), 11.7
+    // (4), 12.2 (8); one request of 32768 keys 43 (16), 33.5 (64).
+    auto splits = [&](uint64_t blocks, uint64_t keys) {
+        uint64_t n = 512 / (blocks ? blocks : 1);
+        if (n > keys / 128) n = keys / 128;
+        while (n > 1 && n * n * p.rows * uint64_t(s->dim) > keys * 6400) --n;
         return uint32_t(n < 1 ? 1 : n > 256 ? 256 : n);
     };
     // Requests with rows enough for tiles read the prefix with their own keys,
@@ -1106,9 +1112,9 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         p.flat_tile = all_rows > 2 * kStreamRows;
         const uint64_t bm = p.flat_tile ? kTileRows : kStreamRows;
         p.tiles_flat = uint32_t((all_rows + bm - 1) / bm);
-        p.parts_flat = splits(uint64_t(p.tiles_flat) * Hk, 512, prefix, 256);
+        p.parts_flat = splits(uint64_t(p.tiles_flat) * Hk, prefix);
     }
-    p.parts_own = splits(own, 512, len > p.first ? len - p.first : 1, 256);
+    p.parts_own = splits(own, len > p.first ? len - p.first : 1);
     p.blocks_flat = p.flat ? uint64_t(p.tiles_flat) * Hk * p.parts_flat : 0;
     p.blocks = p.blocks_flat + own * p.parts_own;
     return p;

@@ -15,7 +15,6 @@ takes both from the engine that it hooks, bench_ghostserve_rdp.py:440-458).
 """
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Sequence
 
 import torch
@@ -117,14 +116,15 @@ def step_tables(page_table: torch.Tensor, cached: torch.Tensor, new: torch.Tenso
     All tensors int32, contiguous, on one GPU; ``page_table`` [batch,
     pages_per_seq].  ``out``: an earlier result of the same sizes, written again.
     Nothing is read back to the host, so the call can be captured in a graph."""
-    if page_table.dim() != 2 or cached.dim() != 1 or new.dim() != 1 or free_pages.dim() != 1:
+    shape = page_table.shape
+    if len(shape) != 2 or cached.dim() != 1 or new.dim() != 1 or free_pages.dim() != 1:
         raise ValueError("page_table must be [batch, pages_per_seq], cached, new and free_pages one-dimensional")
-    B, width = page_table.shape
+    B, width = shape
     if cached.shape[0] != B or new.shape[0] != B:
         raise ValueError(f"cached and new must have one entry for each of {B} requests")
-    for t in (page_table, cached, new, free_pages):
-        if t.dtype != torch.int32:
-            raise ValueError("page_table, cached, new and free_pages must be int32")
+    i32 = torch.int32
+    if page_table.dtype != i32 or cached.dtype != i32 or new.dtype != i32 or free_pages.dtype != i32:
+        raise ValueError("page_table, cached, new and free_pages must be int32")
     dev = page_table.device
     _lib.require_cuda(page_table, cached, new, free_pages, what="step table")
     _lib.require_same_device(dev, cached, new, free_pages, what="step table")
@@ -132,19 +132,20 @@ def step_tables(page_table: torch.Tensor, cached: torch.Tensor, new: torch.Tenso
     if T < 0:
         raise ValueError("max_tokens must not be negative")
     if out is None:
-        buf = torch.empty(2 * T + 2 * B + 2, dtype=torch.int32, device=dev)
+        buf = torch.empty(2 * T + 2 * B + 2, dtype=i32, device=dev)
         out = StepTables(*buf.split_with_sizes([T, T, B + 1, B, 1]))
     else:
         for t, n in zip(out, (T, T, B + 1, B, 1)):
-            if t.dtype != torch.int32 or t.shape != (n,):
+            if t.dtype != i32 or t.shape != (n,):
                 raise ValueError("out is not of this step's sizes")
         _lib.require_cuda(*out, what="step table")
         _lib.require_same_device(dev, *out, what="step table")
-    s = _lib.Step(page_table.data_ptr(), B, width, int(page_tokens), int(pool_pages), cached.data_ptr(),
-                  new.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], out.slots.data_ptr(),
-                  out.positions.data_ptr(), T, out.cu_new.data_ptr(), out.seq_lens.data_ptr(),
-                  out.taken.data_ptr())
-    _lib.call_on(dev, "kvec_step_tables", ctypes.byref(s), _lib.stream_handle(dev))
+    slots, positions, cu_new, seq_lens, taken = out
+    s = _lib.STEP_FORMAT.pack(
+        page_table.data_ptr(), B, width, int(page_tokens), int(pool_pages), cached.data_ptr(), new.data_ptr(),
+        free_pages.data_ptr(), free_pages.shape[0], slots.data_ptr(), positions.data_ptr(), T, cu_new.data_ptr(),
+        seq_lens.data_ptr(), taken.data_ptr())
+    _lib.call_on(dev, "kvec_step_tables", s, _lib.stream_handle(dev))
     return out
 
 

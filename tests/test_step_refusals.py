@@ -199,3 +199,14 @@ def test_attention_python_refusals(pkg):
         pkg.attention.prefix_attention(q[:3], pool, i(4, 3), i(4))
     with pytest.raises(ValueError, match="int32"):
         pkg.attention.prefix_attention(q, pool, i(4, 3).long(), i(4))
+
+
+def test_packed_structs_are_the_structs(pkg):
+    """struct.pack's bytes are the C layouts': every field at its place."""
+    L = pkg._lib
+    for fmt, cls in ((L.STEP_FORMAT, L.Step), (L.NORM_ROTATE_FORMAT, L.NormRotate), (L.ATTENTION_FORMAT, L.Attention)):
+        vals = [float(i) + 0.5 if t is C.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        raw = fmt.pack(*vals)
+        got = cls.from_buffer_copy(raw.ljust(C.sizeof(cls), b"\0"))
+        assert [getattr(got, n) for n, _ in cls._fields_] == vals
+        assert len(raw) <= C.sizeof(cls) < len(raw) + 8
