@@ -144,7 +144,9 @@ struct AttnArgs {
     uint32_t parts_flat, parts_own;            // splits of the keys of each part
     uint32_t blocks_flat;                      // blocks of the shared part, before those of the own keys
     uint32_t tiles_flat, tiles_own;            // row tiles of each (upper bound)
-    uint32_t req_tiles;                        // stream blocks, own keys: row tiles of a request
+    FastDiv by_group, by_req_tiles;            // query heads of a K/V head; stream blocks: row tiles of a request
+    FastDiv by_flat, by_own;                   // splits of each part
+    FastDiv by_heads_flat, by_heads_own;       // K/V heads times splits
     int direct;                                // one part in all: outputs are final
     int wide_q, wide_o;                        // 16-byte rows
     float scale;
@@ -224,24 +226,25 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     Item it{};
     it.flat = id < a.blocks_flat;
     if (!it.flat) id -= a.blocks_flat;
-    const uint32_t parts = it.flat ? a.parts_flat : a.parts_own;
+    const FastDiv by_parts = it.flat ? a.by_flat : a.by_own, by_hp = it.flat ? a.by_heads_flat : a.by_heads_own;
+    const uint32_t parts = by_parts.d, hp = by_hp.d;
     uint32_t tiles = it.flat ? a.tiles_flat : a.tiles_own;
     if (!STREAM && !it.flat) {
         // as many tiles as there are, not the launch's bound: blocks without
         // work come last then, and no compute unit gets a third block for them
         tiles = __builtin_amdgcn_readfirstlane(tile_at(a, 0xFFFFFFFFu).first);
-        if (id >= tiles * parts * a.kv_heads) return it;
+        if (id >= tiles * hp) return it;
     }
     // Blocks go to the eight XCDs in turn: heads and splits first, so that with
     // eight K/V heads (and any eighth of the sizes that serve) an XCD's blocks
     // share their keys in its L2; and the tiles with the most keys, a request's
     // last ones, before the others (both: 1375 -> 1272 us for 8192 tokens behind
     // 8192 in four requests).
-    const uint32_t hp = parts * a.kv_heads, rest = id % hp;
-    uint32_t tile = id / hp;
+    uint32_t tile = fdiv(id, by_hp);
+    const uint32_t rest = id - tile * hp;
     if (!STREAM && !it.flat) tile = tiles - 1 - tile;
-    const uint32_t split = rest % parts;
-    it.head = rest / parts;
+    it.head = fdiv(rest, by_parts);
+    const uint32_t split = rest - it.head * parts;
     it.part = it.flat ? split : a.parts_flat + split;
     uint32_t first = 0, last;
     if (it.flat) {
@@ -252,8 +255,8 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     } else {
         uint32_t local;
         if (STREAM) {
-            it.b = tile / a.req_tiles;
-            local = tile % a.req_tiles;
+            it.b = fdiv(tile, a.by_req_tiles);
+            local = tile - it.b * a.by_req_tiles.d;
         } else {
             const TileAt t = tile_at(a, tile);
             it.b = __builtin_amdgcn_readfirstlane(t.b);
@@ -268,12 +271,12 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
         last = 0;
         if (it.live) {
             const uint32_t end_row = min(it.row0 + BM, it.rows) - 1;
-            last = seen_by(a, it.b, it.t0 + end_row / a.group);
+            last = seen_by(a, it.b, it.t0 + fdiv(end_row, a.by_group));
         }
     }
     // equal shares of the keys, in whole steps
     const uint32_t n = last > first ? last - first : 0u;
-    const uint32_t steps = (n + KEYS - 1) / KEYS, each = (steps + parts - 1) / parts;
+    const uint32_t steps = (n + KEYS - 1) / KEYS, each = fdiv(steps + parts - 1, by_parts);
     it.k0 = first + min(uint64_t(split) * each * KEYS, uint64_t(n));
     it.k1 = first + min(uint64_t(split + 1) * each * KEYS, uint64_t(n));
     return it;
@@ -434,42 +437,10 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t r = lane & 31, h = lane >> 5;
     T* const ty = nullptr;
-
-    // the lane's row
-    const uint32_t row = it.row0 + wave * 32 + r;
-    const bool has = row < it.rows;
-    const uint32_t token = it.t0 + (has ? row / a.group : 0u);
-    const uint32_t head = it.head * a.group + (has ? row % a.group : 0u);
-    // rows that are not there, and rows that see nothing, ask for no mask
-    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
-    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
-    // 0 would make NaN of a masked score; a negative one goes to the query
-    const float c0 = score_factor(a);
-    const uint32_t sign = c0 < 0.0f ? 0x80008000u : 0u;
-    u32x4 qf[KS];
-    {
-        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, uint32_t(s * 16) + h * 8) ^ sign;
-    }
-    // the fewest keys that a row of the wave, and of the block, sees
-    uint32_t low = limit;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
-    low = __builtin_amdgcn_readfirstlane(low);
-    if (lane == 0) lows[wave] = low;
     if (tid == 0) odd = 0;
-    __syncthreads();
-    const uint32_t block_low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
+    if constexpr (FP8) __syncthreads();                   // before a value is taken out
 
-    const float c = fabsf(c0);
-    const float lazy = kLazy / c;
-    float m = -INFINITY, l = 0.0f, mc = 0.0f, bar = -INFINITY;   // bar: the score that moves m
-    f32x16 o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = f32x16{};
-
-    const uint32_t row_bytes = a.token_bytes / a.kv_heads, head_off = it.head * row_bytes;
+    const uint32_t row_bytes = a.dim * (FP8 ? 1 : 2), head_off = it.head * row_bytes;
     // V values that are not finite become 0
     auto scrub = [&](u32x4 v) {
         const uint32_t e = exponent_bits(ty);
@@ -539,6 +510,84 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             }
         }
     };
+    const uint32_t units = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
+    const int32_t* const own_row = a.table + uint64_t(it.b) * a.width;
+    // key_page of a unit's keys, by one row where they lie on one side of the prefix's end
+    auto unit_page = [&](uint32_t base, uint32_t key) __attribute__((always_inline)) {
+        if (!it.flat && base < a.prefix && base + kTileKeys > a.prefix) return key_page(a, it, base + key);
+        const int32_t* row = it.flat || base < a.prefix ? a.prefix_pages : own_row;
+        return uint32_t(as_global(row)[min(base + key, it.k1 - 1) >> a.shift]);
+    };
+    const uint32_t key = lane & 31;
+    // The first units, asked for before anything else is: the queries and their
+    // limits come while these are on their way.
+    // of the lane's key: pages of units j + 3 and j + 4; and which keys of units
+    // j, j + 1 and j + 2 are there
+    uint32_t page3 = 0, page4 = 0, valid0 = 0, valid1 = 0, valid2 = 0, slot2 = 0;
+    if (units) {
+        const uint32_t pg0 = unit_page(it.k0, key), pg1 = unit_page(it.k0 + kTileKeys, key);
+        const uint32_t pg2 = unit_page(it.k0 + 2 * kTileKeys, key);
+        page3 = unit_page(it.k0 + 3 * kTileKeys, key);
+        page4 = unit_page(it.k0 + 4 * kTileKeys, key);
+        const uint32_t s0 = page_slot(a, it, it.k0 + key, pg0), s1 = page_slot(a, it, it.k0 + kTileKeys + key, pg1);
+        slot2 = page_slot(a, it, it.k0 + 2 * kTileKeys + key, pg2);
+        valid0 = uint32_t(__ballot(s0 != kNoCell));
+        valid1 = uint32_t(__ballot(s1 != kNoCell));
+        valid2 = uint32_t(__ballot(slot2 != kNoCell));
+        if constexpr (!FP8) {
+            load_k(s0, k0);
+            load_v(v0);
+            load_k(s1, k1);
+            load_v(v1);
+            load_k(slot2, k2);
+        } else {
+            // one unit at a time in registers; the last one's K stays there
+            load_k(s0, k0);
+            load_v(v0);
+            put_fp8(xk, false, k0, false);
+            put_fp8(xv, true, v0, true);
+            load_k(s1, k1);
+            load_v(v1);
+            put_fp8(xk, false, k1, false);
+            put_fp8(xv, true, v1, true);
+            load_k(slot2, k2);
+            put_fp8(xk, false, k2, false);
+        }
+    }
+
+    // the lane's row
+    const uint32_t row = it.row0 + wave * 32 + r;
+    const bool has = row < it.rows;
+    const uint32_t tok = has ? fdiv(row, a.by_group) : 0u;
+    const uint32_t token = it.t0 + tok, head = it.head * a.group + (has ? row - tok * a.group : 0u);
+    // rows that are not there, and rows that see nothing, ask for no mask
+    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
+    // 0 would make NaN of a masked score; a negative one goes to the query
+    const float c0 = score_factor(a);
+    const uint32_t sign = c0 < 0.0f ? 0x80008000u : 0u;
+    u32x4 qf[KS];
+    {
+        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, uint32_t(s * 16) + h * 8) ^ sign;
+    }
+    // the fewest keys that a row of the wave, and of the block, sees
+    uint32_t low = limit;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
+    low = __builtin_amdgcn_readfirstlane(low);
+    if (lane == 0) lows[wave] = low;
+    __syncthreads();
+    const uint32_t block_low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
+
+    const float c = fabsf(c0);
+    const float lazy = kLazy / c;
+    float m = -INFINITY, l = 0.0f, mc = 0.0f, bar = -INFINITY;   // bar: the score that moves m
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+
     // places in a unit of K and V that the lane reads
     uint32_t at_k[KS], at_v[DB];
     {
@@ -574,42 +623,12 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
         return max_halves(top);
     };
 
-    const uint32_t units = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
-    const int32_t* const own_row = a.table + uint64_t(it.b) * a.width;
-    // key_page of a unit's keys, by one row where they lie on one side of the prefix's end
-    auto unit_page = [&](uint32_t base, uint32_t key) __attribute__((always_inline)) {
-        if (!it.flat && base < a.prefix && base + kTileKeys > a.prefix) return key_page(a, it, base + key);
-        const int32_t* row = it.flat || base < a.prefix ? a.prefix_pages : own_row;
-        return uint32_t(as_global(row)[min(base + key, it.k1 - 1) >> a.shift]);
-    };
-    const uint32_t key = lane & 31;
     f32x16 sa, sb;
     float top = -INFINITY;
-    // of the lane's key: pages of units j + 3 and j + 4; and which keys of units
-    // j + 1 and j + 2 are there
-    uint32_t page3 = 0, page4 = 0, valid1 = 0, valid2 = 0;
     if (units) {
-        const uint32_t s0 = key_slot(a, it, it.k0 + key), s1 = key_slot(a, it, it.k0 + kTileKeys + key);
-        const uint32_t s2 = key_slot(a, it, it.k0 + 2 * kTileKeys + key);
-        page3 = unit_page(it.k0 + 3 * kTileKeys, key);
-        page4 = unit_page(it.k0 + 4 * kTileKeys, key);
-        const uint32_t first[3] = {s0, s1, s2};
-        uint8_t* const ks[3] = {k0, k1, k2};
-        uint8_t* const vs[2] = {v0, v1};
-#pragma unroll
-        for (int u = 0; u < 3; ++u) {
-            load_k(first[u], ks[u]);
-            if (u < 2) load_v(vs[u < 2 ? u : 0]);
-            if constexpr (FP8) {
-                put_fp8(xk, false, ks[u], false);
-                if (u < 2) put_fp8(xv, true, vs[u < 2 ? u : 0], it.k0 + (u + 1) * kTileKeys > block_low);
-            }
-        }
-        valid1 = uint32_t(__ballot(s1 != kNoCell));
-        valid2 = uint32_t(__ballot(s2 != kNoCell));
         meet();
         sa = scores(k0);
-        top = masked(sa, largest(sa), it.k0, uint32_t(__ballot(s0 != kNoCell)));
+        top = masked(sa, largest(sa), it.k0, valid0);
     }
     // Step j: K of unit j + 1 and V of unit j are read, K of unit j + 3 (its
     // lane's slot: `slot`) and V of unit j + 2 loaded.
@@ -709,7 +728,8 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 
     // V values that were taken out, to the rows that see them
     if (odd) {
-        const uint32_t skip = block_low > it.k0 ? (block_low - it.k0) / kTileKeys * kTileKeys : 0u;
+        // (fp8: the first units are looked through before the limits are known)
+        const uint32_t skip = !FP8 && block_low > it.k0 ? (block_low - it.k0) / kTileKeys * kTileKeys : 0u;
         for (uint32_t kk = it.k0 + skip; kk < it.k1; ++kk) {
             const uint32_t sl = kk < limit ? key_slot(a, it, kk) : kNoCell;
 #pragma unroll
@@ -733,7 +753,9 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     const uint32_t at_row = it.row0 + wave * 32 + (anew(lane) & 31);
     if (at_row >= it.rows) return;
     LateArgs& e = late_args();
-    const uint32_t to_token = it.t0 + at_row / e.group, to_head = it.head * e.group + at_row % e.group;
+    const FastDiv by_group = {e.by_group.d, e.by_group.m, e.by_group.s1, e.by_group.s2};
+    const uint32_t to_tok = fdiv(at_row, by_group);
+    const uint32_t to_token = it.t0 + to_tok, to_head = it.head * e.group + at_row - to_tok * e.group;
     const float vs = e.v_scale ? *e.v_scale : 1.0f;
     const float inv = l > 0.0f ? vs / l : l == l ? 0.0f : l;
     if (!e.direct && anew(h) == 0) {
@@ -770,34 +792,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
     T* const ty = nullptr;
     uint8_t* const lv = wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3;
 
-    const uint32_t row = it.row0 + r;
-    const bool has = row < it.rows;
-    const uint32_t token = it.t0 + (has ? row / a.group : 0u);
-    const uint32_t head = it.head * a.group + (has ? row % a.group : 0u);
-    // rows that are not there, and rows that see nothing, ask for no mask
-    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
-    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
-    // 0 would make NaN of a masked score; a negative one goes to the query
-    const float c0 = score_factor(a);
-    const uint32_t sign = c0 < 0.0f ? 0x80008000u : 0u;
-    u32x4 qf[KS];
-    {
-        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, uint32_t(s * 32) + g * 8) ^ sign;
-    }
-    uint32_t low = limit;
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
-    low = __builtin_amdgcn_readfirstlane(low);
-
-    const float c = fabsf(c0);
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
-
-    const uint32_t row_bytes = a.token_bytes / a.kv_heads, head_off = it.head * row_bytes;
+    const uint32_t row_bytes = a.dim * (FP8 ? 1 : 2), head_off = it.head * row_bytes;
     u32x4 xv[PER];
     u32x4 xk[2][KS];                                      // fp8: 8 bytes of each
     auto fetch = [&](uint32_t slot) {                     // slot: of the keys lane % 32
@@ -846,6 +841,34 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
         fetch(slot);
         slot_next = key_slot(a, it, it.k0 + (wave + 4) * kStreamKeys + (lane & 31));
     }
+    // the queries and their limits, while the first keys are on their way
+    const uint32_t row = it.row0 + r;
+    const bool has = row < it.rows;
+    const uint32_t tok = has ? fdiv(row, a.by_group) : 0u;
+    const uint32_t token = it.t0 + tok, head = it.head * a.group + (has ? row - tok * a.group : 0u);
+    // rows that are not there, and rows that see nothing, ask for no mask
+    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
+    // 0 would make NaN of a masked score; a negative one goes to the query
+    const float c0 = score_factor(a);
+    const uint32_t sign = c0 < 0.0f ? 0x80008000u : 0u;
+    u32x4 qf[KS];
+    {
+        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, uint32_t(s * 32) + g * 8) ^ sign;
+    }
+    uint32_t low = limit;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
+    low = __builtin_amdgcn_readfirstlane(low);
+
+    const float c = fabsf(c0);
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
+
     for (uint32_t n = wave; n < nblk; n += 4) {
         const uint32_t base = it.k0 + n * kStreamKeys;
         const uint32_t valid = uint32_t(__ballot(slot != kNoCell));
@@ -985,7 +1008,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 #pragma unroll
         for (int w = 0; w < 4; ++w)
             sum += lm[w][rr] == -INFINITY ? 0.0f : ll[w][rr] * __builtin_amdgcn_exp2f((lm[w][rr] - mx) * c);
-        const uint32_t tk = it.t0 + rw / a.group, hd = it.head * a.group + rw % a.group;
+        const uint32_t tr = fdiv(rw, a.by_group), tk = it.t0 + tr, hd = it.head * a.group + rw - tr * a.group;
         if (!a.direct && d == 0) {
             const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(tk) * a.heads + hd;
             *as_global(a.ws_ml + at) = f32x2{mx == -INFINITY ? -INFINITY : mx * c, sum};
@@ -1224,7 +1247,12 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.blocks_flat = uint32_t(p.blocks_flat);
     a.tiles_flat = p.tiles_flat;
     a.tiles_own = p.tiles_own;
-    a.req_tiles = p.req_tiles;
+    a.by_group = make_fastdiv(a.group);
+    a.by_req_tiles = make_fastdiv(p.req_tiles);
+    a.by_flat = make_fastdiv(p.parts_flat ? p.parts_flat : 1);
+    a.by_own = make_fastdiv(p.parts_own);
+    a.by_heads_flat = make_fastdiv(a.kv_heads * a.by_flat.d);
+    a.by_heads_own = make_fastdiv(a.kv_heads * p.parts_own);
     a.direct = p.direct();
     a.scale = s->scale;
     a.wide_q = aligned16(s->q) && s->q_stride % 8 == 0 && s->q_head_stride % 8 == 0;
