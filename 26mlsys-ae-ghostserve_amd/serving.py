@@ -36,6 +36,8 @@ What differs:
   * the H2D "probe" copy is made only when asked for (``probe_h2d=True``);
   * any backend with ``forward_extend`` is hooked, not only FlashInfer's
     (ROCm serving backends are not FlashInfer).
+:class:`PagedBackend` is a backend of the package's own for the hook: page tables,
+cache writes and attention over a paged pool by this library's kernels.
 The gather of rows to dst is the reference's, and kept: dst receives one row
 per other rank, each over its own link of a fully connected node, whereas
 XOR-reducing per-rank parity contributions would bring it two rows (P's and
@@ -49,12 +51,12 @@ import json
 import math
 import os
 import time
-from typing import Callable, Optional
+from typing import Callable, NamedTuple, Optional
 
 import numpy as np
 import torch
 
-from . import _lib, paged
+from . import _lib, attention, paged
 
 
 def _dist():
@@ -430,3 +432,66 @@ def install(model_runner, hook: Optional[KVParityHook] = None,
     backend.forward_extend = forward_extend
     backend._kvec_hooked = hook
     return hook
+
+
+class ExtendBatch(NamedTuple):
+    """One step of a :class:`PagedBackend` (``slot_mapping`` as the hook reads it)."""
+    slot_mapping: torch.Tensor   # int32 [tokens], -1 where a token has no slot
+    positions: torch.Tensor      # int32 [tokens]
+    cu_new: torch.Tensor         # int32 [batch + 1]
+    seq_lens: torch.Tensor       # int32 [batch], with the step's tokens
+    taken: torch.Tensor          # int32 [1], pages taken of the free list
+    max_new: int
+    max_len: int
+
+
+class PagedBackend:
+    """An attention backend over one layer of a paged K/V pool, in the shape that
+    :func:`install` hooks: ``forward_extend(batch, q, k, v)`` norms and rotates the
+    step's queries and keys, writes K and V to their slots and attends over the
+    pool, the requests' shared prefix once for all; the hook then codes the
+    slots that it wrote.  A decode step is one new token a request.
+
+    ``pool``: [layers, pages, page_tokens, 2, kv_heads, head_dim];
+    ``page_table``: int32 [batch, pages_per_seq], whose rows start with the prefix's
+    pages (whole pages where requests go on behind it).  ``freqs``, weights, ``eps``,
+    ``axis_of``, ``interleaved``, ``factor`` and scales as in
+    :func:`.attention.norm_rotate_write`.  The hook codes pools of 2-byte types."""
+
+    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, layer: int = 0, prefix: int = 0,
+                 freqs: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None, **norm):
+        if pool.dim() != 6 or pool.shape[3] != 2:
+            raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
+        if not 0 <= layer < pool.shape[0]:
+            raise ValueError(f"layer {layer} not in [0, {pool.shape[0]})")
+        self.pool, self.page_table, self.layer, self.prefix = pool, page_table, int(layer), int(prefix)
+        self.freqs, self.k_scale, self.v_scale, self.scale, self.norm = freqs, k_scale, v_scale, scale, norm
+
+    @property
+    def kv_buffer(self) -> torch.Tensor:
+        """The layer as a token pool, [max_tokens, 2, kv_heads, head_dim]."""
+        _, pages, pt, _, H, D = self.pool.shape
+        return self.pool[self.layer].view(pages * pt, 2, H, D)
+
+    def begin(self, cached: torch.Tensor, new: torch.Tensor, free_pages: torch.Tensor, tokens: int,
+              max_new: int, max_len: Optional[int] = None) -> ExtendBatch:
+        """The step in which request b, holding ``cached[b]`` tokens, gets ``new[b]``:
+        pages from ``free_pages`` into the page table, slots and positions
+        (:func:`.paged.step_tables`).  ``tokens``: all new tokens (or more: the rest is
+        padding); ``max_new``, ``max_len``: the most of a request."""
+        _, pages, pt, _, _, _ = self.pool.shape
+        t = paged.step_tables(self.page_table, cached, new, free_pages, pages, pt, tokens)
+        return ExtendBatch(t.slots, t.positions, t.cu_new, t.seq_lens, t.taken, int(max_new),
+                           int(max_len or self.page_table.shape[1] * pt))
+
+    def forward_extend(self, batch: ExtendBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Attention of the step's tokens ([tokens, heads, head_dim], K/V heads for k
+        and v); rows behind the last request's are zeros."""
+        q = attention.norm_rotate_write(
+            q, k, v, batch.positions, self.freqs, self.pool, batch.slot_mapping, layer=self.layer,
+            k_scale=self.k_scale, v_scale=self.v_scale, **self.norm)
+        return attention.prefix_attention(
+            q, self.pool, self.page_table, batch.seq_lens, self.prefix, layer=self.layer, cu_q=batch.cu_new,
+            max_q=batch.max_new, max_len=batch.max_len, scale=self.scale, k_scale=self.k_scale,
+            v_scale=self.v_scale, out=torch.zeros_like(q))

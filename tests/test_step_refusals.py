@@ -210,3 +210,15 @@ def test_packed_structs_are_the_structs(pkg):
         got = cls.from_buffer_copy(raw.ljust(C.sizeof(cls), b"\0"))
         assert [getattr(got, n) for n, _ in cls._fields_] == vals
         assert len(raw) <= C.sizeof(cls) < len(raw) + 8
+
+
+def test_paged_backend_shape_checks(pkg):
+    serving = pkg.serving
+    pool = torch.zeros(2, 6, 4, 2, 1, 8)
+    be = serving.PagedBackend(pool, torch.zeros(1, 3, dtype=torch.int32), layer=1)
+    assert be.kv_buffer.shape == (24, 2, 1, 8)
+    assert be.kv_buffer.data_ptr() == pool[1].data_ptr()
+    with pytest.raises(ValueError, match="layer"):
+        serving.PagedBackend(pool, torch.zeros(1, 3, dtype=torch.int32), layer=2)
+    with pytest.raises(ValueError, match="pool"):
+        serving.PagedBackend(pool[0], torch.zeros(1, 3, dtype=torch.int32))
