@@ -289,10 +289,14 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     NrArgs a{};
     while ((1u << a.lg) < units && a.lg < 6) ++a.lg;
     const uint32_t groups = 64u >> a.lg, rows = uint32_t(s->heads) + 2 * uint32_t(s->kv_heads);
-    // A wave takes three rows of each group where there are waves enough to
-    // fill the card eight deep; a short step spreads its rows instead (latency).
+    // A wave takes three rows of each group where there are waves for the card
+    // twelve times over: what the rows share is loaded once.  Fewer are spread out
+    // (latency, and the data lies in the caches between kernels then).  Measured,
+    // us, one row and three: 32 + 2 x 8 heads of 128, 4096 tokens 20.3, 23.3; 16384
+    // 82.5, 84.5; 32768 164.7, 158.3; three axes, 28 + 2 x 4 heads, 8192 tokens 29.1,
+    // 31.6; 16384 69.9, 67.6; 65536 270.9, 246.7.
     const uint64_t waves1 = uint64_t(s->tokens) * ((rows + groups - 1) / groups);
-    const bool deep = wide && waves1 >= 3 * 256 * 32;
+    const bool deep = wide && waves1 >= 12 * 256 * 32;
     const uint32_t per = groups * (deep ? 3 : 1), chunks = (rows + per - 1) / per;
     if (uint64_t(s->tokens) * chunks >= (uint64_t(1) << 32) - 4)
         return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
