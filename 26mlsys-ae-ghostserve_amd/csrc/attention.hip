@@ -10,7 +10,7 @@
 // request.  Each request's own keys are a second part; parts are joined by
 // their maxima and sums, which are linear once both are brought to one maximum.
 //
-// Both kernels form S^T = K Q^T and O^T += V^T P^T, keys along the rows of the
+// Two kinds of blocks, one kernel.  Both form S^T = K Q^T and O^T += V^T P^T, keys along the rows of the
 // matrix instructions and query rows along their columns: a lane then holds
 // scores of one query row only, so the softmax needs one exchange between lane
 // halves (or quarters) for the maximum and none for the sum, and the scores
@@ -28,7 +28,7 @@
 // a page holds behind its last token (NaN, say) has no part.  Where some rows of
 // a tile see a key and others do not, a V value that is not finite would reach
 // the others as 0 * NaN: such values are taken out of the product and added to
-// the rows that see them (add_not_finite).
+// the rows that see them after the loop.
 #include "lm_types.h"
 #include "paged_geom.h"
 
@@ -1094,8 +1094,8 @@ AttnFn pick_attn(bool flat_tile, bool own_tile, int dim) {
 
 struct AttnPlan {
     bool flat, flat_tile, own_tile;
-    uint32_t parts_flat, parts_own, tiles_flat, tiles_own, req_tiles, first;
-    uint64_t rows, blocks_flat, blocks;
+    uint32_t parts_flat, parts_own, tiles_flat, req_tiles, first;
+    uint64_t rows, tiles_own, blocks_flat, blocks;
     bool direct() const { return parts_flat + parts_own == 1; }
     int64_t bytes(int64_t dim) const {
         return direct() ? 0 : int64_t(uint64_t(parts_flat + parts_own) * rows * (uint64_t(dim) * 4 + 8)) + 16;
@@ -1106,7 +1106,7 @@ struct AttnPlan {
 inline AttnPlan plan_attention(const kvec_attention* s) {
     AttnPlan p{};
     const uint64_t group = uint64_t(s->heads / s->kv_heads), N = uint64_t(s->tokens), B = uint64_t(s->batch);
-    const uint64_t max_q = s->cu_q ? uint64_t(s->max_q) : 1, Hk = uint64_t(s->kv_heads);
+    const uint64_t max_q = s->cu_q ? min(uint64_t(s->max_q), N) : 1, Hk = uint64_t(s->kv_heads);
     const uint64_t req_rows = max_q * group, all_rows = N * group, prefix = uint64_t(s->prefix);
     const uint64_t cap = uint64_t(s->pages_per_seq) * uint64_t(s->page_tokens);
     const uint64_t len = s->max_len > 0 && uint64_t(s->max_len) < cap ? uint64_t(s->max_len) : cap;
@@ -1123,12 +1123,22 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         while (n > 1 && n * n * p.rows * uint64_t(s->dim) > keys * 6400) --n;
         return uint32_t(n < 1 ? 1 : n > 256 ? 256 : n);
     };
-    // Requests with rows enough for tiles read the prefix with their own keys,
-    // without partial results to write and join.
-    p.own_tile = req_rows > 4 * kStreamRows;
-    p.req_tiles = uint32_t((req_rows + kStreamRows - 1) / kStreamRows);
-    p.tiles_own = p.own_tile ? uint32_t(all_rows / kTileRows) + uint32_t(B) : uint32_t(B) * p.req_tiles;
-    const uint64_t own = uint64_t(p.tiles_own) * Hk;
+    // A request's rows as tiles of 128, which read the prefix with the own keys,
+    // or as stream blocks of 16 behind the shared part: by the keys that either's
+    // blocks go through, a stream block's at three fifths of a tile's.  Measured,
+    // bf16, four query heads to a K/V head, us (stream, tile): 64 requests of
+    // 1024 own keys with 16 rows 36, 41, with 64 rows 79, 42; 64 of 500 behind
+    // 4096 with 64 rows 110, 149, with 128 rows 182, 156; behind 512 with 48
+    // rows 60, 44.  Where few requests leave compute units idle the stream
+    // blocks, being more, can be ahead for longer (16 of 500 behind 4096 with
+    // 128 rows 57, 62).
+    const uint64_t own_keys = len > prefix ? len - prefix : 0;
+    const uint64_t by16 = (req_rows + kStreamRows - 1) / kStreamRows, by128 = (req_rows + kTileRows - 1) / kTileRows;
+    p.own_tile = 0.6 * double(own_keys) * double(by16) + double(prefix) * double(req_rows) / kTileRows >
+                 double(prefix + own_keys) * double(by128);
+    p.req_tiles = uint32_t(by16);
+    p.tiles_own = p.own_tile ? min(all_rows / kTileRows + B, B * by128) : B * by16;
+    const uint64_t own = p.tiles_own * Hk;
     p.flat = prefix > 0 && !p.own_tile;
     if (p.flat) {
         p.first = uint32_t(prefix);
@@ -1195,6 +1205,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     if ((s->heads > 1 && s->o_head_stride < s->dim) || (s->tokens > 1 && s->o_stride < s->dim))
         return set_error(KVEC_EINVAL, "%s: rows of out overlap", fn);
     const AttnPlan p = plan_attention(s);
+    if (p.blocks >= (uint64_t(1) << 31)) return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks", fn);
     const int64_t need = p.bytes(s->dim);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return set_error(KVEC_EINVAL, "%s: workspace of %lld bytes, 16-byte aligned, wanted", fn, (long long)need);
@@ -1246,7 +1257,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.parts_own = p.parts_own;
     a.blocks_flat = uint32_t(p.blocks_flat);
     a.tiles_flat = p.tiles_flat;
-    a.tiles_own = p.tiles_own;
+    a.tiles_own = uint32_t(p.tiles_own);
     a.by_group = make_fastdiv(a.group);
     a.by_req_tiles = make_fastdiv(p.req_tiles);
     a.by_flat = make_fastdiv(p.parts_flat ? p.parts_flat : 1);
@@ -1262,7 +1273,6 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
         a.ws_ml = (f32x2*)((uint8_t*)workspace + uint64_t(p.parts_flat + p.parts_own) * p.rows * uint64_t(s->dim) * 4);
     }
     const bool fp8 = s->pool_dtype == KVEC_FP8_E4M3, bf = s->dtype == KVEC_BF16;
-    if (p.blocks >= (uint64_t(1) << 31)) return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks", fn);
     AttnFn f = bf ? (fp8 ? pick_attn<__bf16, true>(p.flat_tile, p.own_tile, s->dim)
                          : pick_attn<__bf16, false>(p.flat_tile, p.own_tile, s->dim))
                   : (fp8 ? pick_attn<_Float16, true>(p.flat_tile, p.own_tile, s->dim)

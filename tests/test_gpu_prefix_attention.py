@@ -167,6 +167,20 @@ def test_extend(pkg, gpu, dtype, pool, D, new, prefix):
     check(run(pkg, c, cu_q=c["cu"], max_q=max(new), **sc), reference(c, **kw))
 
 
+@pytest.mark.parametrize("prefix,own", [(0, 90), (40, 300), (500, 30), (500, 0)])
+@pytest.mark.parametrize("n", [4, 8, 12, 16, 24, 32, 33, 64])
+def test_rows_of_a_request(pkg, gpu, n, prefix, own):
+    """A request's rows from one stream block's to two tiles', with much or little
+    of its keys in the prefix: either kind of block, chosen by max_len too."""
+    new = [n, 1, n - 3]
+    lens = [prefix + own + m for m in new]
+    c = make(gpu, n + prefix, lens, new, 8, 2, 64, BF, BF, 16, prefix)
+    ref = reference(c)
+    for max_len in (None, max(lens), prefix + 1):
+        check(run(pkg, c, max_q=n, max_len=max_len), ref)
+    check(run(pkg, c, max_q=(1 << 31) - 1), ref)
+
+
 def test_queries_inside_the_prefix(pkg, gpu):
     """A request may end inside the prefix, and have more tokens than keys: its
     queries see what lies before them, the first ones nothing."""

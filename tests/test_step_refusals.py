@@ -186,6 +186,18 @@ def test_attention_workspace(pkg):
     assert L.kvec_prefix_attention(C.byref(at(pkg, tokens=0, batch=0, q=None)), None, 0, None) == 0
 
 
+@pytest.mark.parametrize("kw", [{}, {"prefix": 0}, {"heads": 64}, {"tokens": 300}, {"tokens": 300, "prefix": 0}])
+def test_attention_longest_request(pkg, kw):
+    """No request has more tokens than there are: a larger max_q splits the same."""
+    L = pkg._lib.lib()
+    call = at(pkg, cu_q=1 << 26, **kw)
+    need = []
+    for m in (call.tokens, call.tokens + 1, 1 << 24, (1 << 31) - 1):
+        call.max_q = m
+        need.append(L.kvec_prefix_attention_workspace(C.byref(call)))
+    assert need[0] >= 0 and need == [need[0]] * 4
+
+
 def test_attention_python_refusals(pkg):
     i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
     q, pool = torch.zeros(4, 8, 64, dtype=torch.half), torch.zeros(1, 8, 16, 2, 2, 64, dtype=torch.half)
