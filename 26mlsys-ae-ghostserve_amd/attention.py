@@ -168,8 +168,8 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
     share K/V heads in order.  dim: a multiple of 8 (fp8 pool: 16) up to 256.
 
     The first ``prefix`` positions are the same for all requests; they are read
-    from ``prefix_pages`` (default: the first row of ``page_table``) once for all
-    queries.  ``prefix`` need not be whole pages.  0 is ordinary paged attention.
+    from ``prefix_pages`` (default: the first row of ``page_table``, which has to hold
+    them even if its request is idle) once for all queries.  ``prefix`` need not be whole pages.  0 is ordinary paged attention.
 
     Keys on pages outside the pool are left out; a query that sees no key (an idle
     row: ``seq_lens`` 0) gives zeros.  Rows from ``cu_q[-1]`` on are left as they

@@ -454,19 +454,24 @@ class PagedBackend:
 
     ``pool``: [layers, pages, page_tokens, 2, kv_heads, head_dim];
     ``page_table``: int32 [batch, pages_per_seq], whose rows start with the prefix's
-    pages (whole pages where requests go on behind it).  ``freqs``, weights, ``eps``,
+    pages (whole pages where requests go on behind it).  ``prefix_pages``: those pages
+    on their own, int32; without it they are read from the first row, whose request
+    then has to hold them in every step: a row that :meth:`begin` is given no
+    tokens for, cached or new, is emptied.  ``freqs``, weights, ``eps``,
     ``axis_of``, ``interleaved``, ``factor`` and scales as in
     :func:`.attention.norm_rotate_write`.  The hook codes pools of 2-byte types."""
 
     def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, layer: int = 0, prefix: int = 0,
                  freqs: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
-                 v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None, **norm):
+                 v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                 prefix_pages: Optional[torch.Tensor] = None, **norm):
         if pool.dim() != 6 or pool.shape[3] != 2:
             raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
         if not 0 <= layer < pool.shape[0]:
             raise ValueError(f"layer {layer} not in [0, {pool.shape[0]})")
         self.pool, self.page_table, self.layer, self.prefix = pool, page_table, int(layer), int(prefix)
         self.freqs, self.k_scale, self.v_scale, self.scale, self.norm = freqs, k_scale, v_scale, scale, norm
+        self.prefix_pages = prefix_pages
 
     @property
     def kv_buffer(self) -> torch.Tensor:
@@ -493,5 +498,5 @@ class PagedBackend:
             k_scale=self.k_scale, v_scale=self.v_scale, **self.norm)
         return attention.prefix_attention(
             q, self.pool, self.page_table, batch.seq_lens, self.prefix, layer=self.layer, cu_q=batch.cu_new,
-            max_q=batch.max_new, max_len=batch.max_len, scale=self.scale, k_scale=self.k_scale,
-            v_scale=self.v_scale, out=torch.zeros_like(q))
+            max_q=batch.max_new, max_len=batch.max_len, prefix_pages=self.prefix_pages, scale=self.scale,
+            k_scale=self.k_scale, v_scale=self.v_scale, out=torch.zeros_like(q))

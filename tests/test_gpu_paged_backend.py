@@ -230,3 +230,28 @@ def test_fp8_pool(pkg, gpu):
     # the values are within half a step of the 8-bit type of what was written
     err = (kv[:, 1] * float(vs) - v.double().cpu()).abs()
     assert (err <= v.double().cpu().abs() * 2.0 ** -4 * 1.01 + float(vs) * 2.0 ** -10).all()
+
+
+def test_first_request_leaves(pkg, gpu):
+    """The request whose row the prefix came from ends, and its row is emptied: with
+    the prefix's pages given on their own the others still see them."""
+    prefix = 48
+    g, be, model, free, dims = setup(pkg, gpu, seed=6, prefix=prefix)
+    B, Hq, Hk, D, P = dims
+    at = start_prefix(be, model, g, free, dims, prefix, gpu)
+    be.prefix_pages = be.page_table[0, :prefix // P].clone()
+    d = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device=gpu)  # noqa: E731
+    for new in ([0, 1, 1, 1, 1], [0, 20, 0, 3, 7]):
+        cached = [0] + [m.shape[0] for m in model.k[1:]]
+        n = sum(new)
+        batch = be.begin(d(cached), d(new), free[at:].to(gpu), n, max(new))
+        q, k, v = tokens(g, n, Hq, Hk, D)
+        out = be.forward_extend(batch, q.to(gpu), k.to(gpu), v.to(gpu)).cpu()
+        at += int(batch.taken)
+        assert (be.page_table[0] == -1).all()
+        t = 0
+        for b in range(B):
+            if new[b]:
+                r = slice(t, t + new[b])
+                near(out[r], model.extend(b, q[r], k[r], v[r]), f"request {b}")
+            t += new[b]
