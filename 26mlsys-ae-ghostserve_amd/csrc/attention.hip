@@ -1117,8 +1117,9 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     // Measured, bf16, us: 2048 rows behind 8192 keys 49 (32 splits), 42 (16);
     // 512 rows behind 4096 22 (32), 19 (16); 128 rows behind 512 16.6 (1), 11.7
     // (4), 12.2 (8); one request of 32768 keys 43 (16), 33.5 (64).
-    auto splits = [&](uint64_t blocks, uint64_t keys) {
-        uint64_t n = 512 / (blocks ? blocks : 1);
+    auto splits = [&](uint64_t blocks, uint64_t keys, uint64_t room) {
+        blocks = blocks ? blocks : 1;
+        uint64_t n = min((room + blocks / 2) / blocks, 512 / blocks);
         if (n > keys / 128) n = keys / 128;
         while (n > 1 && n * n * p.rows * uint64_t(s->dim) > keys * 6400) --n;
         return uint32_t(n < 1 ? 1 : n > 256 ? 256 : n);
@@ -1145,9 +1146,22 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         p.flat_tile = all_rows > 2 * kStreamRows;
         const uint64_t bm = p.flat_tile ? kTileRows : kStreamRows;
         p.tiles_flat = uint32_t((all_rows + bm - 1) / bm);
-        p.parts_flat = splits(uint64_t(p.tiles_flat) * Hk, prefix);
+        // Tile blocks of the shared part leave places to the stream blocks beside
+        // them, as the two take time: a tile's keys by the matrix units, a
+        // request's by memory, whose bytes a value count in.  Measured, us, with
+        // all places and with their share: 256 requests of 1024 own fp8 keys
+        // behind 32768 208 (8 splits), 192 (6); 128 of 512 bf16 ones behind
+        // 16384 86 (16), 76 (8); 256 of 512 behind 8192, eight K/V heads, 127
+        // (5), 114 (3); no own keys, behind 32768, 173 (8), 187 (6).
+        uint64_t room = 512;
+        if (p.flat_tile) {
+            const double shared = 2.0 * double(p.tiles_flat) * double(prefix);
+            const double beside = double(B * by16) * double(own_keys) * (s->pool_dtype == KVEC_FP8_E4M3 ? 1.0 : 2.0);
+            room = uint64_t(512.0 * shared / (shared + beside));
+        }
+        p.parts_flat = splits(uint64_t(p.tiles_flat) * Hk, prefix, room);
     }
-    p.parts_own = splits(own, len > p.first ? len - p.first : 1);
+    p.parts_own = splits(own, len > p.first ? len - p.first : 1, 512);
     p.blocks_flat = p.flat ? uint64_t(p.tiles_flat) * Hk * p.parts_flat : 0;
     p.blocks = p.blocks_flat + own * p.parts_own;
     return p;
