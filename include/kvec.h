@@ -422,7 +422,8 @@ int kvec_step_tables(const kvec_step* step, void* stream);
  * Pair i is (x[i], x[i + rot/2]), or (x[2i], x[2i+1]) if interleaved; values
  * from rot on are not turned.  Angles in 64 bits, the rest in 32, one rounding
  * at the end.  An fp8 pool gets x / scale, values past +-448 as +-448.
- * Queries go to q_out (q itself with q's strides: in place).  A slot outside
+ * Queries go to q_out (q itself with q's strides: in place; k and v may lie
+ * between its rows then, but share no values with it).  A slot outside
  * [0, n_slots) is skipped; the slots of a call must be distinct.  Tokens from
  * *n_tokens on (if given) are left as they were.  Strides in elements, each
  * head's values adjacent.  dim <= 512, rot even and <= dim, axes <= 8. */

@@ -233,17 +233,20 @@ def test_one_position_row_for_all_axes(pkg, gpu):
     assert torch.equal(got.cpu(), want[0]) and torch.equal(pool.cpu(), want[1])
 
 
-def test_large_step_takes_the_deep_kernel(pkg, gpu):
-    """Enough rows that a wave takes three of each group: the same bytes as in
-    small calls."""
-    N, Hq, Hk, D = 9000, 9, 3, 128
-    c = case(14, N, Hq, Hk, D, D, BF, BF)
+@pytest.mark.parametrize("N,Hq,Hk,D,dtype,pool", [(50000, 9, 3, 128, BF, BF), (17000, 32, 8, 128, HF, HF),
+                                                  (33001, 26, 4, 64, BF, BF), (99000, 4, 2, 64, torch.float32, torch.float32)])
+def test_large_step_takes_the_deep_kernel(pkg, gpu, N, Hq, Hk, D, dtype, pool):
+    """Enough rows that a wave takes three of each group (98304 waves of one
+    each): the same bytes as in small calls."""
+    waves = N * -(-(Hq + 2 * Hk) // (64 // (D // 16)))
+    assert waves >= 12 * 256 * 32
+    c = case(14, N, Hq, Hk, D, D, dtype, pool)
     whole = go(pkg, gpu, c)
     x, pool = c["x"].to(gpu), c["pool"].to(gpu)
     q, k, v = split(c, x)
     parts = []
-    for a in range(0, N, 500):
-        b = min(a + 500, N)
+    for a in range(0, N, 5000):
+        b = min(a + 5000, N)
         parts.append(pkg.attention.norm_rotate_write(
             q[a:b], k[a:b], v[a:b], c["pos"][a:b].to(gpu), c["freqs"].to(gpu), pool, c["slots"][a:b].to(gpu), layer=1,
             q_weight=c["wq"].to(gpu), k_weight=c["wk"].to(gpu)))
