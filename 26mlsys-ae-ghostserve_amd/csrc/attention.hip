@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
     __shared__ f32x4 lo[kAB];
     __shared__ float ll[kAB];
     const uint32_t tid = threadIdx.x, rows = a.tokens * a.heads, row = blockIdx.x;
-    if (row / a.heads >= live_tokens(a)) return;
+    if (row / a.heads >= live_tokens(a) || row / a.heads < first_token(a, 0)) return;
     const uint32_t each = kAB / lanes, mine = tid / lanes, d = tid % lanes * 4;
     const uint32_t parts = a.parts_flat + a.parts_own;
     float top = -INFINITY, l = 0.0f;

@@ -463,7 +463,8 @@ int kvec_norm_rotate_write(const kvec_norm_rotate* step, void* stream);
  * seq_lens[b] - n_b + i and sees the positions up to its own: below `prefix` on
  * the pages of prefix_pages, from there on those of its page table row.  Keys on
  * pages outside [0, pool_pages) and past the row are left out; a query that
- * sees none gives zeros.  Tokens from cu_q[batch] on are left as they were.
+ * sees none gives zeros.  Tokens before cu_q[0] and from cu_q[batch]
+ * on are left as they were.
  * out = softmax(scale * q.k) v by query head; head h reads K/V head
  * h / (heads / kv_heads).  fp8 K and V stand for value * scale.
  * max_q: the most tokens that a request has (more of them are not computed);

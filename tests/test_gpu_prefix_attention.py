@@ -289,6 +289,21 @@ def test_padded_rows_stay(pkg, gpu):
         assert (got[n:] == 3.0).all()
 
 
+@pytest.mark.parametrize("prefix", [0, 32, 600])
+@pytest.mark.parametrize("new", [[2, 1, 3], [100, 30, 3]])
+def test_rows_before_the_first_request_stay(pkg, gpu, new, prefix):
+    """Whether results are joined from parts or written at once."""
+    c = make(gpu, 7, [n + prefix + 400 for n in new], new, 8, 2, 64, BF, BF, 16, prefix)
+    ref, n, gap = reference(c), sum(new), 5
+    q = torch.full((n + 2 * gap, 8, 64), float("nan"), dtype=BF, device=gpu)
+    q[gap:gap + n] = c["q"]
+    out = torch.full_like(q, 3.0)
+    pkg.attention.prefix_attention(q, c["pool"], c["table"], c["lens"], prefix, layer=1, cu_q=c["cu"] + gap, out=out,
+                                   max_q=max(new))
+    check(out[gap:gap + n], ref)
+    assert (out[:gap] == 3.0).all() and (out[gap + n:] == 3.0).all()
+
+
 @pytest.mark.parametrize("prefix", [0, 2100])
 def test_long_and_split(pkg, gpu, prefix):
     """Keys enough that blocks share them out; wrong hints change no result."""
