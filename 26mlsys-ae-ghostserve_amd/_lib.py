@@ -341,6 +341,7 @@ def require_same_device(device, *tensors, what: str = "tensor") -> None:
     """Every tensor given (None: left out) lies on the GPU ``device``."""
     if device.type != "cuda":
         raise ValueError(f"{what}s must be GPU (HIP) tensors of one device")
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:     # -1 on the CPU
             raise ValueError(f"{what}s must be GPU (HIP) tensors of one device")

@@ -136,7 +136,7 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     if tokens is not None and (tokens.dtype != torch.int32 or tokens.numel() != 1):
         raise ValueError("tokens must be one int32 value")
     if out is None:
-        out = torch.empty(qs, dtype=dt, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         o0, o1 = Hq * D, D
     elif out.shape != qs or out.dtype != dt or not (out.is_contiguous() or out is q):
         raise ValueError("out must be contiguous and like q, or q itself")
@@ -213,7 +213,7 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
         if front.dtype != i32 or front.numel() * pt < prefix:
             raise ValueError("prefix_pages must be int32 and hold the prefix")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != dt or not out.is_contiguous():
         raise ValueError("out must be contiguous and like q")
     s = _lib.ATTENTION_FORMAT.pack(
@@ -223,6 +223,6 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
         D ** -0.5 if scale is None else float(scale), _scale(k_scale, dev, "k_scale"),
         _scale(v_scale, dev, "v_scale"))
     need = _lib.lib().kvec_prefix_attention_workspace(s)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     _lib.call_on(dev, "kvec_prefix_attention", s, _ptr(ws), max(need, 0), _lib.stream_handle(dev))
     return out

@@ -132,7 +132,7 @@ def step_tables(page_table: torch.Tensor, cached: torch.Tensor, new: torch.Tenso
     if T < 0:
         raise ValueError("max_tokens must not be negative")
     if out is None:
-        buf = torch.empty(2 * T + 2 * B + 2, dtype=i32, device=dev)
+        buf = cached.new_empty(2 * T + 2 * B + 2)
         out = StepTables(*buf.split_with_sizes([T, T, B + 1, B, 1]))
     else:
         for t, n in zip(out, (T, T, B + 1, B, 1)):
