@@ -737,8 +737,9 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 
     // V values that were taken out, to the rows that see them
     if (odd) {
-        // (fp8: the first units are looked through before the limits are known)
-        const uint32_t skip = !FP8 && block_low > it.k0 ? (block_low - it.k0) / kTileKeys * kTileKeys : 0u;
+        // from the first pass on that was looked through, two units at a time (fp8:
+        // the first units are looked through before the limits are known)
+        const uint32_t skip = !FP8 && block_low > it.k0 ? (block_low - it.k0) / (2 * kTileKeys) * (2 * kTileKeys) : 0u;
         for (uint32_t kk = it.k0 + skip; kk < it.k1; ++kk) {
             const uint32_t sl = kk < limit ? key_slot(a, it, kk) : kNoCell;
 #pragma unroll
