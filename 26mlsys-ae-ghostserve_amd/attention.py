@@ -173,8 +173,8 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
 
     Keys on pages outside the pool are left out; a query that sees no key (an idle
     row: ``seq_lens`` 0) gives zeros.  Rows before ``cu_q[0]`` and from ``cu_q[-1]``
-    on are left as they were.  ``max_q``: the most tokens of a request (default: all tokens), ``max_len``:
-    about the longest of ``seq_lens`` (default: what a table row can hold); closer
+    on are left as they were.  ``max_q``: the most tokens of a request (default: all
+    tokens; a request's tokens past it are left as they were), ``max_len``: about the longest of ``seq_lens`` (default: what a table row can hold); closer
     values split the work better.  ``scale``: default 1/sqrt(dim).  ``k_scale``,
     ``v_scale``: an fp8 pool's, as in :func:`norm_rotate_write`.  Nothing is read
     back to the host, so the call can be captured in a graph."""

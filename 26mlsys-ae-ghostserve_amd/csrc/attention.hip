@@ -144,6 +144,7 @@ struct AttnArgs {
     uint32_t parts_flat, parts_own;            // splits of the keys of each part
     uint32_t blocks_flat;                      // blocks of the shared part, before those of the own keys
     uint32_t tiles_flat, tiles_own;            // row tiles of each (upper bound)
+    uint32_t max_rows;                         // rows of a request that are computed (max_q tokens')
     FastDiv by_group, by_req_tiles;            // query heads of a K/V head; stream blocks: row tiles of a request
     FastDiv by_flat, by_own;                   // splits of each part
     FastDiv by_heads_flat, by_heads_own;       // K/V heads times splits
@@ -168,6 +169,25 @@ __device__ __forceinline__ uint32_t request_of(const AttnArgs& a, uint32_t t) {
         else hi = mid;
     }
     return lo;
+}
+// Whether token t (a live one) is among its request's first max_q.  The request is
+// looked for by a wave, 64 entries at a time.
+__device__ __forceinline__ bool computed(const AttnArgs& a, uint32_t t) {
+    if (!a.cu || a.max_rows >= a.tokens * a.group) return true;
+    uint32_t lo = 0, n = a.batch;              // cu[lo] <= t < cu[lo + n]
+    while (n > 1) {
+        const uint32_t step = (n + 63) / 64, off = ((threadIdx.x & 63) + 1) * step;
+        const bool before = off < n && uint32_t(a.cu[lo + min(off, n)]) <= t;
+        const uint32_t skip = uint32_t(__builtin_popcountll(__ballot(before))) * step;
+        lo += skip;
+        n = min(step, n - skip);
+    }
+    return (t - uint32_t(a.cu[lo])) * a.group < a.max_rows;
+}
+// Rows of request b that are computed; t0: its first token.
+__device__ __forceinline__ uint32_t rows_of(const AttnArgs& a, uint32_t b, uint32_t t0) {
+    const uint32_t t1 = min(first_token(a, b + 1), a.tokens);
+    return t1 > t0 ? min((t1 - t0) * a.group, a.max_rows) : 0u;
 }
 // Keys that token t of request b sees.
 __device__ __forceinline__ uint32_t seen_by(const AttnArgs& a, uint32_t b, uint32_t t) {
@@ -195,8 +215,7 @@ struct TileAt {
     uint32_t b, first;
 };
 __device__ __forceinline__ uint32_t tiles_of(const AttnArgs& a, uint32_t b) {
-    const uint32_t t0 = first_token(a, b), t1 = min(first_token(a, b + 1), a.tokens);
-    return t1 > t0 ? uint32_t((uint64_t(t1 - t0) * a.group + kTileRows - 1) / kTileRows) : 0u;
+    return (rows_of(a, b, first_token(a, b)) + kTileRows - 1) / kTileRows;
 }
 __device__ __forceinline__ TileAt tile_at(const AttnArgs& a, uint32_t tile) {
     const uint32_t lane = threadIdx.x & 63;
@@ -263,8 +282,7 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
             local = tile - __builtin_amdgcn_readfirstlane(t.first);
         }
         it.t0 = first_token(a, it.b);
-        const uint32_t t1 = min(first_token(a, it.b + 1), a.tokens);
-        it.rows = t1 > it.t0 ? (t1 - it.t0) * a.group : 0u;
+        it.rows = rows_of(a, it.b, it.t0);
         it.row0 = local * BM;
         it.live = it.row0 < it.rows;
         first = a.first;
@@ -1061,7 +1079,7 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
     __shared__ f32x4 lo[kAB];
     __shared__ float ll[kAB];
     const uint32_t tid = threadIdx.x, rows = a.tokens * a.heads, row = blockIdx.x;
-    if (row / a.heads >= live_tokens(a) || row / a.heads < first_token(a, 0)) return;
+    if (row / a.heads >= live_tokens(a) || row / a.heads < first_token(a, 0) || !computed(a, row / a.heads)) return;
     const uint32_t each = kAB / lanes, mine = tid / lanes, d = tid % lanes * 4;
     const uint32_t parts = a.parts_flat + a.parts_own;
     float top = -INFINITY, l = 0.0f;
@@ -1282,6 +1300,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     while ((1 << a.shift) < s->page_tokens) ++a.shift;
     a.pool_pages = uint32_t(s->pool_pages);
     a.cap = a.width << a.shift;
+    a.max_rows = uint32_t(s->cu_q ? min(int64_t(s->max_q), s->tokens) : 1) * a.group;
     a.prefix = uint32_t(s->prefix);
     a.first = p.first;
     a.parts_flat = p.parts_flat;
