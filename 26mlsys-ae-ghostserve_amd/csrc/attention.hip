@@ -20,8 +20,9 @@
 // and is needed transposed, which ds_read_b64_tr_b16 does on the way from LDS.
 //
 // Scores, maxima, sums and outputs are 32-bit; P is rounded to 16 bits for the
-// second product (its largest value is near 1, the rounding is half a step of
-// the inputs' own type), and the output once at the end.
+// second product (half a step of the inputs' own type relative to each value; a
+// product of 32-bit values would run at a sixteenth of the rate), and the output
+// once at the end.
 //
 // Masked keys: a key past a row's last one or on a page outside the pool has
 // p = 0 by selection; keys that no row of a tile sees are read as zeros, so what
@@ -43,6 +44,13 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // The running maximum moves only when a score passes it by this much (in
 // powers of two): p stays under 2^8, and most tiles rescale nothing.
 constexpr float kLazy = 8.0f;
+// Powers are formed 2^7 times as large where they are rounded to fp16, whose
+// smallest numbers, 2^-24, would otherwise be short for a long tail far under a
+// peak: 2^18 keys of 2^-25.5 all became 0.  The largest is 2^15 then (fp16 ends at
+// 2^16); sums and outputs carry the factor until they are divided.  bf16 has the
+// exponents of 32 bits.
+template <class T>
+constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -666,7 +674,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
             m = to;
             bar = m + lazy;
-            mc = m == -INFINITY ? 0.0f : m * c;
+            mc = m == -INFINITY ? 0.0f : m * c - kLift<T>;
             l *= f;
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -964,7 +972,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= f;
         }
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        const float mc = m == -INFINITY ? 0.0f : m * c - kLift<T>;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], c, -mc));
