@@ -22,7 +22,8 @@
 // Scores, maxima, sums and outputs are 32-bit; P is rounded to 16 bits for the
 // second product (half a step of the inputs' own type relative to each value; a
 // product of 32-bit values would run at a sixteenth of the rate), and the output
-// once at the end.
+// once at the end.  The sums are those of the rounded P, so the weights of a row
+// add up to one.
 //
 // Masked keys: a key past a row's last one or on a page outside the pool has
 // p = 0 by selection; keys that no row of a tile sees are read as zeros, so what
@@ -974,13 +975,12 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
         }
         const float mc = m == -INFINITY ? 0.0f : m * c - kLift<T>;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], c, -mc));
-            l += s[i / 4][i % 4];
-        }
+        for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], c, -mc));
         // sum over keys 4 g .. and 16 + 4 g .. : what the lane's scores are of
         const u32x4 p = {pack2(s[0][0], s[0][1], ty), pack2(s[0][2], s[0][3], ty), pack2(s[1][0], s[1][1], ty),
                          pack2(s[1][2], s[1][3], ty)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l = add2(uint32_t(p[i]), l, ty);   // the sum is that of the rounded P
         const uint32_t kk = 4 * g + r / 4, z = G::swz_v(kk);   // keys 8 and 16 apart: the same permutation
         const uint8_t* v = lv + kk * G::ROW + (r & 1) * 8;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

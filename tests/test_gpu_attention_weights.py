@@ -46,3 +46,29 @@ def test_a_long_tail_under_a_peak(pkg, gpu, dtype, drop, n, new, prefix, max_len
     tol = u * want + (2 * one / (1 + tail))[:, None, None] * 1.01
     off = (got.double() - want).abs()
     assert (off <= tol).all(), f"{float((off / tol).max()):.3g} of the tolerance, {got[0, 0, 0]} for {float(want[0, 0, 0])}"
+
+
+@pytest.mark.parametrize("dtype,up", [(BF, 128.445), (HF, 128.0624)])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (3, 0), (40, 0), (1, 192), (3, 192)])
+def test_the_average_of_equal_values(pkg, gpu, dtype, up, new, prefix):
+    """V is one value, so the result is that value, whatever the weights are rounded
+    to: it differs by 32-bit sums only.  Here one key outweighs the first by `up`,
+    which is nearly half a step off what 16 bits hold and too little to move the
+    running maximum; the others weigh nothing."""
+    D, P, n = 64, 16, 200
+    value = 2.0 - torch.finfo(dtype).eps
+    width = -(-(n + new) // P)
+    pool = torch.zeros(1, width, P, 2, 1, D, dtype=dtype, device=gpu)
+    flat = pool.view(-1, 2, 1, D)
+    flat[:, 1] = value
+    flat[1:, 0, 0, 0] = -60.0
+    flat[130, 0, 0, 0] = 7.0
+    flat[130, 0, 0, 1] = math.log2(up) - 7.0
+    B = 3 if prefix else 1
+    q = torch.zeros(B * new, 16, D, dtype=dtype, device=gpu)
+    q[..., :2] = 1.0
+    table = torch.arange(width, dtype=torch.int32, device=gpu)[None].expand(B, -1).contiguous()
+    lens = torch.full((B,), n + new, dtype=torch.int32, device=gpu)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=gpu) * new
+    got = pkg.attention.prefix_attention(q, pool, table, lens, prefix, cu_q=cu, max_q=new, max_len=10, scale=math.log(2.0))
+    assert (got == value).all(), f"{float(got[0, 0, 0])} for {value}"
