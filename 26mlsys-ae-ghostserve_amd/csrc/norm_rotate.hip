@@ -118,7 +118,7 @@ __global__ __launch_bounds__(kNRB) void norm_rotate_kernel(NrArgs p) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 
-    const float ik = p.k_scale ? 1.0f / *p.k_scale : 1.0f, iv = p.v_scale ? 1.0f / *p.v_scale : 1.0f;
+    const float k_scale = p.k_scale ? *p.k_scale : 1.0f, v_scale = p.v_scale ? *p.v_scale : 1.0f;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const uint32_t r = row0 + i * groups;
@@ -200,13 +200,15 @@ __global__ __launch_bounds__(kNRB) void norm_rotate_kernel(NrArgs p) {
             PT* y = reinterpret_cast<PT*>(p.pool) +
                     (int64_t(slot) * 2 * p.kv_heads + (r - p.heads)) * int64_t(p.dim);
             if constexpr (!__is_same(T, PT)) {
-                const float f = is_k ? ik : iv;
+                // a quotient, not a product with the reciprocal: that is off by a step
+                // at midpoints, and infinite under 2^-128
+                const float f = is_k ? k_scale : v_scale;
 #pragma unroll
                 for (int n = 0; n < NU; ++n)
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        a[n][j] *= f;
-                        b[n][j] *= f;
+                        a[n][j] /= f;
+                        b[n][j] /= f;
                     }
             }
 #pragma unroll
