@@ -1238,14 +1238,24 @@ inline int check_attention(const kvec_attention* s, const char* fn) {
     return KVEC_OK;
 }
 
+// The plan, and that its launches can be.
+inline int checked_plan(const kvec_attention* s, const char* fn, AttnPlan* p) {
+    *p = plan_attention(s);
+    if (!launchable(p->blocks, kAB) || (!p->direct() && !launchable(p->rows, kAB)))
+        return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks for one launch", fn);
+    return KVEC_OK;
+}
+
 }  // namespace kvec
 
 using namespace kvec;
 
 extern "C" int64_t kvec_prefix_attention_workspace(const kvec_attention* s) {
-    if (check_attention(s, "kvec_prefix_attention_workspace")) return -1;
+    static const char* fn = "kvec_prefix_attention_workspace";
+    if (check_attention(s, fn)) return -1;
     if (s->tokens == 0 || s->batch == 0) return 0;
-    return plan_attention(s).bytes(s->dim);
+    AttnPlan p;
+    return checked_plan(s, fn, &p) ? -1 : p.bytes(s->dim);
 }
 
 extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -1261,8 +1271,8 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
         if (x < 0 || x > (int64_t(1) << 40)) return set_error(KVEC_EINVAL, "%s: stride %lld", fn, (long long)x);
     if ((s->heads > 1 && s->o_head_stride < s->dim) || (s->tokens > 1 && s->o_stride < s->dim))
         return set_error(KVEC_EINVAL, "%s: rows of out overlap", fn);
-    const AttnPlan p = plan_attention(s);
-    if (p.blocks >= (uint64_t(1) << 31)) return set_error(KVEC_EUNSUPPORTED, "%s: too many blocks", fn);
+    AttnPlan p;
+    if ((rc = checked_plan(s, fn, &p))) return rc;
     const int64_t need = p.bytes(s->dim);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return set_error(KVEC_EINVAL, "%s: workspace of %lld bytes, 16-byte aligned, wanted", fn, (long long)need);

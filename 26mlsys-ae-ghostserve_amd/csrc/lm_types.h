@@ -117,6 +117,9 @@ __device__ __forceinline__ void put(T* p, const float* f) {
     else put1(p, f[0]);
 }
 
+// HIP's limit: the threads of a launch are fewer than 2^32.
+inline bool launchable(uint64_t blocks, uint32_t threads) { return blocks < (uint64_t(1) << 32) / threads; }
+
 inline int64_t type_bytes(int dtype) {
     return dtype == KVEC_F32 ? 4 : dtype == KVEC_BF16 || dtype == KVEC_F16 ? 2 : dtype == KVEC_FP8_E4M3 ? 1 : 0;
 }

@@ -304,7 +304,7 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     const uint64_t waves1 = uint64_t(s->tokens) * ((rows + groups - 1) / groups);
     const bool deep = wide && waves1 >= 12 * 256 * 32;
     const uint32_t per = groups * (deep ? 3 : 1), chunks = (rows + per - 1) / per;
-    if (uint64_t(s->tokens) * chunks >= (uint64_t(1) << 32) - 4)
+    if (s->tokens >= (int64_t(1) << 32) || !launchable((uint64_t(s->tokens) * chunks + 3) / 4, kNRB))
         return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
     a.q = (const uint8_t*)s->q;
     a.k = (const uint8_t*)s->k;

@@ -1,0 +1,38 @@
+"""Sizes that no launch can have, and arguments that no call can, are refused on
+the host with a code or a ValueError (CPU only: the addresses are made up)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from test_step_refusals import at, no_gpu, nr  # noqa: F401
+
+
+@pytest.mark.parametrize("kw", [
+    # one block of 256 threads for each of 2^24 rows joins the parts
+    dict(tokens=1 << 21, batch=1 << 21, cu_q=1 << 56, max_q=1, prefix=100),
+    dict(tokens=1 << 20, batch=1 << 20, heads=16, prefix=100),
+    # 2^24 stream blocks: a request's rows by max_q, 16 a block
+    dict(tokens=1 << 20, batch=1 << 15, cu_q=1 << 56, max_q=1 << 20, prefix=128, max_len=128),
+    dict(tokens=1 << 14, batch=1 << 19, cu_q=1 << 56, max_q=1 << 14, heads=64, kv_heads=64, prefix=0, max_len=1),
+])
+def test_attention_grids(pkg, kw):
+    L = pkg._lib.lib()
+    f = dict(q=1 << 50, out=1 << 51, pool=1 << 52, page_table=1 << 53, seq_lens=1 << 54, prefix_pages=1 << 55)
+    f.update(kw)
+    heads = f.get("heads", 8)
+    f.update(q_stride=heads * 64, o_stride=heads * 64)
+    call = at(pkg, **f)
+    assert L.kvec_prefix_attention_workspace(C.byref(call)) == -1
+    assert b"launch" in L.kvec_last_error()
+    assert L.kvec_prefix_attention(C.byref(call), 1 << 57, 1 << 60, None) == -2
+    assert b"launch" in L.kvec_last_error()
+
+
+def test_norm_rotate_grid(pkg):
+    L = pkg._lib.lib()
+    far = dict(q=1 << 50, k=1 << 51, v=1 << 52, q_out=1 << 53, positions=1 << 54, pool=1 << 55, slots=1 << 56,
+               axis_stride=1 << 26)
+    call = nr(pkg, tokens=1 << 26, heads=1, kv_heads=1, dim=64, q_stride=64, o_stride=64, k_stride=64, v_stride=64, **far)
+    assert L.kvec_norm_rotate_write(C.byref(call), None) == -2
+    assert b"launch" in L.kvec_last_error()
