@@ -345,3 +345,11 @@ def require_same_device(device, *tensors, what: str = "tensor") -> None:
     for t in tensors:
         if t is not None and t.get_device() != index:     # -1 on the CPU
             raise ValueError(f"{what}s must be GPU (HIP) tensors of one device")
+
+
+def require_no_grad(*tensors, what: str) -> None:
+    """No tensor given (None: left out) asks for a gradient that ``what`` would drop."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or with detached tensors")

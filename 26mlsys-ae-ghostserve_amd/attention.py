@@ -8,6 +8,9 @@ own cache writes and attention (bench_ghostserve_rdp.py:396-481).
   prefix_attention    attention over the pool for a batch whose requests share
                       a prefix, which is computed once for all of them
 
+Both serve and do not train: there is no backward pass, and tensors that ask for
+a gradient are refused (under ``torch.no_grad()`` nothing asks for one).
+
 Pool tensor: [layers, pool_pages, page_tokens, 2 (K,V), kv_heads, head_dim], of
 the queries' type or float8_e4m3fn with a scale for K and for V, as in
 :mod:`.paged`; slots and page tables as :func:`.paged.step_tables` makes them.
@@ -99,6 +102,7 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     dev, dt = q.device, q.dtype
     if dt not in _COMPUTE or k.dtype != dt or v.dtype != dt:
         raise ValueError("q, k and v must be of one type: float32, bfloat16 or float16")
+    _lib.require_no_grad(q, k, v, q_weight, k_weight, pool, out, what="norm_rotate_write")
     _lib.require_same_device(dev, k, v, positions, freqs, pool, slots, q_weight, k_weight, axis_of, tokens, out,
                              what="norm_rotate_write tensor")
     N, Hq, D = qs
@@ -192,6 +196,7 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
         raise ValueError(f"seq_lens must be [{B}] and cu_q int32 [{B + 1}]")
     if cu_q is None and N != B:
         raise ValueError("without cu_q there is one query token a request")
+    _lib.require_no_grad(q, pool, out, what="prefix_attention")
     _lib.require_same_device(dev, pool, page_table, seq_lens, cu_q, prefix_pages, out, what="prefix_attention tensor")
     base, _, Hk, Dp = _layer(pool, layer)
     if Dp != D or Hq % Hk:

@@ -36,3 +36,33 @@ def test_norm_rotate_grid(pkg):
     call = nr(pkg, tokens=1 << 26, heads=1, kv_heads=1, dim=64, q_stride=64, o_stride=64, k_stride=64, v_stride=64, **far)
     assert L.kvec_norm_rotate_write(C.byref(call), None) == -2
     assert b"launch" in L.kvec_last_error()
+
+
+def test_gradients_are_refused(pkg):
+    """There is no backward pass: a result that silently lost its history would train
+    nothing.  Without gradients in play the call goes on (to its other checks)."""
+    A = pkg.attention
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    q, kv = torch.zeros(4, 2, 64), torch.zeros(4, 2, 64)
+    pool, w = torch.zeros(1, 2, 4, 2, 2, 64), torch.zeros(64)
+
+    def write(**g):
+        t = {n: x.clone().requires_grad_(n in g) for n, x in (("q", q), ("k", kv), ("v", kv), ("w", w), ("pool", pool))}
+        A.norm_rotate_write(t["q"], t["k"], t["v"], None, None, t["pool"], i(4), q_weight=t["w"], k_weight=w)
+
+    for n in ("q", "k", "v", "w", "pool"):
+        with pytest.raises(ValueError, match="no backward"):
+            write(**{n: True})
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+            write(**{n: True})
+    with pytest.raises(ValueError, match="GPU"):
+        write()
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        A.norm_rotate_write(q, kv, kv, None, None, pool, i(4), q_weight=torch.nn.Parameter(w))
+    for n in ("q", "pool"):
+        t = {"q": q.half(), "pool": pool.half()}
+        t[n].requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            A.prefix_attention(t["q"], t["pool"], i(4, 3), i(4))
+        with torch.inference_mode(), pytest.raises(ValueError, match="GPU"):
+            A.prefix_attention(t["q"], t["pool"], i(4, 3), i(4))
