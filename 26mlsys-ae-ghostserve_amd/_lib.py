@@ -191,6 +191,15 @@ NORM_ROTATE_FORMAT = struct.Struct("@qiiiiPPPqqqqqqPqqifPPiiiPqPPfPiqPPPP")
 ATTENTION_FORMAT = struct.Struct("@qiiiiiPqqPqqPiqiPiPPiqqPfPP")
 _nrp = C.POINTER(NormRotate)
 
+
+def pack(fmt: struct.Struct, *fields) -> bytes:
+    """The fields' bytes; a ValueError for one that its C type cannot hold."""
+    try:
+        return fmt.pack(*fields)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"argument out of range: {e}") from None
+
+
 # name -> (restype, argtypes); mirrors include/kvec.h
 SIGNATURES = {
     "kvec_version": (_i, []),

@@ -22,6 +22,7 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+_FLOAT_MAX = torch.finfo(torch.float32).max
 _COMPUTE = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -146,11 +147,13 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
         raise ValueError("out must be contiguous and like q, or q itself")
     else:
         o0, o1, _ = out.stride()
-    s = _lib.NORM_ROTATE_FORMAT.pack(
-        N, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1, out.data_ptr(),
-        o0, o1, bool(norm), eps, _ptr(q_weight), _ptr(k_weight), 2 * half, bool(interleaved), axes, _ptr(positions),
-        axis_stride, _ptr(axis_of), _ptr(freqs), factor, base, _DTYPES[pool_dt], n_slots, slots.data_ptr(),
-        _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), _ptr(tokens))
+    if not (abs(eps) <= _FLOAT_MAX and abs(factor) <= _FLOAT_MAX):
+        raise ValueError("eps and factor must be finite 32-bit numbers")
+    s = _lib.pack(
+        _lib.NORM_ROTATE_FORMAT, N, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), q0, q1, k0, k1,
+        v0, v1, out.data_ptr(), o0, o1, bool(norm), eps, _ptr(q_weight), _ptr(k_weight), 2 * half, bool(interleaved),
+        axes, _ptr(positions), axis_stride, _ptr(axis_of), _ptr(freqs), factor, base, _DTYPES[pool_dt], n_slots,
+        slots.data_ptr(), _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), _ptr(tokens))
     _lib.call_on(dev, "kvec_norm_rotate_write", s, _lib.stream_handle(dev))
     return out
 
@@ -221,12 +224,15 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != dt or not out.is_contiguous():
         raise ValueError("out must be contiguous and like q")
-    s = _lib.ATTENTION_FORMAT.pack(
-        N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q0, q1, out.data_ptr(), Hq * D, D, base, _DTYPES[pool_dt], pages,
-        pt, page_table.data_ptr(), width, seq_lens.data_ptr(), _ptr(cu_q),
-        max(N, 1) if max_q is None else int(max_q), int(max_len or 0), prefix, front.data_ptr(),
-        D ** -0.5 if scale is None else float(scale), _scale(k_scale, dev, "k_scale"),
-        _scale(v_scale, dev, "v_scale"))
+    max_q = max(N, 1) if max_q is None else min(int(max_q), max(N, 1))
+    max_len = min(int(max_len or 0), width * pt)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if max_q < 0 or max_len < 0 or not 0.0 <= scale <= _FLOAT_MAX:
+        raise ValueError("max_q, max_len and scale must not be negative, and scale finite")
+    s = _lib.pack(
+        _lib.ATTENTION_FORMAT, N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q0, q1, out.data_ptr(), Hq * D, D, base,
+        _DTYPES[pool_dt], pages, pt, page_table.data_ptr(), width, seq_lens.data_ptr(), _ptr(cu_q), max_q, max_len,
+        prefix, front.data_ptr(), scale, _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"))
     need = _lib.lib().kvec_prefix_attention_workspace(s)
     ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     _lib.call_on(dev, "kvec_prefix_attention", s, _ptr(ws), max(need, 0), _lib.stream_handle(dev))

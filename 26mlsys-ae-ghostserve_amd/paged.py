@@ -129,8 +129,8 @@ def step_tables(page_table: torch.Tensor, cached: torch.Tensor, new: torch.Tenso
     _lib.require_cuda(page_table, cached, new, free_pages, what="step table")
     _lib.require_same_device(dev, cached, new, free_pages, what="step table")
     T = int(max_tokens)
-    if T < 0:
-        raise ValueError("max_tokens must not be negative")
+    if not 0 <= T < (1 << 31) - 1024:
+        raise ValueError("max_tokens must not be negative, and under 2^31 - 1024")
     if out is None:
         buf = cached.new_empty(2 * T + 2 * B + 2)
         out = StepTables(*buf.split_with_sizes([T, T, B + 1, B, 1]))
@@ -141,10 +141,10 @@ def step_tables(page_table: torch.Tensor, cached: torch.Tensor, new: torch.Tenso
         _lib.require_cuda(*out, what="step table")
         _lib.require_same_device(dev, *out, what="step table")
     slots, positions, cu_new, seq_lens, taken = out
-    s = _lib.STEP_FORMAT.pack(
-        page_table.data_ptr(), B, width, int(page_tokens), int(pool_pages), cached.data_ptr(), new.data_ptr(),
-        free_pages.data_ptr(), free_pages.shape[0], slots.data_ptr(), positions.data_ptr(), T, cu_new.data_ptr(),
-        seq_lens.data_ptr(), taken.data_ptr())
+    s = _lib.pack(
+        _lib.STEP_FORMAT, page_table.data_ptr(), B, width, int(page_tokens), int(pool_pages), cached.data_ptr(),
+        new.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], slots.data_ptr(), positions.data_ptr(), T,
+        cu_new.data_ptr(), seq_lens.data_ptr(), taken.data_ptr())
     _lib.call_on(dev, "kvec_step_tables", s, _lib.stream_handle(dev))
     return out
 
