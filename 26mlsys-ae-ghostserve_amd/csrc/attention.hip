@@ -1269,7 +1269,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     const int64_t str[4] = {s->q_stride, s->q_head_stride, s->o_stride, s->o_head_stride};
     for (int64_t x : str)
         if (x < 0 || x > (int64_t(1) << 40)) return set_error(KVEC_EINVAL, "%s: stride %lld", fn, (long long)x);
-    if ((s->heads > 1 && s->o_head_stride < s->dim) || (s->tokens > 1 && s->o_stride < s->dim))
+    if (rows_overlap(s->tokens, s->o_stride, s->heads, s->o_head_stride, s->dim))
         return set_error(KVEC_EINVAL, "%s: rows of out overlap", fn);
     AttnPlan p;
     if ((rc = checked_plan(s, fn, &p))) return rc;

@@ -117,6 +117,19 @@ __device__ __forceinline__ void put(T* p, const float* f) {
     else put1(p, f[0]);
 }
 
+// Whether two of the n x h rows of `len` values at i * s + j * t share one.
+inline bool rows_overlap(int64_t n, int64_t s, int64_t h, int64_t t, int64_t len) {
+    typedef __int128 wide;
+    if ((n > 1 && s < len) || (h > 1 && t < len)) return true;
+    if (n <= 1 || h <= 1 || s >= wide(h - 1) * t + len || t >= wide(n - 1) * s + len) return false;
+    for (int64_t j = 1; j < h; ++j) {                     // the rows on either side of 0, j
+        const wide d = wide(j) * t, i = d / s;
+        if (i < n && d - i * s < len) return true;
+        if (i + 1 < n && (i + 1) * s - d < len) return true;
+    }
+    return false;
+}
+
 // HIP's limit: the threads of a launch are fewer than 2^32.
 inline bool launchable(uint64_t blocks, uint32_t threads) { return blocks < (uint64_t(1) << 32) / threads; }
 

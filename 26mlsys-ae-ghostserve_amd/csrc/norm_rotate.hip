@@ -264,7 +264,7 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     for (int64_t x : str)
         if (x < 0 || x > (int64_t(1) << 40)) return set_error(KVEC_EINVAL, "%s: stride %lld", fn, (long long)x);
     const bool same = s->q_out == s->q && s->o_stride == s->q_stride && s->o_head_stride == s->q_head_stride;
-    if ((s->heads > 1 && s->o_head_stride < s->dim) || (s->tokens > 1 && s->o_stride < s->dim))
+    if (rows_overlap(s->tokens, s->o_stride, s->heads, s->o_head_stride, s->dim))
         return set_error(KVEC_EINVAL, "%s: rows of q_out overlap", fn);
     auto span = [&](const void* p, int64_t st, int64_t hs, int64_t h, const char* name) {
         return Span{p, uint64_t((s->tokens - 1) * st + (h - 1) * hs + s->dim) * uint64_t(es), name, -1};

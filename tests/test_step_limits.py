@@ -66,3 +66,30 @@ def test_gradients_are_refused(pkg):
             A.prefix_attention(t["q"], t["pool"], i(4, 3), i(4))
         with torch.inference_mode(), pytest.raises(ValueError, match="GPU"):
             A.prefix_attention(t["q"], t["pool"], i(4, 3), i(4))
+
+
+def rows_meet(n, s, h, t, length):
+    at = sorted(i * s + j * t for i in range(n) for j in range(h))
+    return any(b - a < length for a, b in zip(at, at[1:]))
+
+
+@pytest.mark.parametrize("n,h", [(1, 1), (1, 5), (5, 1), (2, 2), (4, 8), (7, 3)])
+def test_rows_of_the_result_that_overlap(pkg, n, h):
+    """Every pair of strides: refused just where two rows share a value (a call that is
+    taken goes on to the next refusal)."""
+    L = pkg._lib.lib()
+    seen = set()
+    for s in (0, 4, 8, 12, 16, 20, 24, 40, 64, 100, 1 << 40):
+        for t in (0, 4, 8, 12, 16, 20, 24, 32, 56, 57, 1 << 40):
+            meet = rows_meet(n, s, h, t, 8)
+            seen.add(meet)
+            call = nr(pkg, tokens=n, heads=h, kv_heads=1, dim=8, rot=0, o_stride=s, o_head_stride=t, q_stride=8 * h,
+                      q_head_stride=8, q_out=1 << 27, pool=1 << 27)
+            assert L.kvec_norm_rotate_write(C.byref(call), None) == -1
+            assert (b"rows of q_out overlap" in L.kvec_last_error()) == meet, (s, t)
+            call = at(pkg, tokens=n, batch=n, heads=h, kv_heads=1, dim=8, o_stride=s, o_head_stride=t, q_stride=8 * h,
+                      q_head_stride=8, prefix=0)
+            call.out = call.pool
+            assert L.kvec_prefix_attention(C.byref(call), 1 << 50, 1 << 40, None) == -1
+            assert (b"rows of out overlap" in L.kvec_last_error()) == meet, (s, t)
+    assert seen == ({False} if n * h == 1 else {False, True})
