@@ -229,6 +229,8 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
     scale = D ** -0.5 if scale is None else float(scale)
     if max_q < 0 or max_len < 0 or not 0.0 <= scale <= _FLOAT_MAX:
         raise ValueError("max_q, max_len and scale must not be negative, and scale finite")
+    if max_q == 0 and cu_q is not None:           # every request is idle
+        return out
     s = _lib.pack(
         _lib.ATTENTION_FORMAT, N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q0, q1, out.data_ptr(), Hq * D, D, base,
         _DTYPES[pool_dt], pages, pt, page_table.data_ptr(), width, seq_lens.data_ptr(), _ptr(cu_q), max_q, max_len,
