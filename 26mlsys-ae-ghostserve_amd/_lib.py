@@ -189,7 +189,6 @@ class Attention(C.Structure):
 STEP_FORMAT = struct.Struct("@PiiiqPPPqPPqPPP")
 NORM_ROTATE_FORMAT = struct.Struct("@qiiiiPPPqqqqqqPqqifPPiiiPqPPfPiqPPPP")
 ATTENTION_FORMAT = struct.Struct("@qiiiiiPqqPqqPiqiPiPPiqqPfPP")
-_nrp = C.POINTER(NormRotate)
 
 
 def pack(fmt: struct.Struct, *fields) -> bytes:

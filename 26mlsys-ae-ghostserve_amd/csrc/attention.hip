@@ -152,7 +152,6 @@ struct AttnArgs {
     uint32_t first;                            // first own key: prefix, or 0 with the prefix's pages read there
     uint32_t parts_flat, parts_own;            // splits of the keys of each part
     uint32_t blocks_flat;                      // blocks of the shared part, before those of the own keys
-    uint32_t tiles_flat, tiles_own;            // row tiles of each (upper bound)
     uint32_t max_rows;                         // rows of a request that are computed (max_q tokens')
     FastDiv by_group, by_req_tiles;            // query heads of a K/V head; stream blocks: row tiles of a request
     FastDiv by_flat, by_own;                   // splits of each part
@@ -256,7 +255,7 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     if (!it.flat) id -= a.blocks_flat;
     const FastDiv by_parts = it.flat ? a.by_flat : a.by_own, by_hp = it.flat ? a.by_heads_flat : a.by_heads_own;
     const uint32_t parts = by_parts.d, hp = by_hp.d;
-    uint32_t tiles = it.flat ? a.tiles_flat : a.tiles_own;
+    uint32_t tiles = 0;
     if (!STREAM && !it.flat) {
         // as many tiles as there are, not the launch's bound: blocks without
         // work come last then, and no compute unit gets a third block for them
@@ -1324,8 +1323,6 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.parts_flat = p.parts_flat;
     a.parts_own = p.parts_own;
     a.blocks_flat = uint32_t(p.blocks_flat);
-    a.tiles_flat = p.tiles_flat;
-    a.tiles_own = uint32_t(p.tiles_own);
     a.by_group = make_fastdiv(a.group);
     a.by_req_tiles = make_fastdiv(p.req_tiles);
     a.by_flat = make_fastdiv(p.parts_flat ? p.parts_flat : 1);
