@@ -56,3 +56,17 @@ def test_lengths_grow_under_a_graph(pkg, gpu, cached):
             at = torch.cat([torch.arange(n) for n in now]).to(gpu)
             check(out[at < 20], (o[at < 20], tol[at < 20]))
             assert (out[at >= 20] == 3.0).all()
+
+
+@pytest.mark.parametrize("B", [64, 65, 130, 5000])
+def test_many_requests(pkg, gpu, B):
+    """Requests enough that a row's is looked for in one, two and three steps, idle
+    ones among them, joined from parts."""
+    new = [(1, 0, 2, 1, 3)[i * 7 % 5] for i in range(B)]
+    c = make(gpu, 43, [64 + 1 + n for n in new], new, 2, 1, 64, BF, BF, 16, 64)
+    o, tol = reference(c)
+    out = torch.full_like(c["q"], 3.0)
+    pkg.attention.prefix_attention(c["q"], c["pool"], c["table"], c["lens"], 64, layer=1, cu_q=c["cu"], out=out, max_q=2)
+    at = torch.cat([torch.arange(n) for n in new]).to(gpu)
+    check(out[at < 2], (o[at < 2], tol[at < 2]))
+    assert (out[at >= 2] == 3.0).all()
