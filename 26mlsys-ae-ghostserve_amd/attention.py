@@ -176,15 +176,25 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
 
     The first ``prefix`` positions are the same for all requests; they are read
     from ``prefix_pages`` (default: the first row of ``page_table``, which has to hold
-    them even if its request is idle) once for all queries.  ``prefix`` need not be whole pages.  0 is ordinary paged attention.
+    them even if its request is idle) once for all queries.  ``prefix`` need not be
+    whole pages.  0 is ordinary paged attention.
 
     Keys on pages outside the pool are left out; a query that sees no key (an idle
     row: ``seq_lens`` 0) gives zeros.  Rows before ``cu_q[0]`` and from ``cu_q[-1]``
-    on are left as they were.  ``max_q``: the most tokens of a request (default: all
-    tokens; a request's tokens past it are left as they were), ``max_len``: about the longest of ``seq_lens`` (default: what a table row can hold); closer
-    values split the work better.  ``scale``: default 1/sqrt(dim).  ``k_scale``,
-    ``v_scale``: an fp8 pool's, as in :func:`norm_rotate_write`.  Nothing is read
-    back to the host, so the call can be captured in a graph."""
+    on are left as they were.
+
+    ``max_q``: the most tokens of a request; a request's tokens past it are left as
+    they were.  The kind of blocks is chosen by it, once for the call: without it every
+    request is taken for one of all tokens, which for 64 decoding requests behind 8192
+    shared keys takes six times as long, and a step of few long and many short requests
+    is faster as two calls.  ``max_len``: about the longest of ``seq_lens`` (default:
+    what a table row can hold), by which the work is split.  ``scale``: default
+    1/sqrt(dim).  ``k_scale``, ``v_scale``: an fp8 pool's, as in
+    :func:`norm_rotate_write`.  Nothing is read back to the host, so the call can be
+    captured in a graph.
+
+    Scores, maxima, sums and outputs are 32-bit; the softmax's weights are rounded to
+    the queries' type before they multiply V."""
     shape, tab = q.shape, page_table.shape
     if len(shape) != 3:
         raise ValueError("q must be [tokens, heads, dim]")

@@ -10,12 +10,12 @@
 // request.  Each request's own keys are a second part; parts are joined by
 // their maxima and sums, which are linear once both are brought to one maximum.
 //
-// Two kinds of blocks, one kernel.  Both form S^T = K Q^T and O^T += V^T P^T, keys along the rows of the
-// matrix instructions and query rows along their columns: a lane then holds
-// scores of one query row only, so the softmax needs one exchange between lane
-// halves (or quarters) for the maximum and none for the sum, and the scores
-// that a lane holds are, rounded to 16 bits, just what the second product wants
-// from it (the instruction sums over keys in any order, so long as V^T comes
+// Two kinds of blocks, one kernel.  Both form S^T = K Q^T and O^T += V^T P^T, keys
+// along the rows of the matrix instructions and query rows along their columns: a
+// lane then holds scores of one query row only, so the softmax needs one exchange
+// between lane halves (or quarters) for the maximum and none for the sum, and the
+// scores that a lane holds are, rounded to 16 bits, just what the second product
+// wants from it (the instruction sums over keys in any order, so long as V^T comes
 // in the same one: rows 4h .. and 8 + 4h .. of each 16).  V lies [key][value]
 // and is needed transposed, which ds_read_b64_tr_b16 does on the way from LDS.
 //
@@ -416,7 +416,11 @@ __device__ __forceinline__ void emit4(Args& a, const Item& it, uint32_t token, u
 // accordingly).  An fp8 pool's values are widened on the way, by register.
 //
 // Measured, 32 query heads to 8 K/V heads of 128, bf16: 4 x 2048 tokens behind 8192
-// 1270 us, 973 TFLOP/s, where a library product of 8192 x 8192 x 8192 reaches 1265;
+// 1270 us, 973 TFLOP/s, where a library product of 8192 x 8192 x 8192 reaches 1265
+// (fp16 1287, fp8 pool 1271); the same at 64 / 16 heads of 64 835 TFLOP/s, 32 / 8 of
+// 80 741 and of 96 869 (80 takes rows of 16 chunks in LDS, six of them zeros), of 192
+// 534 (in the kernel of 256 values, a quarter of its products by zeros), 16 / 4 of
+// 256 708 (one block a compute unit); 16 x 2048 with no prefix 748;
 // 16 x 128 behind 4096 157 us, 889 TFLOP/s (512 blocks, all at once: their start
 // and end are not hidden behind others).  256 requests of one token behind 32768,
 // four K/V heads: 171 us, with an fp8 pool 176.  No one part bounds it: the matrix
@@ -812,10 +816,11 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 // 16 rows against a run of keys that the block's four waves share out, 32 keys
 // at a time: for the few rows of a request that decodes, bound by reading K and
 // V.  A wave works alone until the end (its V in a part of LDS of its own, its
-// maximum and sum its own), then the four results are joined.  Measured: 64 requests of
-// 2048 own keys, 8 K/V heads of 128, bf16: 4.1 TB/s (a copy reaches 5.1).  Four
-// requests behind 512 tokens 8.6 us, most of it the way to the first keys (table,
-// then keys: about 6 us) and the joining of the waves.
+// maximum and sum its own), then the four results are joined.  Measured: 64 requests
+// of 2048 own keys, 8 K/V heads of 128, bf16: 109 us, 4.9 TB/s (a read stream reaches
+// 7.1); 256 such 400 us, 5.4 TB/s; 64 over an fp8 pool 50 us, 5.4 TB/s.  Four requests
+// behind 512 tokens 8.4 us, most of it the way to the first keys (table, then keys:
+// about 6 us) and the joining of the waves.
 template <class T, bool FP8, int DP>
 __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, uint8_t* v0, uint8_t* v1, uint8_t* v2,
                                             uint8_t* v3) {
@@ -1080,7 +1085,8 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a
 // Partial results of a row brought to one maximum, summed, divided and rounded.
 // A block takes one row: `lanes` threads a part, the parts shared out to the
 // others, so that a row's parts are read side by side.  Measured: 2048 rows of 128
-// with 12 parts 5.7 us, 8192 rows with 7 parts 12.6, 128 rows with 5 parts 3.9.
+// with 12 parts 6.0 us (6.5 where the row's request is looked for), 8192 rows with 7
+// parts 12.7, 128 rows with 5 parts 3.8.
 template <class T>
 __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lanes) {
     __shared__ f32x4 lo[kAB];
@@ -1171,7 +1177,11 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     // 4096 with 64 rows 110, 149, with 128 rows 182, 156; behind 512 with 48
     // rows 60, 44.  Where few requests leave compute units idle the stream
     // blocks, being more, can be ahead for longer (16 of 500 behind 4096 with
-    // 128 rows 57, 62).
+    // 128 rows 57, 62).  All of that is for requests of equally many rows.  The
+    // choice is one for the call, by the longest request, so in a step of few long
+    // and many short ones the short ones go through the prefix by tiles of their
+    // own: 255 requests of one token and one of 512 behind 8192 take 1172 us, in two
+    // calls 160 and 109; 60 and four 560, in two calls 45 and 322.
     const uint64_t own_keys = len > prefix ? len - prefix : 0;
     const uint64_t by16 = (req_rows + kStreamRows - 1) / kStreamRows, by128 = (req_rows + kTileRows - 1) / kTileRows;
     p.own_tile = 0.6 * double(own_keys) * double(by16) + double(prefix) * double(req_rows) / kTileRows >

@@ -16,9 +16,13 @@
 // and only the remainder (at most half a turn) goes to 32 bits.  No wave waits
 // for another, so there is no barrier.
 //
-// Measured: 32768 tokens of 32 + 2 x 8 heads of 128, bf16: 155 us, 5.2 TB/s (a copy
-// reaches 5.1); 3998 tokens of 32 + 2 x 4 heads, fp16 into fp8, 19.9 us, 3.9 TB/s;
-// 5001 tokens on three axes 19.8 us, 4.7 TB/s; 16 tokens 4.3 us.
+// Measured: 32768 tokens of 32 + 2 x 8 heads of 128, bf16: 156 us, 5.2 TB/s (a copy
+// reaches 6.0); 3998 tokens of 32 + 2 x 4 heads, fp16 into fp8, 20.4 us, 3.8 TB/s, of
+// which the quotients by the scales are 0.7; 5001 tokens on three axes 20 us, 4.6
+// TB/s; 16 tokens 4.4 us.  8192 tokens of 32 + 2 x 8 heads of 128: bf16 35 us, 5.7
+// TB/s, float32 77 us, 5.2 TB/s, float32 into fp8 67 us, 5.3 TB/s.  Where pairs lie in
+// no whole 16-byte chunks (heads of 80 half turned) or rows start off 16 bytes a lane
+// takes one value at a time: 194 and 191 us, 0.65 and 1.06 TB/s.
 #include "lm_types.h"
 
 namespace kvec {

@@ -465,10 +465,12 @@ int kvec_norm_rotate_write(const kvec_norm_rotate* step, void* stream);
  * pages outside [0, pool_pages) and past the row are left out; a query that
  * sees none gives zeros.  Tokens before cu_q[0] and from cu_q[batch]
  * on are left as they were.
- * out = softmax(scale * q.k) v by query head; head h reads K/V head
+ * out = softmax(scale * q.k) v by query head, in 32 bits but for the softmax's
+ * weights, which are rounded to `dtype` before they multiply v; head h reads K/V head
  * h / (heads / kv_heads).  fp8 K and V stand for value * scale.
  * max_q: the most tokens that a request has (its tokens past that are left as
- * they were, and change nothing for other requests);
+ * they were, and change nothing for other requests); the kind of blocks is chosen
+ * by it once for the call;
  * max_len: about the longest seq_lens (0: pages_per_seq * page_tokens), which
  * only decides how the work is split.  dim: a multiple of 8 (fp8 pool: 16) up to
  * 256.  workspace: kvec_prefix_attention_workspace bytes, 16-byte aligned (0:
