@@ -551,11 +551,14 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     };
     const uint32_t units = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
     const int32_t* const own_row = a.table + uint64_t(it.b) * a.width;
-    // key_page of a unit's keys, by one row where they lie on one side of the prefix's end
+    // Of a key of the unit at `base`.  The row is chosen by lane: chosen once for the
+    // unit, where its keys lie on one side of the prefix's end, the compiler lost the
+    // choice for the fifth unit and read the request's own row there (seen in the
+    // generated code).
     auto unit_page = [&](uint32_t base, uint32_t key) __attribute__((always_inline)) {
-        if (!it.flat && base < a.prefix && base + kTileKeys > a.prefix) return key_page(a, it, base + key);
-        const int32_t* row = it.flat || base < a.prefix ? a.prefix_pages : own_row;
-        return uint32_t(as_global(row)[min(base + key, it.k1 - 1) >> a.shift]);
+        const uint32_t pos = min(base + key, it.k1 - 1);
+        const int32_t* row = it.flat || pos < a.prefix ? a.prefix_pages : own_row;
+        return uint32_t(*as_global(row + (pos >> a.shift)));
     };
     const uint32_t key = lane & 31;
     // The first units, asked for before anything else is: the queries and their
