@@ -186,7 +186,7 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
     ``max_q``: the most tokens of a request; a request's tokens past it are left as
     they were.  The kind of blocks is chosen by it, once for the call: without it every
     request is taken for one of all tokens, which for 64 decoding requests behind 8192
-    shared keys takes six times as long, and a step of few long and many short requests
+    shared keys takes nearly six times as long, and a step of few long and many short requests
     is faster as two calls.  ``max_len``: about the longest of ``seq_lens`` (default:
     what a table row can hold), by which the work is split.  ``scale``: default
     1/sqrt(dim).  ``k_scale``, ``v_scale``: an fp8 pool's, as in

@@ -30,7 +30,8 @@
 // a page holds behind its last token (NaN, say) has no part.  Where some rows of
 // a tile see a key and others do not, a V value that is not finite would reach
 // the others as 0 * NaN: such values are taken out of the product and added to
-// the rows that see them after the loop.
+// the rows that see them after the loop.  (Under a weight that is rounded to 0, in
+// fp16 one of less than 2^-32, an infinity that is not taken out becomes NaN.)
 #include "lm_types.h"
 #include "paged_geom.h"
 
@@ -416,17 +417,16 @@ __device__ __forceinline__ void emit4(Args& a, const Item& it, uint32_t token, u
 // accordingly).  An fp8 pool's values are widened on the way, by register.
 //
 // Measured, 32 query heads to 8 K/V heads of 128, bf16: 4 x 2048 tokens behind 8192
-// 1270 us, 973 TFLOP/s, where a library product of 8192 x 8192 x 8192 reaches 1265
-// (fp16 1287, fp8 pool 1271); the same at 64 / 16 heads of 64 835 TFLOP/s, 32 / 8 of
-// 80 741 and of 96 869 (80 takes rows of 16 chunks in LDS, six of them zeros), of 192
-// 534 (in the kernel of 256 values, a quarter of its products by zeros), 16 / 4 of
-// 256 708 (one block a compute unit); 16 x 2048 with no prefix 748;
-// 16 x 128 behind 4096 157 us, 889 TFLOP/s (512 blocks, all at once: their start
-// and end are not hidden behind others).  256 requests of one token behind 32768,
-// four K/V heads: 171 us, with an fp8 pool 176.  No one part bounds it: the matrix
-// units are busy 41 % of the time and instructions issue in 69 %; without the
-// powers the 1270 us become 1186, without either product about 1000, without the
-// loads to LDS 1068.
+// 1216 us, 1017 TFLOP/s, where a library product of 8192 x 8192 x 8192 reaches 1267
+// (fp16 1243, fp8 pool 1223); the same at 64 / 16 heads of 64 866 TFLOP/s, 32 / 8 of
+// 80 763 and of 96 892 (80 takes rows of 16 chunks in LDS, six of them zeros), of 192
+// 562 (in the kernel of 256 values, a quarter of its products by zeros), 16 / 4 of
+// 256 741 (one block a compute unit); 16 x 2048 with no prefix 765; 16 x 128 behind
+// 4096 151 us, 926 TFLOP/s (512 blocks, all at once: their start and end are not
+// hidden behind others).  No one part bounds it: the matrix units are busy 46 % of
+// the time and instructions issue in 72 %; when the whole took 1270 us, without the
+// powers it took 1186, without either product about 1000, without the loads to LDS
+// 1068.
 template <int DP>
 struct TileGeom {
     static constexpr int ROW = DP == 64 ? 128 : DP <= 128 ? 256 : 512;   // bytes of a key's row in LDS
@@ -1183,8 +1183,8 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     // 128 rows 57, 62).  All of that is for requests of equally many rows.  The
     // choice is one for the call, by the longest request, so in a step of few long
     // and many short ones the short ones go through the prefix by tiles of their
-    // own: 255 requests of one token and one of 512 behind 8192 take 1172 us, in two
-    // calls 160 and 109; 60 and four 560, in two calls 45 and 322.
+    // own: 255 requests of one token and one of 512 behind 8192 take 1125 us, in two
+    // calls 160 and 106; 60 and four 538, in two calls 45 and 299.
     const uint64_t own_keys = len > prefix ? len - prefix : 0;
     const uint64_t by16 = (req_rows + kStreamRows - 1) / kStreamRows, by128 = (req_rows + kTileRows - 1) / kTileRows;
     p.own_tile = 0.6 * double(own_keys) * double(by16) + double(prefix) * double(req_rows) / kTileRows >
