@@ -46,6 +46,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // The running maximum moves only when a score passes it by this much (in
 // powers of two): p stays under 2^8, and most tiles rescale nothing.
 constexpr float kLazy = 8.0f;
+// Powers are formed as 2^(s c - m c), one operation, where m c is up to this; past
+// it the rounding of m c counts (from 2^24 on in whole powers of two, so that a row
+// could become 0 or infinite), and the maximum is taken off the score first.
+constexpr float kFar = 256.0f;
+constexpr float kFloatMax = 3.402823466e38f;
 // Powers are formed 2^7 times as large where they are rounded to fp16, whose
 // smallest numbers, 2^-24, would otherwise be short for a long tail far under a
 // peak: 2^18 keys of 2^-25.5 all became 0.  The largest is 2^15 then (fp16 ends at
@@ -145,7 +150,7 @@ struct AttnArgs {
     const int32_t* cu;                         // null: one token a request
     const float *k_scale, *v_scale;
     float* ws_o;                               // [parts][rows][dim]
-    f32x2* ws_ml;                              // [parts][rows]: maximum (powers of two), sum
+    f32x2* ws_ml;                              // [parts][rows]: maximum, sum
     uint32_t rec, token_bytes;                 // bytes of a token record, of its K
     uint32_t tokens, batch, heads, kv_heads, group, dim;
     uint32_t width, shift, pool_pages, cap;    // cap: positions that a table row covers
@@ -624,7 +629,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     const uint32_t block_low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
 
     const float c = fabsf(c0);
-    const float lazy = kLazy / c;
+    const float lazy = fminf(kLazy / c, kFloatMax);
     float m = -INFINITY, l = 0.0f, mc = 0.0f, bar = -INFINITY;   // bar: the score that moves m
     f32x16 o[DB];
 #pragma unroll
@@ -680,8 +685,12 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             const float to = fmaxf(m, top);
             const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
             m = to;
-            bar = m + lazy;
-            mc = m == -INFINITY ? 0.0f : m * c - kLift<T>;
+            // a row with scores past kFar comes here with every unit
+            const float off = fabsf(m) * c > kFar && m != -INFINITY ? m : 0.0f;
+            bar = off != 0.0f ? -INFINITY : m + lazy;
+            mc = (off != 0.0f || m == -INFINITY ? 0.0f : m * c) - kLift<T>;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] -= off;
             l *= f;
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -803,7 +812,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     const float inv = l > 0.0f ? vs / l : l == l ? 0.0f : l;
     if (!e.direct && anew(h) == 0) {
         const uint64_t at = uint64_t(it.part) * e.tokens * e.heads + uint64_t(to_token) * e.heads + to_head;
-        *as_global(e.ws_ml + at) = f32x2{m == -INFINITY ? -INFINITY : m * c, l};
+        *as_global(e.ws_ml + at) = f32x2{m, l};
     }
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -980,9 +989,10 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= f;
         }
-        const float mc = m == -INFINITY ? 0.0f : m * c - kLift<T>;
+        const float off = m == -INFINITY ? 0.0f : m;
+        const float lift = __uint_as_float(anew(__float_as_uint(kLift<T>)));   // not held in a scalar register
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], c, -mc));
+        for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4] - off, c, lift));
         // sum over keys 4 g .. and 16 + 4 g .. : what the lane's scores are of
         const u32x4 p = {pack2(s[0][0], s[0][1], ty), pack2(s[0][2], s[0][3], ty), pack2(s[1][0], s[1][1], ty),
                          pack2(s[1][2], s[1][3], ty)};
@@ -1057,7 +1067,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
         const uint32_t tr = fdiv(rw, a.by_group), tk = it.t0 + tr, hd = it.head * a.group + rw - tr * a.group;
         if (!a.direct && d == 0) {
             const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(tk) * a.heads + hd;
-            *as_global(a.ws_ml + at) = f32x2{mx == -INFINITY ? -INFINITY : mx * c, sum};
+            *as_global(a.ws_ml + at) = f32x2{mx, sum};
         }
         emit4<T>(a, it, tk, hd, d, x, sum > 0.0f ? vs / sum : sum == sum ? 0.0f : sum);
     }
@@ -1099,6 +1109,7 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
     const uint32_t each = kAB / lanes, mine = tid / lanes, d = tid % lanes * 4;
     const uint32_t parts = a.parts_flat + a.parts_own;
     float top = -INFINITY, l = 0.0f;
+    const float c = fabsf(score_factor(a));
     f32x4 o = {0, 0, 0, 0};
     for (uint32_t p = tid & 63; p < parts; p += 64) top = fmaxf(top, as_global(a.ws_ml)[uint64_t(p) * rows + row].x);
 #pragma unroll
@@ -1108,7 +1119,7 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
         const uint64_t at = uint64_t(p) * rows + row;
         const f32x2 ml = as_global(a.ws_ml)[at];
         if (ml.x == -INFINITY) continue;                  // nothing seen there
-        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        const float f = __builtin_amdgcn_exp2f((ml.x - top) * c);
         l += ml.y * f;
         if (d < a.dim) o += *as_global(reinterpret_cast<const f32x4*>(a.ws_o + at * a.dim + d)) * f;
     }
