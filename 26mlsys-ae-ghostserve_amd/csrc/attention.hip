@@ -1255,7 +1255,8 @@ inline int check_attention(const kvec_attention* s, const char* fn) {
         return set_error(KVEC_EINVAL, "%s: prefix=%lld past the page table", fn, (long long)s->prefix);
     if (s->cu_q ? s->max_q < 1 && s->tokens > 0 : s->tokens != s->batch)
         return set_error(KVEC_EINVAL, "%s: max_q=%d tokens=%lld batch=%d", fn, s->max_q, (long long)s->tokens, s->batch);
-    if (!(s->scale >= 0.0f) || s->scale > 3e38f) return set_error(KVEC_EINVAL, "%s: scale must be finite and not negative", fn);
+    if (!(s->scale >= 0.0f) || s->scale > kFloatMax / kLog2e)
+        return set_error(KVEC_EINVAL, "%s: scale must not be negative, and finite times log2(e)", fn);
     if (s->tokens * s->heads >= (int64_t(1) << 31) / 64 || int64_t(s->batch) * s->pages_per_seq >= (int64_t(1) << 31))
         return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
     return KVEC_OK;

@@ -93,3 +93,14 @@ def test_rows_of_the_result_that_overlap(pkg, n, h):
             assert L.kvec_prefix_attention(C.byref(call), 1 << 50, 1 << 40, None) == -1
             assert (b"rows of out overlap" in L.kvec_last_error()) == meet, (s, t)
     assert seen == ({False} if n * h == 1 else {False, True})
+
+
+def test_scales_that_overflow(pkg):
+    """A scale whose product with log2(e) is no 32-bit number would make NaN of every row."""
+    L = pkg._lib.lib()
+    for scale, code in ((2.5e38, -1), (3.4e38, -1), (2.2e38, 0)):
+        call = at(pkg, scale=scale)
+        need = L.kvec_prefix_attention_workspace(C.byref(call))
+        assert (need < 0) == (code < 0)
+        if code:
+            assert b"scale" in L.kvec_last_error()
