@@ -14,6 +14,7 @@ signatures:
   chunked     per-prefill-chunk RDP + RS coding of a paged (e.g. fp8) cache
   attention   per-head norm + rotation + cache write, and attention with a
               shared prefix, over the same pool
+  blockscale  the pool in 8 or 4 bits with block scales; its tokens read back
   offload     parity copies to pinned host memory on a side stream
   serving     forward_extend hook: per-step KV delta parity, JSONL metrics;
               an attention backend over the pool
@@ -21,6 +22,6 @@ signatures:
 Import the package with ``importlib.import_module("26mlsys-ae-ghostserve_amd")``
 (the directory name is not a Python identifier).
 """
-from . import _lib, attention, chunked, offload, paged, rdp, rdp_kv_ops, rs, serving, spec, xor  # noqa: F401
+from . import _lib, attention, blockscale, chunked, offload, paged, rdp, rdp_kv_ops, rs, serving, spec, xor  # noqa: F401
 
-__all__ = ["xor", "rdp", "rs", "rdp_kv_ops", "spec", "paged", "chunked", "attention", "offload", "serving"]
+__all__ = ["xor", "rdp", "rs", "rdp_kv_ops", "spec", "paged", "chunked", "attention", "blockscale", "offload", "serving"]

@@ -150,6 +150,22 @@ class NormRotate(C.Structure):
     ]
 
 
+class BlockRead(C.Structure):
+    """struct kvec_block_read of include/kvec.h."""
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("kv_heads", C.c_int),
+        ("dim", C.c_int),
+        ("pool_dtype", C.c_int),
+        ("pool", C.c_void_p),
+        ("n_slots", C.c_int64),
+        ("slots", C.c_void_p),
+        ("dtype", C.c_int),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+    ]
+
+
 class Attention(C.Structure):
     """struct kvec_attention of include/kvec.h."""
     _fields_ = [
@@ -188,6 +204,7 @@ class Attention(C.Structure):
 # small call is bound by its host time.  Formats in the order of the fields.
 STEP_FORMAT = struct.Struct("@PiiiqPPPqPPqPPP")
 NORM_ROTATE_FORMAT = struct.Struct("@qiiiiPPPqqqqqqPqqifPPiiiPqPPfPiqPPPP")
+BLOCK_READ_FORMAT = struct.Struct("@qiiiPqPiPP")
 ATTENTION_FORMAT = struct.Struct("@qiiiiiPqqPqqPiqiPiPPiqqPfPP")
 
 
@@ -245,6 +262,7 @@ SIGNATURES = {
     "kvec_gf16_tables": (_i, [_vp, _vp]),
     "kvec_step_tables": (_i, [_vp, _vp]),
     "kvec_norm_rotate_write": (_i, [_vp, _vp]),
+    "kvec_block_read_kv": (_i, [_vp, _vp]),
     "kvec_prefix_attention_workspace": (_i64, [_vp]),
     "kvec_prefix_attention": (_i, [_vp, _vp, _i64, _vp]),
 }

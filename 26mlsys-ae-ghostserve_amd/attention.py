@@ -13,13 +13,15 @@ a gradient are refused (under ``torch.no_grad()`` nothing asks for one).
 
 Pool tensor: [layers, pool_pages, page_tokens, 2 (K,V), kv_heads, head_dim], of
 the queries' type or float8_e4m3fn with a scale for K and for V, as in
-:mod:`.paged`; slots and page tables as :func:`.paged.step_tables` makes them.
+:mod:`.paged`, or a :class:`.blockscale.BlockPool`, in 8 or 4 bits with scales that are
+found as it is written; slots and page tables as :func:`.paged.step_tables` makes them.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib
+from .blockscale import BlockPool
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
 _FLOAT_MAX = torch.finfo(torch.float32).max
@@ -44,8 +46,11 @@ def rotary_axes(sections, device="cuda") -> torch.Tensor:
     return torch.repeat_interleave(torch.arange(len(sections), dtype=torch.uint8), n).to(device)
 
 
-def _layer(pool: torch.Tensor, layer: int) -> tuple[int, int, int, int]:
-    """(address of the layer, slots, kv_heads, head_dim) of a pool."""
+def _layer(pool: torch.Tensor | BlockPool, layer: int, dtype: torch.dtype) -> tuple[int, int, int, int, int]:
+    """(address of the layer, slots, kv_heads, head_dim, KVEC_* type) of a pool beside
+    queries of ``dtype``."""
+    if isinstance(pool, BlockPool):
+        return (*pool.layer(layer), pool.kv_heads, pool.dim, pool.code)
     shape = pool.shape
     if len(shape) != 6 or shape[3] != 2:
         raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
@@ -54,8 +59,15 @@ def _layer(pool: torch.Tensor, layer: int) -> tuple[int, int, int, int]:
     L, pages, pt, _, H, D = shape
     if not 0 <= layer < L:
         raise ValueError(f"layer {layer} not in [0, {L})")
-    n = pages * pt
-    return pool.data_ptr() + layer * n * 2 * H * D * pool.element_size(), n, H, D
+    n, pool_dt = pages * pt, pool.dtype
+    if pool_dt != dtype and pool_dt != torch.float8_e4m3fn:
+        raise ValueError("pool must be of q's type, float8_e4m3fn or a BlockPool")
+    return pool.data_ptr() + layer * n * 2 * H * D * pool.element_size(), n, H, D, _DTYPES[pool_dt]
+
+
+def _data(pool) -> torch.Tensor:
+    """The tensor that holds a pool."""
+    return pool.data if isinstance(pool, BlockPool) else pool
 
 
 def _scale(t, device, what: str):
@@ -72,7 +84,7 @@ def _ptr(t) -> int:
 
 
 def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor | None,
-                      freqs: torch.Tensor | None, pool: torch.Tensor, slots: torch.Tensor, *, layer: int = 0,
+                      freqs: torch.Tensor | None, pool: torch.Tensor | BlockPool, slots: torch.Tensor, *, layer: int = 0,
                       norm: bool = True, q_weight: torch.Tensor | None = None,
                       k_weight: torch.Tensor | None = None, eps: float = 1e-6,
                       axis_of: torch.Tensor | None = None, interleaved: bool = False, factor: float = 1.0,
@@ -92,7 +104,9 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
 
     Token t's K and V go to slot ``slots[t]`` (int32, page * page_tokens + place;
     negative or past the pool: none) of the pool's ``layer``, in the queries' type
-    or, float8_e4m3fn, as value / scale.  The slots of a call must be distinct.
+    or, float8_e4m3fn, as value / scale, or, a :class:`.blockscale.BlockPool`, as codes
+    with their blocks' scales (K computed in 64 bits and rounded to 32 first, so that its
+    codes do not hang on how the sums were split).  The slots of a call must be distinct.
     ``tokens`` (int32 [1] on the GPU, e.g. ``cu_new[-1:]``): tokens from that
     number on are left as they were, here and in the result.
 
@@ -103,16 +117,14 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     dev, dt = q.device, q.dtype
     if dt not in _COMPUTE or k.dtype != dt or v.dtype != dt:
         raise ValueError("q, k and v must be of one type: float32, bfloat16 or float16")
-    _lib.require_no_grad(q, k, v, q_weight, k_weight, pool, out, what="norm_rotate_write")
-    _lib.require_same_device(dev, k, v, positions, freqs, pool, slots, q_weight, k_weight, axis_of, tokens, out,
+    data = _data(pool)
+    _lib.require_no_grad(q, k, v, q_weight, k_weight, data, out, what="norm_rotate_write")
+    _lib.require_same_device(dev, k, v, positions, freqs, data, slots, q_weight, k_weight, axis_of, tokens, out,
                              what="norm_rotate_write tensor")
     N, Hq, D = qs
-    base, n_slots, Hk, Dp = _layer(pool, layer)
+    base, n_slots, Hk, Dp, pool_dt = _layer(pool, layer, dt)
     if Hk != ks[1] or Dp != D:
         raise ValueError(f"pool holds {Hk} heads of {Dp}, k has {ks[1]} of {D}")
-    pool_dt = pool.dtype
-    if pool_dt != dt and pool_dt != torch.float8_e4m3fn:
-        raise ValueError("pool must be of q's type or float8_e4m3fn")
     (q0, q1, q2), (k0, k1, k2), (v0, v1, v2) = q.stride(), k.stride(), v.stride()
     if D > 1 and N and not q2 == k2 == v2 == 1:
         raise ValueError("a head's values must be adjacent")
@@ -152,13 +164,13 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     s = _lib.pack(
         _lib.NORM_ROTATE_FORMAT, N, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), q0, q1, k0, k1,
         v0, v1, out.data_ptr(), o0, o1, bool(norm), eps, _ptr(q_weight), _ptr(k_weight), 2 * half, bool(interleaved),
-        axes, _ptr(positions), axis_stride, _ptr(axis_of), _ptr(freqs), factor, base, _DTYPES[pool_dt], n_slots,
+        axes, _ptr(positions), axis_stride, _ptr(axis_of), _ptr(freqs), factor, base, pool_dt, n_slots,
         slots.data_ptr(), _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"), _ptr(tokens))
     _lib.call_on(dev, "kvec_norm_rotate_write", s, _lib.stream_handle(dev))
     return out
 
 
-def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+def prefix_attention(q: torch.Tensor, pool: torch.Tensor | BlockPool, page_table: torch.Tensor, seq_lens: torch.Tensor,
                      prefix: int = 0, *, layer: int = 0, cu_q: torch.Tensor | None = None,
                      max_q: int | None = None, max_len: int | None = None,
                      prefix_pages: torch.Tensor | None = None, scale: float | None = None,
@@ -172,7 +184,8 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
     ``seq_lens[b]`` tokens, its new ones included (their K and V are in the pool
     already, see :func:`norm_rotate_write`), on the pages of its row of
     ``page_table``; each query sees the positions up to its own.  Query heads
-    share K/V heads in order.  dim: a multiple of 8 (fp8 pool: 16) up to 256.
+    share K/V heads in order.  dim: a multiple of 8 (fp8 pool: 16, a BlockPool: 32) up to
+    256.  K and V of a BlockPool are what :func:`.blockscale.read` gives in the queries' type.
 
     The first ``prefix`` positions are the same for all requests; they are read
     from ``prefix_pages`` (default: the first row of ``page_table``, which has to hold
@@ -209,14 +222,12 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
         raise ValueError(f"seq_lens must be [{B}] and cu_q int32 [{B + 1}]")
     if cu_q is None and N != B:
         raise ValueError("without cu_q there is one query token a request")
-    _lib.require_no_grad(q, pool, out, what="prefix_attention")
-    _lib.require_same_device(dev, pool, page_table, seq_lens, cu_q, prefix_pages, out, what="prefix_attention tensor")
-    base, _, Hk, Dp = _layer(pool, layer)
+    data = _data(pool)
+    _lib.require_no_grad(q, data, out, what="prefix_attention")
+    _lib.require_same_device(dev, data, page_table, seq_lens, cu_q, prefix_pages, out, what="prefix_attention tensor")
+    base, _, Hk, Dp, pool_dt = _layer(pool, layer, dt)
     if Dp != D or Hq % Hk:
         raise ValueError(f"q has {Hq} heads of {D}, the pool {Hk} of {Dp}")
-    pool_dt = pool.dtype
-    if pool_dt != dt and pool_dt != torch.float8_e4m3fn:
-        raise ValueError("pool must be of q's type or float8_e4m3fn")
     for t in (page_table, seq_lens, cu_q, prefix_pages):
         if t is not None and not t.is_contiguous():
             raise ValueError("page_table, seq_lens, cu_q and prefix_pages must be contiguous")
@@ -243,7 +254,7 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tens
         return out
     s = _lib.pack(
         _lib.ATTENTION_FORMAT, N, B, Hq, Hk, D, _DTYPES[dt], q.data_ptr(), q0, q1, out.data_ptr(), Hq * D, D, base,
-        _DTYPES[pool_dt], pages, pt, page_table.data_ptr(), width, seq_lens.data_ptr(), _ptr(cu_q), max_q, max_len,
+        pool_dt, pages, pt, page_table.data_ptr(), width, seq_lens.data_ptr(), _ptr(cu_q), max_q, max_len,
         prefix, front.data_ptr(), scale, _scale(k_scale, dev, "k_scale"), _scale(v_scale, dev, "v_scale"))
     need = _lib.lib().kvec_prefix_attention_workspace(s)
     ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None

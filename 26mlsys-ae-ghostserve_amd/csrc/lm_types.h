@@ -133,8 +133,21 @@ inline bool rows_overlap(int64_t n, int64_t s, int64_t h, int64_t t, int64_t len
 // HIP's limit: the threads of a launch are fewer than 2^32.
 inline bool launchable(uint64_t blocks, uint32_t threads) { return blocks < (uint64_t(1) << 32) / threads; }
 
+// A pool with block scales: bits of a value's code, 0 for other types.
+inline int block_bits(int dtype) { return dtype == KVEC_BLOCK_E4M3 ? 8 : dtype == KVEC_BLOCK_E2M1 ? 4 : 0; }
+constexpr int kScaleBlock = 32;   // neighbouring values of a head that share a scale
+constexpr int kMaxBlockDim = 256;
+
 inline int64_t type_bytes(int dtype) {
     return dtype == KVEC_F32 ? 4 : dtype == KVEC_BF16 || dtype == KVEC_F16 ? 2 : dtype == KVEC_FP8_E4M3 ? 1 : 0;
+}
+
+// Bytes of K (or V) of one token in one layer of a pool; with block scales codes,
+// a byte for each block, and up to 15 unused ones.
+inline uint64_t half_bytes(int kv_heads, int dim, int dtype) {
+    const uint64_t n = uint64_t(kv_heads) * uint64_t(dim);
+    const int bits = block_bits(dtype);
+    return bits ? (n * uint64_t(bits) / 8 + n / kScaleBlock + 15) / 16 * 16 : n * uint64_t(type_bytes(dtype));
 }
 
 }  // namespace kvec

@@ -23,52 +23,9 @@
 // TB/s, float32 77 us, 5.2 TB/s, float32 into fp8 67 us, 5.3 TB/s.  Where pairs lie in
 // no whole 16-byte chunks (heads of 80 half turned) or rows start off 16 bytes a lane
 // takes one value at a time: 194 and 191 us, 0.65 and 1.06 TB/s.
-#include "lm_types.h"
+#include "norm_rotate.h"
 
 namespace kvec {
-
-constexpr int kNRB = 256;
-constexpr int kMaxDim = 512;
-constexpr int kMaxHalf = kMaxDim / 2;
-
-struct NrArgs {
-    const uint8_t *q, *k, *v;
-    uint8_t* o;
-    int64_t qs, qh, ks, kh, vs, vh, os, oh;   // elements
-    const uint8_t *wq, *wk;
-    const int32_t* pos;
-    int64_t axis_stride;
-    const uint8_t* axis_of;
-    const double* freqs;
-    uint8_t* pool;
-    const int32_t* slots;
-    const float *k_scale, *v_scale;
-    const int32_t* n_tokens;
-    int64_t n_slots;
-    FastDiv div_chunks;                       // pieces of a token's rows, one wave each
-    uint32_t items;                           // tokens * pieces
-    uint32_t heads, kv_heads, dim, rot, axes;
-    uint32_t lg;                              // log2 of the lanes of a row
-    int norm, interleaved;
-    float eps, factor;
-};
-
-// The two chunks of unit u: first values at a and b (b == dim: there is none).
-template <int W>
-__device__ __forceinline__ void unit_at(const NrArgs& p, uint32_t u, uint32_t& a, uint32_t& b, uint32_t& pair,
-                                        bool& turned) {
-    const uint32_t half = p.rot / 2, nu = half / W;
-    turned = u < nu;
-    if (turned) {
-        pair = u * W;
-        a = p.interleaved ? 2 * u * W : u * W;
-        b = p.interleaved ? a + W : half + u * W;
-    } else {
-        pair = 0;
-        a = min(p.rot + (u - nu) * 2 * W, p.dim);
-        b = min(a + W, p.dim);
-    }
-}
 
 template <class T, class PT, int W, int NU, int ITER>
 __global__ __launch_bounds__(kNRB) void norm_rotate_kernel(NrArgs p) {
@@ -251,10 +208,13 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
         return set_error(KVEC_EINVAL, "%s: rot=%d must be even and at most dim=%d", fn, s->rot, s->dim);
     if (s->dtype != KVEC_F32 && s->dtype != KVEC_BF16 && s->dtype != KVEC_F16)
         return set_error(KVEC_EINVAL, "%s: dtype %d", fn, s->dtype);
-    if (s->pool_dtype != s->dtype && s->pool_dtype != KVEC_FP8_E4M3)
-        return set_error(KVEC_EINVAL, "%s: pool_dtype %d is neither dtype nor fp8", fn, s->pool_dtype);
-    if (s->pool_dtype == s->dtype && (s->k_scale || s->v_scale))
+    const bool blocks = block_bits(s->pool_dtype) != 0;
+    if (s->pool_dtype != s->dtype && s->pool_dtype != KVEC_FP8_E4M3 && !blocks)
+        return set_error(KVEC_EINVAL, "%s: pool_dtype %d is neither dtype, fp8 nor one with block scales", fn, s->pool_dtype);
+    if (s->pool_dtype != KVEC_FP8_E4M3 && (s->k_scale || s->v_scale))
         return set_error(KVEC_EINVAL, "%s: scales are an fp8 pool's", fn);
+    if (blocks && (s->dim % kScaleBlock || s->dim > kMaxBlockDim))
+        return set_error(KVEC_EUNSUPPORTED, "%s: dim=%d must be a multiple of %d up to %d", fn, s->dim, kScaleBlock, kMaxBlockDim);
     if (s->rot && (s->axes < 1 || s->axes > 8 || s->axis_stride < 0 || s->axis_stride > (int64_t(1) << 40)))
         return set_error(KVEC_EINVAL, "%s: axes=%d axis_stride=%lld", fn, s->axes, (long long)s->axis_stride);
     if (s->norm && !(s->eps >= 0.0f)) return set_error(KVEC_EINVAL, "%s: eps must not be negative", fn);
@@ -262,7 +222,7 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     if (!s->q || !s->k || !s->v || !s->q_out || !s->slots || (s->n_slots && !s->pool) ||
         (s->rot && (!s->positions || !s->freqs)))
         return set_error(KVEC_EINVAL, "%s: null array", fn);
-    const int64_t es = type_bytes(s->dtype), ps = type_bytes(s->pool_dtype);
+    const int64_t es = type_bytes(s->dtype);
     const int64_t str[8] = {s->q_stride, s->q_head_stride, s->k_stride, s->k_head_stride,
                             s->v_stride, s->v_head_stride, s->o_stride, s->o_head_stride};
     for (int64_t x : str)
@@ -273,7 +233,7 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     auto span = [&](const void* p, int64_t st, int64_t hs, int64_t h, const char* name) {
         return Span{p, uint64_t((s->tokens - 1) * st + (h - 1) * hs + s->dim) * uint64_t(es), name, -1};
     };
-    const uint64_t pool_bytes = uint64_t(s->n_slots) * 2 * uint64_t(s->kv_heads) * uint64_t(s->dim) * uint64_t(ps);
+    const uint64_t pool_bytes = uint64_t(s->n_slots) * 2 * half_bytes(s->kv_heads, s->dim, s->pool_dtype);
     const Span q = span(s->q, s->q_stride, s->q_head_stride, s->heads, "q"),
                k = span(s->k, s->k_stride, s->k_head_stride, s->kv_heads, "k"),
                v = span(s->v, s->v_stride, s->v_head_stride, s->kv_heads, "v"),
@@ -307,8 +267,9 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     // 31.6; 16384 69.9, 67.6; 65536 270.9, 246.7.
     const uint64_t waves1 = uint64_t(s->tokens) * ((rows + groups - 1) / groups);
     const bool deep = wide && waves1 >= 12 * 256 * 32;
+    if (s->tokens >= (int64_t(1) << 32)) return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
     const uint32_t per = groups * (deep ? 3 : 1), chunks = (rows + per - 1) / per;
-    if (s->tokens >= (int64_t(1) << 32) || !launchable((uint64_t(s->tokens) * chunks + 3) / 4, kNRB))
+    if (!blocks && !launchable((uint64_t(s->tokens) * chunks + 3) / 4, kNRB))
         return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
     a.q = (const uint8_t*)s->q;
     a.k = (const uint8_t*)s->k;
@@ -339,6 +300,7 @@ extern "C" int kvec_norm_rotate_write(const kvec_norm_rotate* s, void* stream) {
     a.interleaved = s->interleaved;
     a.eps = s->eps;
     a.factor = s->factor;
+    if (blocks) return launch_block_write(a, s->tokens, s->dtype, s->pool_dtype, wide, fn, stream);
     const bool fp8 = s->pool_dtype == KVEC_FP8_E4M3;
     NrFn f = s->dtype == KVEC_F32 ? pick_nr_pool<float>(fp8, wide, deep)
              : s->dtype == KVEC_BF16 ? pick_nr_pool<__bf16>(fp8, wide, deep)

@@ -3,7 +3,8 @@ bench_ghostserve_rdp.py:440-458, over a paged pool), and the fused
 gather + RDP encode that codes a prefill chunk straight out of the pool.
 
 Pool tensor: [layers, pool_pages, page_tokens, 2 (K,V), kv_heads, head_dim] of
-any dtype (coded as raw bytes).  Page table: int32 [batch, pages_per_seq] of
+any dtype (coded as raw bytes), or a :class:`.blockscale.BlockPool` (its codes and
+scales likewise).  Page table: int32 [batch, pages_per_seq] of
 pool page indices.  Stream of a chunk of ``tokens`` positions starting at
 ``tok_off``: the chunk's token records in order,
 [layers, batch, tokens, 2 (K,V), kv_heads, head_dim], so each pool page
@@ -20,13 +21,16 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _lib
+from .blockscale import BlockPool
 
 
 class PagedKV:
     """A chunk of a paged KV pool: the descriptor the kernels take."""
 
-    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, tok_off: int = 0,
+    def __init__(self, pool: torch.Tensor | BlockPool, page_table: torch.Tensor, tok_off: int = 0,
                  tokens: int | None = None):
+        if isinstance(pool, BlockPool):
+            pool = pool.records
         if pool.dim() != 6 or pool.shape[3] != 2:
             raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
         if page_table.dtype != torch.int32 or page_table.dim() != 2:

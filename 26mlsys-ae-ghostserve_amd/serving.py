@@ -57,6 +57,7 @@ import numpy as np
 import torch
 
 from . import _lib, attention, paged
+from .blockscale import BlockPool
 
 
 def _dist():
@@ -452,7 +453,8 @@ class PagedBackend:
     pool, the requests' shared prefix once for all; the hook then codes the
     slots that it wrote.  A decode step is one new token a request.
 
-    ``pool``: [layers, pages, page_tokens, 2, kv_heads, head_dim];
+    ``pool``: [layers, pages, page_tokens, 2, kv_heads, head_dim], or a
+    :class:`.blockscale.BlockPool`, whose records the hook codes as they are;
     ``page_table``: int32 [batch, pages_per_seq], whose rows start with the prefix's
     pages (whole pages where requests go on behind it).  ``prefix_pages``: those pages
     on their own, int32; without it they are read from the first row, whose request
@@ -461,11 +463,11 @@ class PagedBackend:
     ``axis_of``, ``interleaved``, ``factor`` and scales as in
     :func:`.attention.norm_rotate_write`.  The hook codes pools of 2-byte types."""
 
-    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, layer: int = 0, prefix: int = 0,
+    def __init__(self, pool: torch.Tensor | BlockPool, page_table: torch.Tensor, layer: int = 0, prefix: int = 0,
                  freqs: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                  prefix_pages: Optional[torch.Tensor] = None, **norm):
-        if pool.dim() != 6 or pool.shape[3] != 2:
+        if len(pool.shape) != 6 or pool.shape[3] != 2:
             raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
         if not 0 <= layer < pool.shape[0]:
             raise ValueError(f"layer {layer} not in [0, {pool.shape[0]})")
@@ -475,8 +477,11 @@ class PagedBackend:
 
     @property
     def kv_buffer(self) -> torch.Tensor:
-        """The layer as a token pool, [max_tokens, 2, kv_heads, head_dim]."""
+        """The layer as a token pool, [max_tokens, 2, kv_heads, head_dim]; a BlockPool's
+        as 2-byte words, [max_tokens, 2, 1, words of a half record]."""
         _, pages, pt, _, H, D = self.pool.shape
+        if isinstance(self.pool, BlockPool):
+            return self.pool.data[self.layer].view(torch.int16).view(pages * pt, 2, 1, -1)
         return self.pool[self.layer].view(pages * pt, 2, H, D)
 
     def begin(self, cached: torch.Tensor, new: torch.Tensor, free_pages: torch.Tensor, tokens: int,

@@ -43,7 +43,7 @@ extern "C" {
  * neither).  1.1.0: kvec_hook_step added.  1.2.0: the *_kv entry points over
  * kvec_kv_bhtd added.  1.3.0: kvec_step_tables, kvec_norm_rotate_write,
  * kvec_prefix_attention added. */
-#define KVEC_VERSION 10300
+#define KVEC_VERSION 10400
 int kvec_version(void);
 /* Static description of a KVEC_E* code. */
 const char* kvec_strerror(int code);
@@ -381,6 +381,18 @@ int kvec_gf16_tables(uint16_t* gf_exp, uint16_t* gf_log);
 #define KVEC_BF16 1
 #define KVEC_F16 2
 #define KVEC_FP8_E4M3 3 /* the finite-only e4m3 of the OCP 8-bit formats */
+/* Pools of 8 or 4 bits a value with block scales (the OCP microscaling formats'
+ * elements and scales).  K (or V) of a token is a half record of kv_heads * dim
+ * codes (e4m3 bytes; e2m1, 0 .5 1 1.5 2 3 4 6 and a sign, two to a byte, the first
+ * in the low half), then a byte for each block of 32 neighbouring values of a head,
+ * then up to 15 bytes, never written, to a multiple of 16.  A value is code *
+ * 2^(byte - 127); byte 255: NaN, all 32.  dim: a multiple of 32 up to 256.
+ * Writing: byte - 127 is the smallest whole number >= -127 with which no value of
+ * the block passes the largest code (448, 6), codes are the nearest ones, ties to
+ * even; a block with an infinity or NaN gets 255; values that would round past the
+ * largest of the type they come from become the last that does not. */
+#define KVEC_BLOCK_E4M3 4
+#define KVEC_BLOCK_E2M1 5
 
 /* Page table rows and slots of a step, from the requests' lengths.  Request b
  * holds `cached[b]` tokens and gets `new_tokens[b]` more (negative: none).  Its
@@ -421,7 +433,10 @@ int kvec_step_tables(const kvec_step* step, void* stream);
  *   factor * cos, factor * sin of positions[axis_of[i]][t] * freqs[i]
  * Pair i is (x[i], x[i + rot/2]), or (x[2i], x[2i+1]) if interleaved; values
  * from rot on are not turned.  Angles in 64 bits, the rest in 32, one rounding
- * at the end.  An fp8 pool gets x / scale, values past +-448 as +-448.
+ * at the end.  An fp8 pool gets x / scale, values past +-448 as +-448.  For a pool
+ * with block scales keys are computed in 64 bits and rounded to 32 before they are
+ * quantised: a code is a decision, which the noise of 32 bits would make differently
+ * in another kernel, and the bytes are what the codes above protect.
  * Queries go to q_out (q itself with q's strides: in place; k and v may lie
  * between its rows then, but share no values with it).  A slot outside
  * [0, n_slots) is skipped; the slots of a call must be distinct.  Tokens from
@@ -448,7 +463,7 @@ typedef struct kvec_norm_rotate {
     const double* freqs;        /* [rot/2] radians a position */
     float factor;
     void* pool;                 /* the layer: [n_slots][2 (K,V)][kv_heads][dim] */
-    int pool_dtype;             /* dtype, or KVEC_FP8_E4M3 */
+    int pool_dtype;             /* dtype, KVEC_FP8_E4M3, or KVEC_BLOCK_*: [n_slots][2] half records */
     int64_t n_slots;
     const int32_t* slots;       /* [tokens] */
     const float* k_scale;       /* [1] each, device, or NULL: 1 */
@@ -456,6 +471,22 @@ typedef struct kvec_norm_rotate {
     const int32_t* n_tokens;    /* [1], device, or NULL: all */
 } kvec_norm_rotate;
 int kvec_norm_rotate_write(const kvec_norm_rotate* step, void* stream);
+
+/* Tokens of one layer of a pool with block scales read back: token t's K and V, at
+ * slots[t], rounded to `dtype` (values past its largest: infinite) into row t of k and
+ * v; zeros where the slot is outside [0, n_slots). */
+typedef struct kvec_block_read {
+    int64_t tokens;
+    int kv_heads, dim;
+    int pool_dtype;             /* KVEC_BLOCK_E4M3, KVEC_BLOCK_E2M1 */
+    const void* pool;           /* the layer: [n_slots][2 (K,V)] half records */
+    int64_t n_slots;
+    const int32_t* slots;       /* [tokens] */
+    int dtype;                  /* of k and v: KVEC_F32, KVEC_BF16, KVEC_F16 */
+    void* k;                    /* [tokens][kv_heads][dim] */
+    void* v;
+} kvec_block_read;
+int kvec_block_read_kv(const kvec_block_read* call, void* stream);
 
 /* Attention of a step's queries over one layer of the pool, for requests that
  * share their first `prefix` positions (0: none).  Token i of request b's n_b
