@@ -8,6 +8,7 @@ struct AttnPlan {
     bool flat, flat_tile, own_tile;
     uint32_t parts_flat, parts_own, tiles_flat, req_tiles, first;
     uint64_t rows, tiles_own, blocks_flat, blocks;
+    uint32_t side, groups, run_keys;           // pools with block scales: see AttnArgs
     bool direct() const { return parts_flat + parts_own == 1; }
     int64_t bytes(int64_t dim) const {
         return direct() ? 0 : int64_t(uint64_t(parts_flat + parts_own) * rows * (uint64_t(dim) * 4 + 8)) + 16;
@@ -72,10 +73,11 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         // behind 32768 208 (8 splits), 192 (6); 128 of 512 bf16 ones behind
         // 16384 86 (16), 76 (8); 256 of 512 behind 8192, eight K/V heads, 127
         // (5), 114 (3); no own keys, behind 32768, 173 (8), 187 (6).
+        const double value_bytes = s->pool_dtype == KVEC_BLOCK_E2M1 ? 0.5 : s->pool_dtype == s->dtype ? 2.0 : 1.0;
         uint64_t room = 512;
         if (p.flat_tile) {
             const double shared = 2.0 * double(p.tiles_flat) * double(prefix);
-            const double beside = double(B * by16) * double(own_keys) * (s->pool_dtype == KVEC_FP8_E4M3 ? 1.0 : 2.0);
+            const double beside = double(B * by16) * double(own_keys) * value_bytes;
             room = uint64_t(512.0 * shared / (shared + beside));
         }
         p.parts_flat = splits(uint64_t(p.tiles_flat) * Hk, prefix, room);
@@ -83,6 +85,33 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     p.parts_own = splits(own, len > p.first ? len - p.first : 1, 512);
     p.blocks_flat = p.flat ? uint64_t(p.tiles_flat) * Hk * p.parts_flat : 0;
     p.blocks = p.blocks_flat + own * p.parts_own;
+    p.side = Hk >= 3 ? 4 : uint32_t(Hk);
+    p.groups = uint32_t((Hk + p.side - 1) / p.side);
+    if (block_bits(s->pool_dtype)) {
+        // runs: a wave's, eight pairs of rows and runs on as many XCDs
+        auto run_blocks = [&](uint64_t tiles, uint64_t parts) {
+            const uint64_t apart = 4 / p.side, pairs = tiles * ((parts + apart - 1) / apart);
+            return (pairs + 7) / 8 * 8 * p.groups;
+        };
+        auto runs = [&](uint64_t tiles, uint64_t keys, uint32_t* parts) {
+            // about four waves a SIMD, 128 keys a run, 512 runs of a row
+            uint64_t n = 4096 / (tiles * Hk);
+            if (n > keys / 128) n = keys / 128;
+            n = n < 1 ? 1 : n > 512 ? 512 : n;
+            *parts = uint32_t(n);
+            return uint32_t((keys + n - 1) / n + kStreamKeys - 1) / kStreamKeys * kStreamKeys;
+        };
+        uint32_t each = 0;
+        if (p.flat && !p.flat_tile) {
+            each = runs(p.tiles_flat, prefix, &p.parts_flat);
+            p.blocks_flat = run_blocks(p.tiles_flat, p.parts_flat);
+        }
+        if (!p.own_tile) {
+            each = runs(p.tiles_own, len > p.first ? len - p.first : 1, &p.parts_own);
+            p.run_keys = each;
+            p.blocks = p.blocks_flat + run_blocks(p.tiles_own, p.parts_own);
+        }
+    }
     return p;
 }
 
@@ -92,11 +121,12 @@ inline int check_attention(const kvec_attention* s, const char* fn) {
         s->pages_per_seq < 1 || s->pool_pages < 0 || s->prefix < 0)
         return set_error(KVEC_EINVAL, "%s: bad sizes", fn);
     if (s->dtype != KVEC_BF16 && s->dtype != KVEC_F16) return set_error(KVEC_EINVAL, "%s: dtype %d", fn, s->dtype);
-    if (s->pool_dtype != s->dtype && s->pool_dtype != KVEC_FP8_E4M3)
-        return set_error(KVEC_EINVAL, "%s: pool_dtype %d is neither dtype nor fp8", fn, s->pool_dtype);
-    if (s->pool_dtype == s->dtype && (s->k_scale || s->v_scale))
+    const bool blocks = block_bits(s->pool_dtype) != 0;
+    if (s->pool_dtype != s->dtype && s->pool_dtype != KVEC_FP8_E4M3 && !blocks)
+        return set_error(KVEC_EINVAL, "%s: pool_dtype %d is neither dtype, fp8 nor one with block scales", fn, s->pool_dtype);
+    if (s->pool_dtype != KVEC_FP8_E4M3 && (s->k_scale || s->v_scale))
         return set_error(KVEC_EINVAL, "%s: scales are an fp8 pool's", fn);
-    const int unit = s->pool_dtype == KVEC_FP8_E4M3 ? 16 : 8;
+    const int unit = blocks ? kScaleBlock : s->pool_dtype == KVEC_FP8_E4M3 ? 16 : 8;
     if (s->dim > 256 || s->dim % unit)
         return set_error(KVEC_EUNSUPPORTED, "%s: dim=%d must be a multiple of %d up to 256", fn, s->dim, unit);
     if (s->page_tokens < 1 || (s->page_tokens & (s->page_tokens - 1)))
@@ -153,8 +183,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     const int64_t need = p.bytes(s->dim);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return set_error(KVEC_EINVAL, "%s: workspace of %lld bytes, 16-byte aligned, wanted", fn, (long long)need);
-    const int64_t ps = type_bytes(s->pool_dtype);
-    const uint64_t rec = 2 * uint64_t(s->kv_heads) * uint64_t(s->dim) * uint64_t(ps);
+    const uint64_t rec = 2 * half_bytes(s->kv_heads, s->dim, s->pool_dtype);
     if (rec / 2 >= (uint64_t(1) << 30)) return set_error(KVEC_EUNSUPPORTED, "%s: token record too large", fn);
     {
         auto span = [&](const void* q, int64_t st, int64_t hs, const char* name) {
@@ -185,6 +214,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.v_scale = s->v_scale;
     a.rec = uint32_t(rec);
     a.token_bytes = uint32_t(rec / 2);
+    a.scales = uint32_t(uint64_t(s->kv_heads) * uint64_t(s->dim) * uint64_t(block_bits(s->pool_dtype)) / 8);
     a.tokens = uint32_t(s->tokens);
     a.batch = uint32_t(s->batch);
     a.heads = uint32_t(s->heads);
@@ -207,6 +237,11 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.by_own = make_fastdiv(p.parts_own);
     a.by_heads_flat = make_fastdiv(a.kv_heads * a.by_flat.d);
     a.by_heads_own = make_fastdiv(a.kv_heads * p.parts_own);
+    a.side = p.side;
+    a.run_keys = p.run_keys;
+    a.by_groups = make_fastdiv(p.groups);
+    a.by_run_flat = make_fastdiv(p.parts_flat ? (p.parts_flat + 4 / p.side - 1) / (4 / p.side) : 1);
+    a.by_run_own = make_fastdiv((p.parts_own + 4 / p.side - 1) / (4 / p.side));
     a.direct = p.direct();
     a.scale = s->scale;
     a.wide_q = aligned16(s->q) && s->q_stride % 8 == 0 && s->q_head_stride % 8 == 0;
@@ -216,10 +251,12 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
         a.ws_ml = (f32x2*)((uint8_t*)workspace + uint64_t(p.parts_flat + p.parts_own) * p.rows * uint64_t(s->dim) * 4);
     }
     const bool fp8 = s->pool_dtype == KVEC_FP8_E4M3, bf = s->dtype == KVEC_BF16;
-    AttnFn f = bf ? (fp8 ? pick_attn<__bf16, true>(p.flat_tile, p.own_tile, s->dim)
-                         : pick_attn<__bf16, false>(p.flat_tile, p.own_tile, s->dim))
-                  : (fp8 ? pick_attn<_Float16, true>(p.flat_tile, p.own_tile, s->dim)
-                         : pick_attn<_Float16, false>(p.flat_tile, p.own_tile, s->dim));
+    const int bits = block_bits(s->pool_dtype);
+    AttnFn f = bits ? pick_block_attn(bf, bits, p.flat_tile, p.own_tile, s->dim)
+               : bf ? (fp8 ? pick_attn<__bf16, kFp8>(p.flat_tile, p.own_tile, s->dim)
+                           : pick_attn<__bf16, kPlain>(p.flat_tile, p.own_tile, s->dim))
+                    : (fp8 ? pick_attn<_Float16, kFp8>(p.flat_tile, p.own_tile, s->dim)
+                           : pick_attn<_Float16, kPlain>(p.flat_tile, p.own_tile, s->dim));
     hipLaunchKernelGGL(f, dim3(unsigned(p.blocks)), dim3(kAB), 0, as_stream(stream), a);
     if ((rc = check_launch(fn)) || p.direct()) return rc;
     uint32_t lanes = 16;

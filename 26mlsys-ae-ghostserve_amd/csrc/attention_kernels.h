@@ -34,7 +34,7 @@
 // fp16 one of less than 2^-32, an infinity that is not taken out becomes NaN.)
 #pragma once
 
-#include "lm_types.h"
+#include "block_scale.h"
 #include "paged_geom.h"
 
 namespace kvec {
@@ -60,6 +60,15 @@ constexpr float kFloatMax = 3.402823466e38f;
 // exponents of 32 bits.
 template <class T>
 constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
+
+// What a pool holds: values of the queries' type, e4m3 with one scale for K and one
+// for V, or codes of 8 or 4 bits with block scales (block_scale.h).
+enum Pool { kPlain, kFp8, kBlock8, kBlock4 };
+template <int POOL>
+constexpr bool kBlocks = POOL == kBlock8 || POOL == kBlock4;
+// Bits of a value, for pools that are not plain; bytes of `n` values.
+template <int POOL>
+constexpr int kBits = POOL == kPlain ? 16 : POOL == kBlock4 ? 4 : 8;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -154,6 +163,7 @@ struct AttnArgs {
     float* ws_o;                               // [parts][rows][dim]
     f32x2* ws_ml;                              // [parts][rows]: maximum, sum
     uint32_t rec, token_bytes;                 // bytes of a token record, of its K
+    uint32_t scales;                           // block scales: where those of its K start
     uint32_t tokens, batch, heads, kv_heads, group, dim;
     uint32_t width, shift, pool_pages, cap;    // cap: positions that a table row covers
     uint32_t prefix;                           // keys of the shared part (0: none)
@@ -164,6 +174,10 @@ struct AttnArgs {
     FastDiv by_group, by_req_tiles;            // query heads of a K/V head; stream blocks: row tiles of a request
     FastDiv by_flat, by_own;                   // splits of each part
     FastDiv by_heads_flat, by_heads_own;       // K/V heads times splits
+    // Runs (stream blocks of a pool with block scales): the K/V heads that a block's
+    // waves take side by side (1, 2 or 4), groups of so many, and the fewest keys of a run
+    uint32_t side, run_keys;
+    FastDiv by_groups, by_run_flat, by_run_own;   // groups; blocks of a row tile's runs
     int direct;                                // one part in all: outputs are final
     int wide_q, wide_o;                        // 16-byte rows
     float scale;
@@ -316,6 +330,51 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     return it;
 }
 
+// A wave's run of a pool with block scales: block `id` and its wave.  Blocks go to the
+// eight XCDs in turn, so ids eight apart are one (rows, run) pair's groups of heads.
+__device__ __forceinline__ Item make_run(const AttnArgs& a, uint32_t id, uint32_t wave) {
+    Item it{};
+    it.flat = id < a.blocks_flat;
+    if (!it.flat) id -= a.blocks_flat;
+    const FastDiv by_parts = it.flat ? a.by_flat : a.by_own;      // splits
+    const FastDiv by_run_blocks = it.flat ? a.by_run_flat : a.by_run_own;
+    const uint32_t parts = by_parts.d, apart = 4 / a.side;       // runs that a block takes
+    const uint32_t k = id >> 3, eight = fdiv(k, a.by_groups);
+    it.head = (k - eight * a.by_groups.d) * a.side + (wave & (a.side - 1));
+    const uint32_t pair = eight * 8 + (id & 7);                  // of rows and a block's runs
+    const uint32_t tile = fdiv(pair, by_run_blocks);
+    const uint32_t split = (pair - tile * by_run_blocks.d) * apart + wave / a.side;
+    if (it.head >= a.kv_heads || split >= parts) return it;
+    it.part = it.flat ? split : a.parts_flat + split;
+    uint32_t first = 0, last;
+    if (it.flat) {
+        it.rows = live_tokens(a) * a.group;
+        it.row0 = tile * kStreamRows;
+        it.live = it.row0 < it.rows;
+        last = a.prefix;
+    } else {
+        it.b = fdiv(tile, a.by_req_tiles);
+        if (it.b >= a.batch) return it;
+        it.t0 = first_token(a, it.b);
+        it.rows = rows_of(a, it.b, it.t0);
+        it.row0 = (tile - it.b * a.by_req_tiles.d) * kStreamRows;
+        it.live = it.row0 < it.rows;
+        first = a.first;
+        last = 0;
+        if (it.live) {
+            const uint32_t end_row = min(it.row0 + kStreamRows, it.rows) - 1;
+            last = seen_by(a, it.b, it.t0 + fdiv(end_row, a.by_group));
+        }
+    }
+    // runs of run_keys, or longer where so many do not hold them
+    const uint32_t n = last > first ? last - first : 0u;
+    const uint32_t steps = (n + kStreamKeys - 1) / kStreamKeys;
+    const uint32_t each = max(fdiv(steps + parts - 1, by_parts) * kStreamKeys, it.flat ? 0u : a.run_keys);
+    it.k0 = first + min(uint64_t(split) * each, uint64_t(n));
+    it.k1 = first + min(uint64_t(split + 1) * each, uint64_t(n));
+    return it;
+}
+
 // The page of a key, as the table has it (of the last key past that: its place
 // is looked at before it is used), and its slot, or kNoCell where there is none.
 // In two steps, so that the table's entry can be on its way for a while.
@@ -351,13 +410,53 @@ __device__ __forceinline__ f32x2 settle(float m, float l, bool sees) {
     return f32x2{sees ? top : -INFINITY, sees ? l : 0.0f};
 }
 
-// Four values of a key's V row from value d on, zeros where there are none.
-template <class T, bool FP8>
-__device__ __forceinline__ u32x2 value4(const AttnArgs& a, uint32_t slot, uint32_t head_off, uint32_t d) {
-    const uint8_t* p = chunk_at(a, slot, a.token_bytes + head_off + d * (FP8 ? 1 : 2), d < anew(a.dim));
-    if constexpr (FP8) return fp8_widen(*as_global(reinterpret_cast<const uint32_t*>(p)), (T*)nullptr);
+// Four values of a key's V row (of K/V head `head`) from value d on, zeros where there
+// are none.
+template <class T, int POOL>
+__device__ __forceinline__ u32x2 value4(const AttnArgs& a, uint32_t slot, uint32_t head, uint32_t d) {
+    if constexpr (kBlocks<POOL>) {
+        // (a rare path: offsets worked out anew for each, not held)
+        const uint32_t at = anew(head * a.dim + d);
+        const bool in = d < anew(a.dim);
+        u32x2 x = {0, 0};
+        const uint8_t* p = chunk_at(a, anew(slot), a.token_bytes + at * kBits<POOL> / 8, in);
+        if constexpr (POOL == kBlock8) x.x = *as_global(reinterpret_cast<const uint32_t*>(p));
+        else x.x = *as_global(reinterpret_cast<const uint16_t*>(p));
+        p = chunk_at(a, anew(slot), a.token_bytes + a.scales + at / kScaleBlock, in);
+        const u32x4 w = widen8<kBits<POOL>>(x, scale_of(*as_global(p)), (T*)nullptr);
+        return u32x2{w.x, w.y};
+    }
+    const uint8_t* p = chunk_at(a, slot, a.token_bytes + (head * a.dim + d) * kBits<POOL> / 8, d < anew(a.dim));
+    if constexpr (POOL == kFp8) return fp8_widen(*as_global(reinterpret_cast<const uint32_t*>(p)), (T*)nullptr);
     else return *as_global(reinterpret_cast<const u32x2*>(p));
 }
+
+// Sixteen codes as they lie in memory, and their scale's byte.
+template <int POOL>
+struct Codes16 {
+    u32x4 v;
+    uint32_t scale;
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (POOL == kBlock4) {
+            const u32x2 x = *as_global(reinterpret_cast<const u32x2*>(p));
+            v.x = x.x, v.y = x.y;
+        } else {
+            v = ld16(p);
+        }
+    }
+    // values 8 j .. 8 j + 7
+    template <class T>
+    __device__ __forceinline__ u32x4 widen(int j, T* ty) const {
+        if constexpr (POOL == kFp8) {
+            const u32x2 x0 = fp8_widen(v[2 * j], ty), x1 = fp8_widen(v[2 * j + 1], ty);
+            return u32x4{x0.x, x0.y, x1.x, x1.y};
+        } else if constexpr (POOL == kBlock8) {
+            return widen8<8>(u32x2{v[2 * j], v[2 * j + 1]}, scale_of(scale), ty);
+        } else {
+            return widen8<4>(u32x2{v[j], 0}, scale_of(scale), ty);
+        }
+    }
+};
 
 // Eight values of a query row (zeros past the head's end).
 template <class T>
@@ -470,12 +569,13 @@ __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
-template <class T, bool FP8, int DP>
+template <class T, int POOL, int DP>
 __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uint8_t* k0, uint8_t* k1, uint8_t* k2, uint8_t* k3,
                                           uint8_t* v0, uint8_t* v1, uint8_t* v2, uint8_t* v3) {
     using G = TileGeom<DP>;
+    constexpr bool CODES = POOL != kPlain;                // widened on the way
     constexpr int KS = DP / 16, DB = DP / 32;
-    constexpr int CH = FP8 ? DP / 16 : G::POS;             // chunks of a key that are loaded
+    constexpr int CH = CODES ? DP / 16 : G::POS;             // chunks of a key that are loaded
     constexpr int PER = (kTileKeys * CH + kAB - 1) / kAB;  // of them by a thread
     __shared__ uint32_t odd;                              // V values that are not finite were taken out
     __shared__ uint32_t lows[4];
@@ -484,9 +584,9 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     const uint32_t r = lane & 31, h = lane >> 5;
     T* const ty = nullptr;
     if (tid == 0) odd = 0;
-    if constexpr (FP8) __syncthreads();                   // before a value is taken out
+    if constexpr (CODES) __syncthreads();                   // before a value is taken out
 
-    const uint32_t row_bytes = a.dim * (FP8 ? 1 : 2), head_off = it.head * row_bytes;
+    const uint32_t row_bytes = a.dim * kBits<POOL> / 8, head_off = it.head * row_bytes;
     // V values that are not finite become 0
     auto scrub = [&](u32x4 v) {
         const uint32_t e = exponent_bits(ty);
@@ -503,29 +603,42 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     };
     // A unit's K and V rows on their way; slot: of its key `lane` % 32.  A chunk
     // past the head's end, or of a key that is not there, is read from zeros.
-    u32x4 xk[FP8 ? PER : 1], xv[FP8 ? PER : 1];
+    Codes16<POOL> xk[CODES ? PER : 1], xv[CODES ? PER : 1];
     const uint8_t *from_k[PER], *from_v[PER];
     uint32_t step_k[PER], step_v[PER];                    // bytes a slot
     const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeroCell);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const uint32_t idx = FP8 ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH, pos = idx % CH;
-        const uint32_t ck = (FP8 ? pos : pos ^ G::swz_k(key)) * 16, cv = (FP8 ? pos : pos ^ G::swz_v(key)) * 16;
+    for (int i = 0; i < PER && !kBlocks<POOL>; ++i) {
+        const uint32_t idx = CODES ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH, pos = idx % CH;
+        constexpr uint32_t CB = POOL == kBlock4 ? 8 : 16;         // bytes of a chunk
+        const uint32_t ck = (CODES ? pos : pos ^ G::swz_k(key)) * CB, cv = (CODES ? pos : pos ^ G::swz_v(key)) * CB;
         const bool in = key < uint32_t(kTileKeys);
         step_k[i] = in && ck < row_bytes ? a.rec : 0u;
         step_v[i] = in && cv < row_bytes ? a.rec : 0u;
         from_k[i] = step_k[i] ? a.pool + head_off + ck : zeros;
         from_v[i] = step_v[i] ? a.pool + a.token_bytes + head_off + cv : zeros;
     }
+    // Block scales: the lane's chunk of a key's K (from = 0) or V (token_bytes) and its
+    // scale.
+    auto load_codes = [&](Codes16<POOL>& x, int i, uint32_t slot, uint32_t from) __attribute__((always_inline)) {
+        const uint32_t idx = i * kAB + tid, pos = idx % CH;
+        const bool in = idx / CH < uint32_t(kTileKeys) && pos * 16 < a.dim;
+        x.load(chunk_at(a, slot, from + (it.head * a.dim + pos * 16) * kBits<POOL> / 8, in));
+        x.scale = *as_global(chunk_at(a, slot, from + a.scales + (it.head * a.dim + pos * 16) / kScaleBlock, in));
+    };
     uint32_t sl[PER];                                     // the slots that K was loaded from last
     auto load_k = [&](uint32_t slot, uint8_t* k) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const uint32_t idx = FP8 ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH;
+            const uint32_t idx = CODES ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH;
             sl[i] = uint32_t(__shfl(int(slot), int(key & 31), 64));
+            if constexpr (kBlocks<POOL>) {
+                load_codes(xk[i], i, sl[i], 0);
+                continue;
+            }
             const bool there = sl[i] != kNoCell;
             const uint8_t* p = (there ? from_k[i] : zeros) + uint64_t(there ? sl[i] : 0u) * step_k[i];
-            if constexpr (FP8) xk[i] = ld16(p);
+            if constexpr (CODES) xk[i].load(p);
             else load_to_lds(p, k + (wave * PER + i) * 1024);
         }
     };
@@ -533,24 +646,26 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     auto load_v = [&](uint8_t* v) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
+            if constexpr (kBlocks<POOL>) {
+                load_codes(xv[i], i, sl[i], a.token_bytes);
+                continue;
+            }
             const bool there = sl[i] != kNoCell;
             const uint8_t* p = (there ? from_v[i] : zeros) + uint64_t(there ? sl[i] : 0u) * step_v[i];
-            if constexpr (FP8) xv[i] = ld16(p);
+            if constexpr (CODES) xv[i].load(p);
             else load_to_lds(p, v + (wave * PER + i) * 1024);
         }
     };
-    // fp8: what load() holds in registers, widened into LDS
-    auto put_fp8 = [&](const u32x4* from, bool is_v, uint8_t* to, bool careful) __attribute__((always_inline)) {
+    // codes: what load() holds in registers, widened into LDS
+    auto put_codes = [&](const Codes16<POOL>* from, bool is_v, uint8_t* to, bool careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const uint32_t idx = i * kAB + tid, key = idx / CH, ch = idx % CH;
             if (kTileKeys * CH % kAB && key >= uint32_t(kTileKeys)) break;
             const uint32_t swz = is_v ? G::swz_v(key) : G::swz_k(key);
-            const u32x4 x = from[FP8 ? i : 0];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const u32x2 x0 = fp8_widen(x[2 * j], ty), x1 = fp8_widen(x[2 * j + 1], ty);
-                u32x4 w = {x0.x, x0.y, x1.x, x1.y};
+                u32x4 w = from[CODES ? i : 0].widen(j, ty);
                 if (careful) w = scrub(w);
                 *reinterpret_cast<u32x4*>(to + key * G::ROW + ((ch * 2 + j) ^ swz) * 16) = w;
             }
@@ -583,7 +698,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
         valid0 = uint32_t(__ballot(s0 != kNoCell));
         valid1 = uint32_t(__ballot(s1 != kNoCell));
         valid2 = uint32_t(__ballot(slot2 != kNoCell));
-        if constexpr (!FP8) {
+        if constexpr (!CODES) {
             load_k(s0, k0);
             load_v(v0);
             load_k(s1, k1);
@@ -593,14 +708,14 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             // one unit at a time in registers; the last one's K stays there
             load_k(s0, k0);
             load_v(v0);
-            put_fp8(xk, false, k0, false);
-            put_fp8(xv, true, v0, true);
+            put_codes(xk, false, k0, false);
+            put_codes(xv, true, v0, true);
             load_k(s1, k1);
             load_v(v1);
-            put_fp8(xk, false, k1, false);
-            put_fp8(xv, true, v1, true);
+            put_codes(xk, false, k1, false);
+            put_codes(xv, true, v1, true);
             load_k(slot2, k2);
-            put_fp8(xk, false, k2, false);
+            put_codes(xk, false, k2, false);
         }
     }
 
@@ -744,9 +859,9 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             o[i % DB] = mma32(vf[i], p[i / DB], o[i % DB], ty);
         }
         top = masked(s_next, largest(s_next), base + kTileKeys, valid);
-        if constexpr (FP8) {
-            put_fp8(xk, false, k_to, false);
-            put_fp8(xv, true, v_to, base + 3 * kTileKeys > block_low);
+        if constexpr (CODES) {
+            put_codes(xk, false, k_to, false);
+            put_codes(xv, true, v_to, base + 3 * kTileKeys > block_low);
         }
     };
     // Two steps, with a barrier before them: what either reads has come in the
@@ -756,7 +871,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
                     uint8_t* kd, uint8_t* vd) __attribute__((always_inline)) {
         const uint32_t base = it.k0 + j * kTileKeys;
         meet();
-        if (!FP8 && rarely<DP <= 128>(base + 2 * kTileKeys > block_low)) {
+        if (!CODES && rarely<DP <= 128>(base + 2 * kTileKeys > block_low)) {
             for (uint32_t e = tid; e < uint32_t(G::BYTES) / 16; e += kAB) {
                 const u32x4 x = reinterpret_cast<const u32x4*>(va)[e], y = reinterpret_cast<const u32x4*>(vb)[e];
                 reinterpret_cast<u32x4*>(va)[e] = scrub(x);
@@ -781,16 +896,16 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 
     // V values that were taken out, to the rows that see them
     if (odd) {
-        // from the first pass on that was looked through, two units at a time (fp8:
+        // from the first pass on that was looked through, two units at a time (codes:
         // the first units are looked through before the limits are known)
-        const uint32_t skip = !FP8 && block_low > it.k0 ? (block_low - it.k0) / (2 * kTileKeys) * (2 * kTileKeys) : 0u;
+        const uint32_t skip = !CODES && block_low > it.k0 ? (block_low - it.k0) / (2 * kTileKeys) * (2 * kTileKeys) : 0u;
         for (uint32_t kk = it.k0 + skip; kk < it.k1; ++kk) {
             const uint32_t sl = kk < limit ? key_slot(a, it, kk) : kNoCell;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 x = not_finite(value4<T, FP8>(a, sl, head_off, uint32_t(d * 32 + 8 * i) + 4 * h), ty);
+                    const f32x4 x = not_finite(value4<T, POOL>(a, sl, it.head, uint32_t(d * 32 + 8 * i) + 4 * h), ty);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[d][4 * i + j] += x[j];
                     __builtin_amdgcn_sched_barrier(0);    // a rare path: few registers, not speed
@@ -835,12 +950,13 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 // 7.1); 256 such 400 us, 5.4 TB/s; 64 over an fp8 pool 50 us, 5.4 TB/s.  Four requests
 // behind 512 tokens 8.4 us, most of it the way to the first keys (table, then keys:
 // about 6 us) and the joining of the waves.
-template <class T, bool FP8, int DP>
+template <class T, int POOL, int DP>
 __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, uint8_t* v0, uint8_t* v1, uint8_t* v2,
                                             uint8_t* v3) {
     using G = TileGeom<DP>;                               // V lies as in the tile blocks
+    constexpr bool CODES = POOL != kPlain;                // widened on the way
     constexpr int KS = DP / 32, DB = DP / 16;
-    constexpr int CH = DP / (FP8 ? 16 : 8);
+    constexpr int CH = DP / (CODES ? 16 : 8);
     constexpr int PER = (kStreamKeys * CH + 63) / 64;
     static_assert(kStreamKeys == kTileKeys && G::BYTES >= kStreamRows * DP * 4, "a unit of V, or the rows' results");
     __shared__ float lm[4][kStreamRows], ll[4][kStreamRows];
@@ -850,8 +966,8 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
     T* const ty = nullptr;
     uint8_t* const lv = wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3;
 
-    const uint32_t row_bytes = a.dim * (FP8 ? 1 : 2), head_off = it.head * row_bytes;
-    u32x4 xv[PER];
+    const uint32_t row_bytes = a.dim * kBits<POOL> / 8, head_off = it.head * row_bytes;
+    Codes16<POOL> xv[PER];
     u32x4 xk[2][KS];                                      // fp8: 8 bytes of each
     auto fetch = [&](uint32_t slot) {                     // slot: of the keys lane % 32
         const uint32_t inside = anew(row_bytes);
@@ -861,7 +977,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const uint32_t d = ks * 32 + g * 8;
-                if constexpr (FP8) {
+                if constexpr (POOL == kFp8) {
                     const u32x2 v = *as_global(reinterpret_cast<const u32x2*>(chunk_at(a, s, head_off + d, d < inside)));
                     xk[kb][ks].x = v.x;
                     xk[kb][ks].y = v.y;
@@ -875,7 +991,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
             const uint32_t idx = i * 64 + lane, key = idx / CH, ch = idx % CH;
             const uint32_t s = uint32_t(__shfl(int(slot), int(key & 31), 64));
             const bool in = ch * 16 < inside && key < uint32_t(kStreamKeys);
-            xv[i] = ld16(chunk_at(a, s, a.token_bytes + head_off + ch * 16, in));
+            xv[i].load(chunk_at(a, s, a.token_bytes + head_off + ch * 16, in));
         }
     };
     auto scrub = [&](u32x4& v) {
@@ -939,16 +1055,15 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
             if (kStreamKeys * CH % 64 && key >= uint32_t(kStreamKeys)) break;
             uint8_t* pv = lv + key * G::ROW;
             const uint32_t swz = G::swz_v(key);
-            if constexpr (FP8) {
+            if constexpr (CODES) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const u32x2 v0 = fp8_widen(xv[i][2 * j], ty), v1 = fp8_widen(xv[i][2 * j + 1], ty);
-                    u32x4 v = {v0.x, v0.y, v1.x, v1.y};
+                    u32x4 v = xv[i].widen(j, ty);
                     if (careful) odd |= scrub(v);
                     *reinterpret_cast<u32x4*>(pv + ((ch * 2 + j) ^ swz) * 16) = v;
                 }
             } else {
-                u32x4 v = xv[i];
+                u32x4 v = xv[i].v;
                 if (careful) odd |= scrub(v);
                 *reinterpret_cast<u32x4*>(pv + (ch ^ swz) * 16) = v;
             }
@@ -959,7 +1074,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 u32x4 kf = xk[kb][ks];
-                if constexpr (FP8) {
+                if constexpr (POOL == kFp8) {
                     const u32x2 k0 = fp8_widen(kf.x, ty), k1 = fp8_widen(kf.y, ty);
                     kf = u32x4{k0.x, k0.y, k1.x, k1.y};
                 }
@@ -1023,7 +1138,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
                 const uint32_t sl = key < limit ? key_slot(a, it, key) : kNoCell;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
-                    o[d] += not_finite(value4<T, FP8>(a, sl, head_off, uint32_t(d * 16) + 4 * g), ty);
+                    o[d] += not_finite(value4<T, POOL>(a, sl, it.head, uint32_t(d * 16) + 4 * g), ty);
             }
         }
     }
@@ -1075,10 +1190,271 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
     }
 }
 
+// -------------------------------------------- stream blocks of a pool with block scales
+// 16 rows against a run of keys, as above, but a wave takes one K/V head and the block's
+// waves the heads beside it (or, with fewer than four heads, further runs): a key's
+// codes of one head are 64 or 128 bytes and its scales 4, so that blocks of one head
+// each, on XCDs with L2s of their own, would fetch every line several times over.  Waves
+// work alone to the end, each with a partial result of its own; there is no barrier.
+//
+// A lane holds the same stretch of DP / 4 values of a key for the first product as it
+// loads: that instruction sums over its values in any order, so long as the query's come
+// in the same one.  Codes become 16-bit values with their block's scale in one
+// conversion a pair; V goes through LDS (of the wave's own) to be read transposed.  PF
+// units of 32 keys are on their way at a time.
+template <int DP>
+struct RunGeom {
+    static constexpr int ROW = TileGeom<DP>::ROW;         // bytes of a key's V in LDS
+    // writes: 16 lanes, one chunk of 16 keys each; transposed reads: 32 lanes, two
+    // neighbouring chunks of 8 keys: both on different banks
+    static __device__ __forceinline__ uint32_t swz(uint32_t key) {
+        return DP == 64 ? ((key >> 1) & 3) << 1 | ((key >> 3) & 1) : (key & 7) << 1 | ((key >> 3) & 1);
+    }
+};
+
+// The larger of the two lanes' values 16 apart, in both.
+__device__ __forceinline__ float max_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// N words from an address that is a multiple of 4.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* to) {
+    typedef u32x4 u32x4u __attribute__((aligned(4)));
+    typedef u32x2 u32x2u __attribute__((aligned(4)));
+    constexpr int N4 = N / 4 * 4;
+#pragma unroll
+    for (int i = 0; i < N4; i += 4) {
+        const u32x4 v = *as_global(reinterpret_cast<const u32x4u*>(p + 4 * i));
+        to[i] = v.x, to[i + 1] = v.y, to[i + 2] = v.z, to[i + 3] = v.w;
+    }
+    if constexpr (N % 4 >= 2) {
+        const u32x2 v = *as_global(reinterpret_cast<const u32x2u*>(p + 4 * N4));
+        to[N4] = v.x, to[N4 + 1] = v.y;
+    }
+    if constexpr (N % 2) to[N - 1] = *as_global(reinterpret_cast<const uint32_t*>(p + 4 * (N - 1)));
+}
+
+template <class T, int POOL, int DP>
+__device__ __forceinline__ void attn_run(const AttnArgs& a, const Item& it, uint8_t* lv) {
+    using G = RunGeom<DP>;
+    constexpr int BITS = kBits<POOL>, KS = DP / 32, DB = DP / 16;
+    constexpr int PCS = DP == 256 ? 2 : 1;                // stretches of a lane, each inside the head or not
+    constexpr int PD = DP / 4 / PCS, PW = PD * BITS / 32; // values and words of one
+    constexpr int PF = POOL == kBlock4 && DP <= 128 ? 2 : 1;
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    T* const ty = nullptr;
+
+    // where a lane's stretches lie in a half record; one past the head's end is read
+    // from the head's start (its queries are zeros and its values go nowhere)
+    uint32_t at_code[PCS], at_scale[PCS];
+#pragma unroll
+    for (int p = 0; p < PCS; ++p) {
+        uint32_t d = g * (DP / 4) + p * PD;
+        d = d < a.dim ? d : 0u;
+        at_code[p] = (it.head * a.dim + d) * BITS / 8;
+        at_scale[p] = a.scales + (it.head * a.dim + d) / kScaleBlock;
+    }
+    struct Unit {
+        uint32_t k[2][PCS][PW], v[2][PCS][PW];
+        uint32_t sk[2][PCS], sv[2][PCS];                  // scale bytes; of 96 values the stretch's last in the second byte
+        uint32_t valid;
+    };
+    Unit unit[PF];
+    auto scales = [&](const uint8_t* p) __attribute__((always_inline)) {
+        uint32_t x = *as_global(p);
+        if constexpr (DP == 96) x |= uint32_t(*as_global(p + (g * 24 % 32 + 23) / 32)) << 8;
+        return x;
+    };
+    // keys that are not there are read from the pool's first record
+    auto fetch = [&](Unit& u, uint32_t slot) __attribute__((always_inline)) {   // slot: of the keys lane % 32
+        u.valid = uint32_t(__ballot(slot != kNoCell));
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            uint32_t s = uint32_t(__shfl(int(slot), int(kb * 16 + r), 64));
+            s = s == kNoCell ? 0u : s;
+            const uint8_t* rec = a.pool + uint64_t(s) * a.rec;
+#pragma unroll
+            for (int p = 0; p < PCS; ++p) {
+                load_words<PW>(rec + at_code[p], u.k[kb][p]);
+                u.sk[kb][p] = scales(rec + at_scale[p]);
+            }
+            rec += a.token_bytes;
+#pragma unroll
+            for (int p = 0; p < PCS; ++p) {
+                load_words<PW>(rec + at_code[p], u.v[kb][p]);
+                u.sv[kb][p] = scales(rec + at_scale[p]);
+            }
+        }
+    };
+    // eight values: step s of a lane's
+    auto widen = [&](const uint32_t (&w)[PCS][PW], const uint32_t (&sc)[PCS], int s) __attribute__((always_inline)) {
+        const int p = s / (KS / PCS), i = s % (KS / PCS);
+        uint32_t byte = sc[p];
+        if constexpr (DP == 96) byte = byte >> (g * 24 % 32 + 8 * i < 32 ? 0 : 8) & 255u;
+        return widen8<BITS>(BITS == 8 ? u32x2{w[p][2 * i % PW], w[p][(2 * i + 1) % PW]} : u32x2{w[p][i], 0}, scale_of(byte), ty);
+    };
+
+    const uint32_t units = a.pool_pages && it.k1 > it.k0 ? (it.k1 - it.k0 + kStreamKeys - 1) / kStreamKeys : 0u;
+    const uint32_t key = lane & 31;
+    uint32_t page = 0;                                    // of the lane's key of the unit to be fetched next
+    if (units) {
+#pragma unroll
+        for (int j = 0; j < PF; ++j) fetch(unit[j], key_slot(a, it, it.k0 + j * kStreamKeys + key));
+        page = key_page(a, it, it.k0 + PF * kStreamKeys + key);
+    }
+    // the queries and their limits, while the first keys are on their way
+    const uint32_t row = it.row0 + r;
+    const bool has = row < it.rows;
+    const uint32_t tok = has ? fdiv(row, a.by_group) : 0u;
+    const uint32_t token = it.t0 + tok, head = it.head * a.group + (has ? row - tok * a.group : 0u);
+    // rows that are not there, and rows that see nothing, ask for no mask
+    const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
+    const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
+    // 0 would make NaN of a masked score
+    const float c = fabsf(score_factor(a));
+    u32x4 qf[KS];
+    {
+        const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, g * (DP / 4) + uint32_t(s * 8));
+    }
+    uint32_t low = limit;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
+    low = __builtin_amdgcn_readfirstlane(low);
+
+    bool odd = false;                                     // V values that are not finite were taken out
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
+
+    const uint32_t zw = G::swz(r), zr = G::swz(4 * g + r / 4);
+    auto step = [&](uint32_t n, Unit& u) __attribute__((always_inline)) {
+        const uint32_t base = it.k0 + n * kStreamKeys, valid = u.valid;
+        const bool careful = base + kStreamKeys > low;
+        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[kb] = mma16(widen(u.k[kb], u.sk[kb], ks), qf[ks], s[kb], ty);
+        if (valid != 0xFFFFFFFFu) {
+            // V of keys that are not there: zeros
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const bool there = valid >> (kb * 16 + r) & 1;
+#pragma unroll
+                for (int p = 0; p < PCS; ++p) {
+#pragma unroll
+                    for (int i = 0; i < PW; ++i) u.v[kb][p][i] = there ? u.v[kb][p][i] : 0u;
+                    u.sv[kb][p] = there ? u.sv[kb][p] : 0u;
+                }
+            }
+        }
+        // V to LDS; the reads of the unit before have all been waited for by its
+        // products, and a wave's LDS operations keep their order
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                u32x4 v = widen(u.v[kb], u.sv[kb], ks);
+                if (careful) {
+                    const uint32_t e = exponent_bits(ty);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t w = v[j];
+                        if ((w & e) == e) w &= 0xFFFF0000u, odd = true;
+                        if (((w >> 16) & e) == e) w &= 0x0000FFFFu, odd = true;
+                        v[j] = w;
+                    }
+                }
+                *reinterpret_cast<u32x4*>(lv + (kb * 16 + r) * G::ROW + ((g * KS + ks) ^ zw) * 16) = v;
+            }
+        if (n + PF < units) {
+            fetch(u, page_slot(a, it, base + PF * kStreamKeys + key, page));
+            page = key_page(a, it, base + (PF + 1) * kStreamKeys + key);
+        }
+        // keys: 16 kb + 4 g + i
+        if (valid != 0xFFFFFFFFu || careful) {
+            const uint32_t see = (valid & low_bits(int32_t(min(limit, 0x7FFFFFFFu) - base))) >> (4 * g);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[kb][i] = see & (1u << (kb * 16 + i)) ? s[kb][i] : -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+        top = max_halves(max_quarters(top));
+        if (__any((top - m) * c > kLazy || m == -INFINITY)) {
+            const float to = fmaxf(m, top);
+            const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= f;
+        }
+        const float off = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4] - off, c, kLift<T>));
+        // sum over keys 4 g .. and 16 + 4 g .. : what the lane's scores are of
+        const u32x4 p = {pack2(s[0][0], s[0][1], ty), pack2(s[0][2], s[0][3], ty), pack2(s[1][0], s[1][1], ty),
+                         pack2(s[1][2], s[1][3], ty)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l = add2(uint32_t(p[i]), l, ty);   // the sum is that of the rounded P
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const uint8_t* v = lv + (4 * g + r / 4) * G::ROW + (r & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const uint8_t* vd = v + ((d * 2 + ((r >> 1) & 1)) ^ zr) * 16;
+            const u32x2 x0 = lds_tr(vd), x1 = lds_tr(vd + 16 * G::ROW);
+            o[d] = mma16(u32x4{x0.x, x0.y, x1.x, x1.y}, p, o[d], ty);
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+    for (uint32_t n = 0; n < units; n += PF) {
+#pragma unroll
+        for (int j = 0; j < PF; ++j)
+            if (n + j < units) step(n + j, unit[j]);
+    }
+
+    // V values that were taken out, to the rows that see them
+    if (__any(odd)) {
+        const uint32_t skip = low > it.k0 ? (low - it.k0) / kStreamKeys * kStreamKeys : 0u;
+        for (uint32_t k = it.k0 + skip; k < it.k1; ++k) {
+            const uint32_t sl = k < limit ? key_slot(a, it, k) : kNoCell;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] += not_finite(value4<T, POOL>(a, sl, it.head, uint32_t(d * 16) + 4 * g), ty);
+        }
+    }
+
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const f32x2 ml = settle(m, l, seen != 0);
+    if (!has) return;
+    if (!a.direct && g == 0) {
+        const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(token) * a.heads + head;
+        *as_global(a.ws_ml + at) = ml;
+    }
+    // (a part without keys is not read)
+    if (!a.direct && ml.x == -INFINITY) return;
+    const float inv = ml.y > 0.0f ? 1.0f / ml.y : ml.y == ml.y ? 0.0f : ml.y;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        f32x4 x = o[d];
+        if (ml.y == 0.0f) x = f32x4{0, 0, 0, 0};
+        emit4<T>(a, it, token, head, uint32_t(d * 16) + 4 * g, x, inv);
+    }
+}
+
 // The kernels: FLAT and OWN say what takes the shared part and the own keys (0: no
 // such blocks, 1: stream blocks, 2: tile blocks).  Both parts are one launch: the
 // one is bound by the matrix units, the other by memory.
-template <class T, bool FP8, int DP, int FLAT, int OWN>
+template <class T, int POOL, int DP, int FLAT, int OWN>
 __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a) {
     using G = TileGeom<DP>;
     constexpr bool TILE = FLAT == 2 || OWN == 2;
@@ -1090,10 +1466,14 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a
     const uint32_t id = blockIdx.x;
     if (TILE && (FLAT != 2 || OWN == 2 || id < a.blocks_flat)) {
         const Item it = make_item<false>(a, id);
-        if (it.live) attn_tile<T, FP8, DP>(a, it, k0, k1, k2, k3, v0, v1, v2, v3);
+        if (it.live) attn_tile<T, POOL, DP>(a, it, k0, k1, k2, k3, v0, v1, v2, v3);
+    } else if (OWN == 1 && kBlocks<POOL>) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const Item it = make_run(a, id, wave);
+        if (it.live) attn_run<T, POOL, DP>(a, it, wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3);
     } else if (OWN == 1) {
         const Item it = make_item<true>(a, id);
-        if (it.live) attn_stream<T, FP8, DP>(a, it, v0, v1, v2, v3);
+        if (it.live) attn_stream<T, POOL, DP>(a, it, v0, v1, v2, v3);
     }
 }
 
@@ -1141,16 +1521,19 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
 
 typedef void (*AttnFn)(AttnArgs);
 
-template <class T, bool FP8, int FLAT, int OWN>
+// The kernel for a pool with block scales (attention_blocks.hip).
+AttnFn pick_block_attn(bool bf16, int bits, bool flat_tile, bool own_tile, int dim);
+
+template <class T, int POOL, int FLAT, int OWN>
 AttnFn pick_dim(int dim) {
-    return dim <= 64    ? &attn_kernel<T, FP8, 64, FLAT, OWN>
-           : dim <= 96  ? &attn_kernel<T, FP8, 96, FLAT, OWN>
-           : dim <= 128 ? &attn_kernel<T, FP8, 128, FLAT, OWN>
-                        : &attn_kernel<T, FP8, 256, FLAT, OWN>;
+    return dim <= 64    ? &attn_kernel<T, POOL, 64, FLAT, OWN>
+           : dim <= 96  ? &attn_kernel<T, POOL, 96, FLAT, OWN>
+           : dim <= 128 ? &attn_kernel<T, POOL, 128, FLAT, OWN>
+                        : &attn_kernel<T, POOL, 256, FLAT, OWN>;
 }
-template <class T, bool FP8>
+template <class T, int POOL>
 AttnFn pick_attn(bool flat_tile, bool own_tile, int dim) {
-    return own_tile ? pick_dim<T, FP8, 0, 2>(dim) : flat_tile ? pick_dim<T, FP8, 2, 1>(dim) : pick_dim<T, FP8, 1, 1>(dim);
+    return own_tile ? pick_dim<T, POOL, 0, 2>(dim) : flat_tile ? pick_dim<T, POOL, 2, 1>(dim) : pick_dim<T, POOL, 1, 1>(dim);
 }
 
 }  // namespace kvec

@@ -498,7 +498,8 @@ int kvec_block_read_kv(const kvec_block_read* call, void* stream);
  * on are left as they were.
  * out = softmax(scale * q.k) v by query head, in 32 bits but for the softmax's
  * weights, which are rounded to `dtype` before they multiply v; head h reads K/V head
- * h / (heads / kv_heads).  fp8 K and V stand for value * scale.
+ * h / (heads / kv_heads).  fp8 K and V stand for value * scale, codes with block
+ * scales for their values rounded to `dtype`.
  * max_q: the most tokens that a request has (its tokens past that are left as
  * they were, and change nothing for other requests); the kind of blocks is chosen
  * by it once for the call;
@@ -515,7 +516,7 @@ typedef struct kvec_attention {
     void* out;
     int64_t o_stride, o_head_stride;
     const void* pool;           /* the layer: [pool_pages][page_tokens][2 (K,V)][kv_heads][dim] */
-    int pool_dtype;             /* dtype, or KVEC_FP8_E4M3 */
+    int pool_dtype;             /* dtype, KVEC_FP8_E4M3, or KVEC_BLOCK_*: half records for [kv_heads][dim] */
     int64_t pool_pages;
     int page_tokens;            /* a power of two */
     const int32_t* page_table;  /* device [batch][pages_per_seq] */
