@@ -8,7 +8,8 @@ struct AttnPlan {
     bool flat, flat_tile, own_tile;
     uint32_t parts_flat, parts_own, tiles_flat, req_tiles, first;
     uint64_t rows, tiles_own, blocks_flat, blocks;
-    uint32_t side, groups, run_keys;           // pools with block scales: see AttnArgs
+    // pools with block scales: K/V heads of a wave, groups of a block's, runs, and see AttnArgs
+    uint32_t wave_heads, run_heads, groups, run_keys, runs_flat, runs_own;
     bool direct() const { return parts_flat + parts_own == 1; }
     int64_t bytes(int64_t dim) const {
         return direct() ? 0 : int64_t(uint64_t(parts_flat + parts_own) * rows * (uint64_t(dim) * 4 + 8)) + 16;
@@ -85,31 +86,38 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     p.parts_own = splits(own, len > p.first ? len - p.first : 1, 512);
     p.blocks_flat = p.flat ? uint64_t(p.tiles_flat) * Hk * p.parts_flat : 0;
     p.blocks = p.blocks_flat + own * p.parts_own;
-    p.side = Hk >= 3 ? 4 : uint32_t(Hk);
-    p.groups = uint32_t((Hk + p.side - 1) / p.side);
-    if (block_bits(s->pool_dtype)) {
-        // runs: a wave's, eight pairs of rows and runs on as many XCDs
-        auto run_blocks = [&](uint64_t tiles, uint64_t parts) {
-            const uint64_t apart = 4 / p.side, pairs = tiles * ((parts + apart - 1) / apart);
-            return (pairs + 7) / 8 * 8 * p.groups;
-        };
-        auto runs = [&](uint64_t tiles, uint64_t keys, uint32_t* parts) {
-            // about four waves a SIMD, 128 keys a run, 512 runs of a row
-            uint64_t n = 4096 / (tiles * Hk);
-            if (n > keys / 128) n = keys / 128;
-            n = n < 1 ? 1 : n > 512 ? 512 : n;
-            *parts = uint32_t(n);
+    if (const int bits = block_bits(s->pool_dtype)) {
+        // Runs: waves of two heads where the codes have 4 bits and each head's rows of a
+        // request are no more than eight; blocks of four times as many heads, or as there
+        // are; eight pairs of rows and runs on as many XCDs.
+        p.wave_heads = bits == 4 && Hk >= 2 && req_rows <= kStreamRows / 2 ? 2 : 1;
+        const uint64_t rows = kStreamRows / p.wave_heads, most = 4 * p.wave_heads;
+        p.run_heads = p.wave_heads;
+        while (p.run_heads < most && p.run_heads < Hk) p.run_heads *= 2;
+        p.groups = uint32_t((Hk + p.run_heads - 1) / p.run_heads);
+        const uint64_t subs = most / p.run_heads;         // times 32 keys, each with partial results of its own
+        auto run_blocks = [&](uint64_t tiles, uint64_t runs) { return (tiles * runs + 7) / 8 * 8 * p.groups; };
+        auto runs = [&](uint64_t tiles, uint64_t keys, uint32_t* count) {
+            // about four blocks a compute unit, 64 keys a wave of a run, 512 parts of a row
+            uint64_t n = 1024 / (tiles * p.groups);
+            if (n > keys / (64 * subs)) n = keys / (64 * subs);
+            if (n > 512 / subs) n = 512 / subs;
+            n = n < 1 ? 1 : n;
+            *count = uint32_t(n);
             return uint32_t((keys + n - 1) / n + kStreamKeys - 1) / kStreamKeys * kStreamKeys;
         };
-        uint32_t each = 0;
         if (p.flat && !p.flat_tile) {
-            each = runs(p.tiles_flat, prefix, &p.parts_flat);
-            p.blocks_flat = run_blocks(p.tiles_flat, p.parts_flat);
+            p.tiles_flat = uint32_t((all_rows + rows - 1) / rows);
+            runs(p.tiles_flat, prefix, &p.runs_flat);
+            p.parts_flat = uint32_t(p.runs_flat * subs);
+            p.blocks_flat = run_blocks(p.tiles_flat, p.runs_flat);
         }
         if (!p.own_tile) {
-            each = runs(p.tiles_own, len > p.first ? len - p.first : 1, &p.parts_own);
-            p.run_keys = each;
-            p.blocks = p.blocks_flat + run_blocks(p.tiles_own, p.parts_own);
+            p.req_tiles = uint32_t((req_rows + rows - 1) / rows);
+            p.tiles_own = B * p.req_tiles;
+            p.run_keys = runs(p.tiles_own, len > p.first ? len - p.first : 1, &p.runs_own);
+            p.parts_own = uint32_t(p.runs_own * subs);
+            p.blocks = p.blocks_flat + run_blocks(p.tiles_own, p.runs_own);
         }
     }
     return p;
@@ -237,11 +245,15 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     a.by_own = make_fastdiv(p.parts_own);
     a.by_heads_flat = make_fastdiv(a.kv_heads * a.by_flat.d);
     a.by_heads_own = make_fastdiv(a.kv_heads * p.parts_own);
-    a.side = p.side;
-    a.run_keys = p.run_keys;
-    a.by_groups = make_fastdiv(p.groups);
-    a.by_run_flat = make_fastdiv(p.parts_flat ? (p.parts_flat + 4 / p.side - 1) / (4 / p.side) : 1);
-    a.by_run_own = make_fastdiv((p.parts_own + 4 / p.side - 1) / (4 / p.side));
+    if (p.run_heads) {
+        a.run_heads = p.run_heads;
+        a.run_keys = p.run_keys;
+        a.by_groups = make_fastdiv(p.groups);
+        a.by_tiles_flat = make_fastdiv(p.tiles_flat ? p.tiles_flat : 1);
+        a.by_tiles_own = make_fastdiv(uint32_t(p.tiles_own));
+        a.by_runs_flat = make_fastdiv(p.runs_flat ? p.runs_flat : 1);
+        a.by_runs_own = make_fastdiv(p.runs_own ? p.runs_own : 1);
+    }
     a.direct = p.direct();
     a.scale = s->scale;
     a.wide_q = aligned16(s->q) && s->q_stride % 8 == 0 && s->q_head_stride % 8 == 0;
@@ -252,16 +264,19 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     }
     const bool fp8 = s->pool_dtype == KVEC_FP8_E4M3, bf = s->dtype == KVEC_BF16;
     const int bits = block_bits(s->pool_dtype);
-    AttnFn f = bits ? pick_block_attn(bf, bits, p.flat_tile, p.own_tile, s->dim)
+    AttnFn f = bits ? pick_block_attn(bf, bits, p.flat_tile, p.own_tile, int(p.wave_heads), s->dim)
                : bf ? (fp8 ? pick_attn<__bf16, kFp8>(p.flat_tile, p.own_tile, s->dim)
                            : pick_attn<__bf16, kPlain>(p.flat_tile, p.own_tile, s->dim))
                     : (fp8 ? pick_attn<_Float16, kFp8>(p.flat_tile, p.own_tile, s->dim)
                            : pick_attn<_Float16, kPlain>(p.flat_tile, p.own_tile, s->dim));
     hipLaunchKernelGGL(f, dim3(unsigned(p.blocks)), dim3(kAB), 0, as_stream(stream), a);
     if ((rc = check_launch(fn)) || p.direct()) return rc;
-    uint32_t lanes = 16;
+    uint32_t lanes = 16, cut = 1;
     while (lanes * 4 < a.dim) lanes *= 2;
-    const dim3 grid(unsigned(p.rows));
+    // Runs can be many: a row by several blocks where rows are few and its parts take several passes.
+    // Measured: 32 rows of 128 with 512 parts XX us by one, YY by eight.
+    while (p.run_heads && p.rows * cut < 512 && lanes > 4 && a.parts_flat + a.parts_own > kAB / lanes) lanes /= 2, cut *= 2;
+    const dim3 grid(unsigned(p.rows), cut);
     if (bf) hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, dim3(kAB), 0, as_stream(stream), a, lanes);
     else hipLaunchKernelGGL(attn_join_kernel<_Float16>, grid, dim3(kAB), 0, as_stream(stream), a, lanes);
     return check_launch(fn);

@@ -174,10 +174,10 @@ struct AttnArgs {
     FastDiv by_group, by_req_tiles;            // query heads of a K/V head; stream blocks: row tiles of a request
     FastDiv by_flat, by_own;                   // splits of each part
     FastDiv by_heads_flat, by_heads_own;       // K/V heads times splits
-    // Runs (stream blocks of a pool with block scales): the K/V heads that a block's
-    // waves take side by side (1, 2 or 4), groups of so many, and the fewest keys of a run
-    uint32_t side, run_keys;
-    FastDiv by_groups, by_run_flat, by_run_own;   // groups; blocks of a row tile's runs
+    // Runs (stream blocks of a pool with block scales): the K/V heads of a block, a power
+    // of two; groups of so many; row tiles and runs of each part; the fewest keys of a run
+    uint32_t run_heads, run_keys;
+    FastDiv by_groups, by_tiles_flat, by_tiles_own, by_runs_flat, by_runs_own;
     int direct;                                // one part in all: outputs are final
     int wide_q, wide_o;                        // 16-byte rows
     float scale;
@@ -330,26 +330,34 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     return it;
 }
 
-// A wave's run of a pool with block scales: block `id` and its wave.  Blocks go to the
-// eight XCDs in turn, so ids eight apart are one (rows, run) pair's groups of heads.
-__device__ __forceinline__ Item make_run(const AttnArgs& a, uint32_t id, uint32_t wave) {
+// A block's run of a pool with block scales.  Blocks go to the eight XCDs in turn: ids
+// eight apart are the groups of heads of the same rows and run; then come the same run of
+// the other row tiles, so that the later runs, which only long requests have, come last;
+// and a tile moves on by one with each run, so that its runs, of which it may have many or
+// few, go to different XCDs.
+template <int HW>
+__device__ __forceinline__ Item make_run(const AttnArgs& a, uint32_t id) {
     Item it{};
     it.flat = id < a.blocks_flat;
     if (!it.flat) id -= a.blocks_flat;
-    const FastDiv by_parts = it.flat ? a.by_flat : a.by_own;      // splits
-    const FastDiv by_run_blocks = it.flat ? a.by_run_flat : a.by_run_own;
-    const uint32_t parts = by_parts.d, apart = 4 / a.side;       // runs that a block takes
+    const FastDiv by_runs = it.flat ? a.by_runs_flat : a.by_runs_own;
+    const FastDiv by_tiles = it.flat ? a.by_tiles_flat : a.by_tiles_own;
+    const uint32_t parts = by_runs.d;
     const uint32_t k = id >> 3, eight = fdiv(k, a.by_groups);
-    it.head = (k - eight * a.by_groups.d) * a.side + (wave & (a.side - 1));
-    const uint32_t pair = eight * 8 + (id & 7);                  // of rows and a block's runs
-    const uint32_t tile = fdiv(pair, by_run_blocks);
-    const uint32_t split = (pair - tile * by_run_blocks.d) * apart + wave / a.side;
-    if (it.head >= a.kv_heads || split >= parts) return it;
-    it.part = it.flat ? split : a.parts_flat + split;
+    it.head = (k - eight * a.by_groups.d) * a.run_heads;
+    const uint32_t pair = eight * 8 + (id & 7);                  // of rows and a run
+    const uint32_t split = fdiv(pair, by_tiles);
+    uint32_t tile = pair - split * by_tiles.d;
+    if (by_tiles.d % 2 == 0) {                                   // (an odd number moves by itself)
+        tile += split;
+        tile -= fdiv(tile, by_tiles) * by_tiles.d;
+    }
+    if (split >= parts) return it;
+    it.part = (it.flat ? 0u : a.parts_flat) + split * (4 * HW / a.run_heads);
     uint32_t first = 0, last;
     if (it.flat) {
         it.rows = live_tokens(a) * a.group;
-        it.row0 = tile * kStreamRows;
+        it.row0 = tile * (kStreamRows / HW);
         it.live = it.row0 < it.rows;
         last = a.prefix;
     } else {
@@ -357,19 +365,19 @@ __device__ __forceinline__ Item make_run(const AttnArgs& a, uint32_t id, uint32_
         if (it.b >= a.batch) return it;
         it.t0 = first_token(a, it.b);
         it.rows = rows_of(a, it.b, it.t0);
-        it.row0 = (tile - it.b * a.by_req_tiles.d) * kStreamRows;
+        it.row0 = (tile - it.b * a.by_req_tiles.d) * (kStreamRows / HW);
         it.live = it.row0 < it.rows;
         first = a.first;
         last = 0;
         if (it.live) {
-            const uint32_t end_row = min(it.row0 + kStreamRows, it.rows) - 1;
+            const uint32_t end_row = min(it.row0 + (kStreamRows / HW), it.rows) - 1;
             last = seen_by(a, it.b, it.t0 + fdiv(end_row, a.by_group));
         }
     }
     // runs of run_keys, or longer where so many do not hold them
     const uint32_t n = last > first ? last - first : 0u;
     const uint32_t steps = (n + kStreamKeys - 1) / kStreamKeys;
-    const uint32_t each = max(fdiv(steps + parts - 1, by_parts) * kStreamKeys, it.flat ? 0u : a.run_keys);
+    const uint32_t each = max(fdiv(steps + parts - 1, by_runs) * kStreamKeys, it.flat ? 0u : a.run_keys);
     it.k0 = first + min(uint64_t(split) * each, uint64_t(n));
     it.k1 = first + min(uint64_t(split + 1) * each, uint64_t(n));
     return it;
@@ -1191,26 +1199,47 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 }
 
 // -------------------------------------------- stream blocks of a pool with block scales
-// 16 rows against a run of keys, as above, but a wave takes one K/V head and the block's
-// waves the heads beside it (or, with fewer than four heads, further runs): a key's
-// codes of one head are 64 or 128 bytes and its scales 4, so that blocks of one head
-// each, on XCDs with L2s of their own, would fetch every line several times over.  Waves
-// work alone to the end, each with a partial result of its own; there is no barrier.
+// A few rows against a run of keys, as above, but for HB K/V heads at once (8 of 4 bits,
+// 4 of 8), or, where there are fewer, for so many times 32 keys.  A key's codes of one
+// head are 64 or 128 bytes and its scales 4, half a line and the thirtieth of one: waves
+// that each load their own head's ask for every line of codes two or more times and of
+// scales eight, and it is the lines asked for that are in the way, not their bytes (256
+// requests of up to 4096 keys in 4 bits: the loads alone took 184 us so, 116 as whole
+// stretches).  So the block loads a unit's records of all its heads together, neighbouring
+// lanes neighbouring chunks of 16 bytes, into registers and from there to LDS, while the
+// unit before is worked on.
 //
-// A lane holds the same stretch of DP / 4 values of a key for the first product as it
-// loads: that instruction sums over its values in any order, so long as the query's come
-// in the same one.  Codes become 16-bit values with their block's scale in one
-// conversion a pair; V goes through LDS (of the wave's own) to be read transposed.  PF
-// units of 32 keys are on their way at a time.
-template <int DP>
+// From there on a wave works alone, with partial results of its own: it takes HW of the
+// heads, 16 / HW rows of each.  Each head's scores are a product with all 16 rows, of
+// which a lane keeps its own head's, and each head's part of the output is a product with
+// the other heads' weights taken as 0, so scores, softmax and outputs are one tile.
+// A conversion of two codes takes their scale with it.  V, once in 16 bits, goes through
+// LDS again (of the wave's own) to be read transposed.  The first product sums over a
+// head's values in any order, so long as K and Q come in the same one: a lane takes DP / 4
+// neighbours.
+//
+// A weight of 0 makes NaN of a V that is not finite, so the loop runs a second time where
+// it has given a NaN: with such values taken out, and added to the rows that see them
+// afterwards.
+template <int DP, int BITS>
 struct RunGeom {
-    static constexpr int ROW = TileGeom<DP>::ROW;         // bytes of a key's V in LDS
-    // writes: 16 lanes, one chunk of 16 keys each; transposed reads: 32 lanes, two
-    // neighbouring chunks of 8 keys: both on different banks
-    static __device__ __forceinline__ uint32_t swz(uint32_t key) {
-        return DP == 64 ? ((key >> 1) & 3) << 1 | ((key >> 3) & 1) : (key & 7) << 1 | ((key >> 3) & 1);
+    static constexpr int ROW = TileGeom<DP>::ROW;         // bytes of a key's V in 16 bits
+    static constexpr int CH = DP == 96 ? BITS : DP * BITS / 128;   // chunks of a key's codes (96 values: of 128)
+    static constexpr int KB = kStreamKeys * CH * 16;      // bytes of a head's codes of 32 keys
+    // V in 16 bits: 16 lanes write the same part of 16 / CH keys' chunks, 32 read two
+    // neighbouring chunks of 8 keys: all on different banks
+    static __device__ __forceinline__ uint32_t swz_v(uint32_t key) {
+        if (DP == 64) key >>= 1;
+        return (key & (DP == 64 ? 3 : 7)) << 1 | ((key ^ key >> 1) & 1);
+    }
+    // Codes of head h: 16 lanes write a key's neighbours, of several heads; 16 read one
+    // chunk of 16 keys, or neighbours.
+    static __device__ __forceinline__ uint32_t code_at(uint32_t h, uint32_t key, uint32_t ch) {
+        return ((key ^ (h & 7)) * CH + (ch ^ (key / (16 / CH) & (CH - 1)))) * 16;
     }
 };
+constexpr int kRunScales = 4096;                          // bytes of a block's scales in LDS
+constexpr int kRunKeys = 256;                             // most keys of a block's unit
 
 // The larger of the two lanes' values 16 apart, in both.
 __device__ __forceinline__ float max_quarters(float x) {
@@ -1218,97 +1247,117 @@ __device__ __forceinline__ float max_quarters(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// N words from an address that is a multiple of 4.
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* to) {
-    typedef u32x4 u32x4u __attribute__((aligned(4)));
-    typedef u32x2 u32x2u __attribute__((aligned(4)));
-    constexpr int N4 = N / 4 * 4;
-#pragma unroll
-    for (int i = 0; i < N4; i += 4) {
-        const u32x4 v = *as_global(reinterpret_cast<const u32x4u*>(p + 4 * i));
-        to[i] = v.x, to[i + 1] = v.y, to[i + 2] = v.z, to[i + 3] = v.w;
-    }
-    if constexpr (N % 4 >= 2) {
-        const u32x2 v = *as_global(reinterpret_cast<const u32x2u*>(p + 4 * N4));
-        to[N4] = v.x, to[N4 + 1] = v.y;
-    }
-    if constexpr (N % 2) to[N - 1] = *as_global(reinterpret_cast<const uint32_t*>(p + 4 * (N - 1)));
+// What a wave wrote to LDS, before what its lanes read there from here on.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <class T, int POOL, int DP>
-__device__ __forceinline__ void attn_run(const AttnArgs& a, const Item& it, uint8_t* lv) {
-    using G = RunGeom<DP>;
-    constexpr int BITS = kBits<POOL>, KS = DP / 32, DB = DP / 16;
-    constexpr int PCS = DP == 256 ? 2 : 1;                // stretches of a lane, each inside the head or not
-    constexpr int PD = DP / 4 / PCS, PW = PD * BITS / 32; // values and words of one
-    constexpr int PF = POOL == kBlock4 && DP <= 128 ? 2 : 1;
-    const uint32_t lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+// A barrier of the block for its LDS alone: loads on their way stay on their way.
+__device__ __forceinline__ void meet_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);                   // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// kc, vc: codes of K and V, HB heads' each; lv: a unit of V of the wave's.
+template <class T, int POOL, int DP, int HW>
+__device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc, uint8_t* vc, uint8_t* lv, uint8_t* ls,
+                                         uint32_t* slots) {
+    constexpr int BITS = kBits<POOL>, KS = DP / 32, DB = DP / 16, HB = 4 * HW;
+    using G = RunGeom<DP, BITS>;
+    constexpr int CH = G::CH, KB = G::KB;
+    constexpr int PER = HB * KB / 16 / kAB;               // chunks of K (and of V) that a thread loads
+    constexpr int VALS = 128 / BITS;                      // values of a chunk
+    constexpr int RH = 16 / HW;                           // rows of a head
+    constexpr int SW = (HB * DP + 511) / 512;             // words with scales that a thread loads, of one head or more a block
+    static_assert(HB * KB <= 2 * TileGeom<DP>::BYTES && 2 * HB * DP <= kRunScales, "LDS");
+    typedef uint32_t any_word __attribute__((aligned(1)));
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t r = lane & 15, g = lane >> 4, mine = r / RH;
     T* const ty = nullptr;
 
-    // where a lane's stretches lie in a half record; one past the head's end is read
-    // from the head's start (its queries are zeros and its values go nowhere)
-    uint32_t at_code[PCS], at_scale[PCS];
-#pragma unroll
-    for (int p = 0; p < PCS; ++p) {
-        uint32_t d = g * (DP / 4) + p * PD;
-        d = d < a.dim ? d : 0u;
-        at_code[p] = (it.head * a.dim + d) * BITS / 8;
-        at_scale[p] = a.scales + (it.head * a.dim + d) / kScaleBlock;
-    }
-    struct Unit {
-        uint32_t k[2][PCS][PW], v[2][PCS][PW];
-        uint32_t sk[2][PCS], sv[2][PCS];                  // scale bytes; of 96 values the stretch's last in the second byte
-        uint32_t valid;
+    // The block's heads (a power of two of them, some past the last one) and how many
+    // times 32 keys it takes; the wave's heads and which 32 keys.
+    const uint32_t nh = a.run_heads, lg_nh = __builtin_ctz(nh), subs = HB >> lg_nh, keys = kStreamKeys * subs;
+    const uint32_t live = min(nh, a.kv_heads - it.head);
+    const uint32_t sub = wave >> (lg_nh - (HW == 2 ? 1 : 0)), h0 = (wave * HW) & (nh - 1);
+    it.part += sub;
+    // The thread's chunk of a key's codes, of its heads one after another.
+    const uint32_t head_bytes = a.dim * BITS / 8, per_head = head_bytes / 16, head_scales = a.dim / kScaleBlock;
+    const uint32_t lg_row = lg_nh + __builtin_ctz(CH);    // chunks of a key: nh * CH, and some of no use
+    const uint32_t cc = tid & ((1u << lg_row) - 1), ck = tid >> lg_row, key_step = kAB >> lg_row;
+    const uint32_t lh = cc / per_head, lc = cc - lh * per_head;   // head and chunk
+    const bool use = lh < live;
+    const uint32_t at_code = it.head * head_bytes + (use ? cc * 16 : 0u);
+    // The heads' scales: words from the first on, or the half record's last, with `skip`
+    // bytes before the first.
+    const uint32_t words = (nh * DP + 127) / 128;         // of a key's K
+    const uint32_t first_scale = a.scales + it.head * head_scales;
+    const uint32_t at_scale = min(first_scale, a.token_bytes - 4 * words), skip = first_scale - at_scale;
+    const uint32_t lg_words = 31 - __builtin_clz(words) + (words & (words - 1) ? 1 : 0);
+
+    const uint32_t units = a.pool_pages && it.k1 > it.k0 ? (it.k1 - it.k0 + keys - 1) / keys : 0u;
+    const int32_t* const list = it.flat ? a.prefix_pages : a.table + uint64_t(it.b) * a.width;
+    // the table's entry for the thread's key of a unit (of the last key past that: its
+    // place is looked at before it is used)
+    auto entry = [&](uint32_t base) __attribute__((always_inline)) {
+        return uint32_t(*as_global(list + (min(base + (tid & (keys - 1)), it.k1 - 1) >> a.shift)));
     };
-    Unit unit[PF];
-    auto scales = [&](const uint8_t* p) __attribute__((always_inline)) {
-        uint32_t x = *as_global(p);
-        if constexpr (DP == 96) x |= uint32_t(*as_global(p + (g * 24 % 32 + 23) / 32)) << 8;
-        return x;
+    uint32_t page = 0;
+    auto put_slots = [&](uint32_t base, uint32_t* to) __attribute__((always_inline)) {
+        if (tid < keys) to[tid] = page_slot(a, it, base + tid, page);
     };
-    // keys that are not there are read from the pool's first record
-    auto fetch = [&](Unit& u, uint32_t slot) __attribute__((always_inline)) {   // slot: of the keys lane % 32
-        u.valid = uint32_t(__ballot(slot != kNoCell));
+    u32x4 xk[PER], xv[PER];
+    uint32_t xs[SW];
+    // Keys that are not there are read from the pool's first record.
+    auto ask = [&](const uint32_t* from) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            uint32_t s = uint32_t(__shfl(int(slot), int(kb * 16 + r), 64));
+        for (int i = 0; i < PER; ++i) {
+            uint32_t s = from[i * key_step + ck];
             s = s == kNoCell ? 0u : s;
-            const uint8_t* rec = a.pool + uint64_t(s) * a.rec;
+            const uint8_t* p = a.pool + uint64_t(s) * a.rec + at_code;
+            xk[i] = ld16(p);
+            xv[i] = ld16(p + a.token_bytes);
+        }
 #pragma unroll
-            for (int p = 0; p < PCS; ++p) {
-                load_words<PW>(rec + at_code[p], u.k[kb][p]);
-                u.sk[kb][p] = scales(rec + at_scale[p]);
-            }
-            rec += a.token_bytes;
-#pragma unroll
-            for (int p = 0; p < PCS; ++p) {
-                load_words<PW>(rec + at_code[p], u.v[kb][p]);
-                u.sv[kb][p] = scales(rec + at_scale[p]);
-            }
+        for (int i = 0; i < SW; ++i) {
+            // word w of K (first half) or V of a key; past the last one the last again
+            const uint32_t idx = min(i * kAB + tid, (2 * keys << lg_words) - 1);
+            const uint32_t w = min(idx & ((1u << lg_words) - 1), words - 1), kv = idx >> lg_words;
+            uint32_t s = from[kv & (keys - 1)];
+            s = s == kNoCell ? 0u : s;
+            xs[i] = *as_global(reinterpret_cast<const any_word*>(a.pool + uint64_t(s) * a.rec + (kv >= keys ? a.token_bytes : 0u) + at_scale) + w);
         }
     };
-    // eight values: step s of a lane's
-    auto widen = [&](const uint32_t (&w)[PCS][PW], const uint32_t (&sc)[PCS], int s) __attribute__((always_inline)) {
-        const int p = s / (KS / PCS), i = s % (KS / PCS);
-        uint32_t byte = sc[p];
-        if constexpr (DP == 96) byte = byte >> (g * 24 % 32 + 8 * i < 32 ? 0 : 8) & 255u;
-        return widen8<BITS>(BITS == 8 ? u32x2{w[p][2 * i % PW], w[p][(2 * i + 1) % PW]} : u32x2{w[p][i], 0}, scale_of(byte), ty);
-    };
-
-    const uint32_t units = a.pool_pages && it.k1 > it.k0 ? (it.k1 - it.k0 + kStreamKeys - 1) / kStreamKeys : 0u;
-    const uint32_t key = lane & 31;
-    uint32_t page = 0;                                    // of the lane's key of the unit to be fetched next
-    if (units) {
+    auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < PF; ++j) fetch(unit[j], key_slot(a, it, it.k0 + j * kStreamKeys + key));
-        page = key_page(a, it, it.k0 + PF * kStreamKeys + key);
-    }
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t key = i * key_step + ck, at = (key / kStreamKeys * nh + lh) * KB + G::code_at(lh, key % kStreamKeys, lc);
+            if (use) {
+                *reinterpret_cast<u32x4*>(kc + at) = xk[i];
+                *reinterpret_cast<u32x4*>(vc + at) = xv[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SW; ++i) {
+            const uint32_t idx = i * kAB + tid;
+            if (idx < 2 * keys << lg_words) *reinterpret_cast<uint32_t*>(ls + idx * 4) = xs[i];
+        }
+    };
+    // Eight values of K's codes: step s of a lane's.  DP / 4 neighbours, but for 96
+    // values, where a lane's 24 would not be whole chunks: 8 of each 32.
+    auto value_at = [&](int s) __attribute__((always_inline)) {
+        return DP == 96 ? uint32_t(s * 32) + g * 8 : g * (DP / 4) + uint32_t(s * 8);
+    };
+    if (units) page = entry(it.k0);
     // the queries and their limits, while the first keys are on their way
-    const uint32_t row = it.row0 + r;
-    const bool has = row < it.rows;
+    const uint32_t row = it.row0 + r % RH;
+    const bool has = row < it.rows && h0 + mine < live;
     const uint32_t tok = has ? fdiv(row, a.by_group) : 0u;
-    const uint32_t token = it.t0 + tok, head = it.head * a.group + (has ? row - tok * a.group : 0u);
+    const uint32_t token = it.t0 + tok, head = (it.head + h0 + mine) * a.group + (has ? row - tok * a.group : 0u);
     // rows that are not there, and rows that see nothing, ask for no mask
     const uint32_t seen = has ? seen_by(a, it.flat ? request_of(a, token) : it.b, token) : 0u;
     const uint32_t limit = seen ? seen : 0xFFFFFFFFu;
@@ -1318,66 +1367,75 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, const Item& it, uint
     {
         const T* p = has ? reinterpret_cast<const T*>(a.q) + int64_t(token) * a.qs + int64_t(head) * a.qh : nullptr;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, g * (DP / 4) + uint32_t(s * 8));
+        for (int s = 0; s < KS; ++s) qf[s] = load_q(a, p, value_at(s));
     }
     uint32_t low = limit;
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) low = min(low, uint32_t(__shfl_xor(int(low), d, 64)));
     low = __builtin_amdgcn_readfirstlane(low);
 
-    bool odd = false;                                     // V values that are not finite were taken out
-    float m = -INFINITY, l = 0.0f;
+    float m, l;
     f32x4 o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
-
-    const uint32_t zw = G::swz(r), zr = G::swz(4 * g + r / 4);
-    auto step = [&](uint32_t n, Unit& u) __attribute__((always_inline)) {
-        const uint32_t base = it.k0 + n * kStreamKeys, valid = u.valid;
-        const bool careful = base + kStreamKeys > low;
+    bool odd = false;                                     // V values that are not finite were taken out
+    const uint32_t zr = G::swz_v(4 * g + r / 4);
+    // a head of the wave's past the last one: the last one's codes (its rows are not there)
+    auto head_of = [&](int h) __attribute__((always_inline)) { return min(h0 + uint32_t(h), live - 1); };
+    auto scale_at = [&](uint32_t key, uint32_t h, uint32_t block) __attribute__((always_inline)) {
+        return scale_of(ls[(key << lg_words) * 4 + skip + h * head_scales + block]);
+    };
+    auto step = [&](uint32_t base, const uint32_t* now, bool safe) __attribute__((always_inline)) {
+        const uint32_t valid = uint32_t(__ballot(now[sub * kStreamKeys + (lane & 31)] != kNoCell));
         f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) s[kb] = mma16(widen(u.k[kb], u.sk[kb], ks), qf[ks], s[kb], ty);
-        if (valid != 0xFFFFFFFFu) {
-            // V of keys that are not there: zeros
+        for (int h = 0; h < HW; ++h) {
+            const uint32_t hh = head_of(h);
+            const uint8_t* codes = kc + (sub * nh + hh) * KB;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const bool there = valid >> (kb * 16 + r) & 1;
+                const uint32_t key = kb * 16 + r;
+                u32x2 x[KS];                              // codes of eight values
+                // steps that a read brings
+                constexpr int STEPS = DP == 96 ? 1 : VALS / 8 < KS ? VALS / 8 : KS;
 #pragma unroll
-                for (int p = 0; p < PCS; ++p) {
-#pragma unroll
-                    for (int i = 0; i < PW; ++i) u.v[kb][p][i] = there ? u.v[kb][p][i] : 0u;
-                    u.sv[kb][p] = there ? u.sv[kb][p] : 0u;
-                }
-            }
-        }
-        // V to LDS; the reads of the unit before have all been waited for by its
-        // products, and a wave's LDS operations keep their order
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                u32x4 v = widen(u.v[kb], u.sv[kb], ks);
-                if (careful) {
-                    const uint32_t e = exponent_bits(ty);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t w = v[j];
-                        if ((w & e) == e) w &= 0xFFFF0000u, odd = true;
-                        if (((w >> 16) & e) == e) w &= 0x0000FFFFu, odd = true;
-                        v[j] = w;
+                for (int ks = 0; ks < KS; ks += STEPS) {
+                    // (past the head's end: what was there; the queries are zeros)
+                    const uint32_t d0 = value_at(ks), d = d0 < a.dim ? d0 : d0 % VALS;
+                    const uint8_t* p = codes + G::code_at(hh, key, d / VALS) + d % VALS * BITS / 8;
+                    constexpr int WORDS = STEPS * BITS / 4;
+                    uint32_t c4[4];
+                    if constexpr (WORDS == 4) {
+                        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+                        c4[0] = v.x, c4[1] = v.y, c4[2] = v.z, c4[3] = v.w;
+                    } else if constexpr (WORDS == 2) {
+                        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+                        c4[0] = v.x, c4[1] = v.y;
+                    } else {
+                        c4[0] = *reinterpret_cast<const uint32_t*>(p);
                     }
+#pragma unroll
+                    for (int j = 0; j < STEPS; ++j)
+                        x[ks + j] = BITS == 8 ? u32x2{c4[2 * j % 4], c4[(2 * j + 1) % 4]} : u32x2{c4[j % 4], 0};
                 }
-                *reinterpret_cast<u32x4*>(lv + (kb * 16 + r) * G::ROW + ((g * KS + ks) ^ zw) * 16) = v;
+                f32x4 y = f32x4{0, 0, 0, 0};
+                float scale = 1.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t d = value_at(ks);
+                    // a lane's values have one scale, or one every 32
+                    if (ks == 0 || DP == 96 || (DP == 256 && ks % 4 == 0))
+                        scale = scale_at(sub * kStreamKeys + key, hh, d < a.dim ? d / kScaleBlock : 0u);
+                    y = mma16(widen8<BITS>(x[ks], scale, ty), qf[ks], y, ty);
+                }
+                if (HW == 1) {
+                    s[kb] = y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[kb][i] = mine == uint32_t(h) ? y[i] : s[kb][i];
+                }
             }
-        if (n + PF < units) {
-            fetch(u, page_slot(a, it, base + PF * kStreamKeys + key, page));
-            page = key_page(a, it, base + (PF + 1) * kStreamKeys + key);
         }
         // keys: 16 kb + 4 g + i
-        if (valid != 0xFFFFFFFFu || careful) {
+        if (rarely<true>(valid != 0xFFFFFFFFu || base + kStreamKeys > low)) {
             const uint32_t see = (valid & low_bits(int32_t(min(limit, 0x7FFFFFFFu) - base))) >> (4 * g);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
@@ -1388,7 +1446,7 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, const Item& it, uint
 #pragma unroll
         for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
         top = max_halves(max_quarters(top));
-        if (__any((top - m) * c > kLazy || m == -INFINITY)) {
+        if (rarely<true>(__any((top - m) * c > kLazy || m == -INFINITY))) {
             const float to = fmaxf(m, top);
             const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
             m = to;
@@ -1404,31 +1462,110 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, const Item& it, uint
                          pack2(s[1][2], s[1][3], ty)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) l = add2(uint32_t(p[i]), l, ty);   // the sum is that of the rounded P
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+
+        // V in 16 bits; of keys that are not there: zeros.  (Reads of the unit before have
+        // been waited for by its products, and a wave's LDS operations keep their order.)
+        auto put_v = [&](uint32_t hh, bool scrub) __attribute__((always_inline)) {
+            const uint8_t* codes = vc + (sub * nh + hh) * KB;
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) {
+                const uint32_t idx = i * 64 + lane, key = idx / CH, ch0 = idx % CH, ch = ch0 * VALS < a.dim ? ch0 : 0u;
+                float scale = scale_at(keys + sub * kStreamKeys + key, hh, ch * VALS / kScaleBlock);
+                u32x4 x = *reinterpret_cast<const u32x4*>(codes + G::code_at(hh, key, ch));
+                if (scrub) {
+                    const bool there = valid >> key & 1;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = there ? x[j] : 0u;
+                    scale = there ? scale : 1.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < VALS / 8; ++j) {
+                    u32x4 v = widen8<BITS>(BITS == 8 ? u32x2{x[2 * j % 4], x[(2 * j + 1) % 4]} : u32x2{x[j], 0}, scale, ty);
+                    if (scrub && safe) {
+                        const uint32_t e = exponent_bits(ty);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t y = v[k];
+                            if ((y & e) == e) y &= 0xFFFF0000u, odd = true;
+                            if (((y >> 16) & e) == e) y &= 0x0000FFFFu, odd = true;
+                            v[k] = y;
+                        }
+                    }
+                    *reinterpret_cast<u32x4*>(lv + key * G::ROW + ((ch0 * (VALS / 8) + j) ^ G::swz_v(key)) * 16) = v;
+                }
+            }
+        };
         const uint8_t* v = lv + (4 * g + r / 4) * G::ROW + (r & 1) * 8;
+        const bool scrub = safe || valid != 0xFFFFFFFFu;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            const uint8_t* vd = v + ((d * 2 + ((r >> 1) & 1)) ^ zr) * 16;
-            const u32x2 x0 = lds_tr(vd), x1 = lds_tr(vd + 16 * G::ROW);
-            o[d] = mma16(u32x4{x0.x, x0.y, x1.x, x1.y}, p, o[d], ty);
+        for (int h = 0; h < HW; ++h) {
+            if (rarely<true>(scrub)) put_v(head_of(h), true);
+            else put_v(head_of(h), false);
+            u32x4 ph = p;
+            if (HW > 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ph[i] = mine == uint32_t(h) ? p[i] : 0u;
+            }
+            wave_order();
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const uint8_t* vd = v + ((d * 2 + ((r >> 1) & 1)) ^ zr) * 16;
+                const u32x2 x0 = lds_tr(vd), x1 = lds_tr(vd + 16 * G::ROW);
+                o[d] = mma16(u32x4{x0.x, x0.y, x1.x, x1.y}, ph, o[d], ty);
+            }
+            wave_order();
         }
-        __builtin_amdgcn_wave_barrier();
     };
-    for (uint32_t n = 0; n < units; n += PF) {
+    // All waves go through the loop together; a wave that has given a NaN has all go again.
+    for (int pass = 0; pass < 2; ++pass) {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < PF; ++j)
-            if (n + j < units) step(n + j, unit[j]);
+        for (int d = 0; d < DB; ++d) o[d] = f32x4{0, 0, 0, 0};
+        if (!units) break;
+        if (pass) page = entry(it.k0);
+        put_slots(it.k0, slots);
+        page = entry(it.k0 + keys);
+        meet_lds();
+        ask(slots);
+        for (uint32_t n = 0; n < units; ++n) {
+            const uint32_t base = it.k0 + n * keys;
+            uint32_t* const now = slots + (n & 1) * kRunKeys;
+            uint32_t* const next = slots + (~n & 1) * kRunKeys;
+            put();
+            put_slots(base + keys, next);
+            page = entry(base + 2 * keys);
+            meet_lds();
+            // (behind the last unit too: a load that may not be there would be waited for as
+            // if none were behind it)
+            ask(next);
+            step(base + sub * kStreamKeys, now, pass);
+            meet_lds();
+        }
+        bool nan = false;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan |= o[d][i] != o[d][i];
+        // (the codes' LDS: every wave is past its last use)
+        if (tid == 0) *reinterpret_cast<uint32_t*>(kc) = 0;
+        meet_lds();
+        if (nan) *reinterpret_cast<uint32_t*>(kc) = 1;
+        meet_lds();
+        const bool again = *reinterpret_cast<volatile uint32_t*>(kc) != 0;
+        meet_lds();
+        if (!again) break;
     }
 
     // V values that were taken out, to the rows that see them
     if (__any(odd)) {
-        const uint32_t skip = low > it.k0 ? (low - it.k0) / kStreamKeys * kStreamKeys : 0u;
-        for (uint32_t k = it.k0 + skip; k < it.k1; ++k) {
-            const uint32_t sl = k < limit ? key_slot(a, it, k) : kNoCell;
+        for (uint32_t n = 0; n < units; ++n) {
+            const uint32_t base = it.k0 + n * keys + sub * kStreamKeys;
+            for (uint32_t k = base; k < min(base + kStreamKeys, it.k1); ++k) {
+                const uint32_t sl = has && k < limit ? key_slot(a, it, k) : kNoCell;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] += not_finite(value4<T, POOL>(a, sl, it.head, uint32_t(d * 16) + 4 * g), ty);
+                for (int d = 0; d < DB; ++d) o[d] += not_finite(value4<T, POOL>(a, sl, it.head + h0 + mine, uint32_t(d * 16) + 4 * g), ty);
+            }
         }
     }
 
@@ -1436,41 +1573,50 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, const Item& it, uint
     l += __shfl_xor(l, 32, 64);
     const f32x2 ml = settle(m, l, seen != 0);
     if (!has) return;
-    if (!a.direct && g == 0) {
-        const uint64_t at = uint64_t(it.part) * a.tokens * a.heads + uint64_t(token) * a.heads + head;
-        *as_global(a.ws_ml + at) = ml;
+    LateArgs& e = late_args();
+    if (!e.direct && g == 0) {
+        const uint64_t at_row = uint64_t(it.part) * e.tokens * e.heads + uint64_t(token) * e.heads + head;
+        *as_global(e.ws_ml + at_row) = ml;
     }
     // (a part without keys is not read)
-    if (!a.direct && ml.x == -INFINITY) return;
+    if (!e.direct && ml.x == -INFINITY) return;
     const float inv = ml.y > 0.0f ? 1.0f / ml.y : ml.y == ml.y ? 0.0f : ml.y;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
         f32x4 x = o[d];
         if (ml.y == 0.0f) x = f32x4{0, 0, 0, 0};
-        emit4<T>(a, it, token, head, uint32_t(d * 16) + 4 * g, x, inv);
+        emit4<T>(e, it, token, head, uint32_t(d * 16) + 4 * g, x, inv);
     }
 }
 
 // The kernels: FLAT and OWN say what takes the shared part and the own keys (0: no
 // such blocks, 1: stream blocks, 2: tile blocks).  Both parts are one launch: the
 // one is bound by the matrix units, the other by memory.
-template <class T, int POOL, int DP, int FLAT, int OWN>
+template <class T, int POOL, int DP, int FLAT, int OWN, int HW = 1>
 __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a) {
     using G = TileGeom<DP>;
     constexpr bool TILE = FLAT == 2 || OWN == 2;
+    constexpr bool RUN = OWN == 1 && kBlocks<POOL>;
     // separate arrays: the compiler can tell their accesses apart, so a read of
     // one does not wait for a load into another
-    __shared__ __attribute__((aligned(16))) uint8_t k0[TILE ? G::BYTES : 16], k1[TILE ? G::BYTES : 16];
-    __shared__ __attribute__((aligned(16))) uint8_t k2[TILE ? G::BYTES : 16], k3[TILE ? G::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t k0[TILE && !RUN ? G::BYTES : 16], k1[TILE && !RUN ? G::BYTES : 16];
+    __shared__ __attribute__((aligned(16))) uint8_t k2[TILE && !RUN ? G::BYTES : 16], k3[TILE && !RUN ? G::BYTES : 16];
     __shared__ __attribute__((aligned(16))) uint8_t v0[G::BYTES], v1[G::BYTES], v2[G::BYTES], v3[G::BYTES];
+    // runs: codes (the tile blocks' K beside them), scales, and slots of two units
+    __shared__ __attribute__((aligned(16))) uint8_t kc[RUN ? 4 * G::BYTES : 16], ls[RUN ? kRunScales : 16];
+    __shared__ uint32_t slots[RUN ? 2 * kRunKeys : 1];
     const uint32_t id = blockIdx.x;
     if (TILE && (FLAT != 2 || OWN == 2 || id < a.blocks_flat)) {
         const Item it = make_item<false>(a, id);
-        if (it.live) attn_tile<T, POOL, DP>(a, it, k0, k1, k2, k3, v0, v1, v2, v3);
-    } else if (OWN == 1 && kBlocks<POOL>) {
+        if (it.live) {
+            if constexpr (RUN) attn_tile<T, POOL, DP>(a, it, kc, kc + G::BYTES, kc + 2 * G::BYTES, kc + 3 * G::BYTES, v0, v1, v2, v3);
+            else attn_tile<T, POOL, DP>(a, it, k0, k1, k2, k3, v0, v1, v2, v3);
+        }
+    } else if constexpr (RUN) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const Item it = make_run(a, id, wave);
-        if (it.live) attn_run<T, POOL, DP>(a, it, wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3);
+        const Item it = make_run<HW>(a, id);
+        if (it.live)
+            attn_run<T, POOL, DP, HW>(a, it, kc, kc + 2 * G::BYTES, wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3, ls, slots);
     } else if (OWN == 1) {
         const Item it = make_item<true>(a, id);
         if (it.live) attn_stream<T, POOL, DP>(a, it, v0, v1, v2, v3);
@@ -1478,8 +1624,8 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a
 }
 
 // Partial results of a row brought to one maximum, summed, divided and rounded.
-// A block takes one row: `lanes` threads a part, the parts shared out to the
-// others, so that a row's parts are read side by side.  Measured: 2048 rows of 128
+// A block takes one row, or 4 * lanes values of it: `lanes` threads a part, the parts
+// shared out to the others, so that a row's parts are read side by side.  Measured: 2048 rows of 128
 // with 12 parts 6.0 us (6.5 where the row's request is looked for), 8192 rows with 7
 // parts 12.7, 128 rows with 5 parts 3.8.
 template <class T>
@@ -1488,7 +1634,7 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
     __shared__ float ll[kAB];
     const uint32_t tid = threadIdx.x, rows = a.tokens * a.heads, row = blockIdx.x;
     if (row / a.heads >= live_tokens(a) || row / a.heads < first_token(a, 0) || !computed(a, row / a.heads)) return;
-    const uint32_t each = kAB / lanes, mine = tid / lanes, d = tid % lanes * 4;
+    const uint32_t each = kAB / lanes, mine = tid / lanes, d = (blockIdx.y * lanes + tid % lanes) * 4;
     const uint32_t parts = a.parts_flat + a.parts_own;
     float top = -INFINITY, l = 0.0f;
     const float c = fabsf(score_factor(a));
@@ -1521,8 +1667,9 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
 
 typedef void (*AttnFn)(AttnArgs);
 
-// The kernel for a pool with block scales (attention_blocks.hip).
-AttnFn pick_block_attn(bool bf16, int bits, bool flat_tile, bool own_tile, int dim);
+// Pools with block scales (attention_blocks.hip): the kernel whose waves take `heads`
+// K/V heads in stream blocks, one, or of 4 bits one or two.
+AttnFn pick_block_attn(bool bf16, int bits, bool flat_tile, bool own_tile, int heads, int dim);
 
 template <class T, int POOL, int FLAT, int OWN>
 AttnFn pick_dim(int dim) {
