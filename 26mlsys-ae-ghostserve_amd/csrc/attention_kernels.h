@@ -1226,18 +1226,44 @@ struct RunGeom {
     static constexpr int ROW = TileGeom<DP>::ROW;         // bytes of a key's V in 16 bits
     static constexpr int CH = DP == 96 ? BITS : DP * BITS / 128;   // chunks of a key's codes (96 values: of 128)
     static constexpr int KB = kStreamKeys * CH * 16;      // bytes of a head's codes of 32 keys
-    // V in 16 bits: 16 lanes write the same part of 16 / CH keys' chunks, 32 read two
-    // neighbouring chunks of 8 keys: all on different banks
-    static __device__ __forceinline__ uint32_t swz_v(uint32_t key) {
-        if (DP == 64) key >>= 1;
-        return (key & (DP == 64 ? 3 : 7)) << 1 | ((key ^ key >> 1) & 1);
+    // LDS takes a load or store of 16 bytes a lane as two of 8, each at half the rate where
+    // the lanes lie 16 bytes apart (1 KB: 13.5 ns; as two of 8 bytes that 32 lanes spread over
+    // all banks, 6.9).  So all go by pieces of 8 bytes, and where a key's pieces lie depends
+    // on the bits of its number, and for codes of the head's, such that 32 lanes always
+    // meet 32 different places of 256 bytes.
+    //
+    // V in 16 bits, 4 values a piece: piece p of a key lies at p ^ v_bits.  Written are one
+    // piece of each of 32 / CH keys' chunks, read (transposed) four neighbours of 8 keys.
+    static __device__ __forceinline__ uint32_t v_bits(uint32_t key) {
+        const uint32_t k0 = key & 1, k1 = key >> 1 & 1, k2 = key >> 2 & 1, k3 = key >> 3 & 1;
+        return DP == 64 ? k1 | k2 << 1 | (k3 ^ k1) << 2 | k2 << 3 : k0 | k1 << 1 | k2 << 2 | k1 << 3 | k0 << 4;
     }
-    // Codes of head h: 16 lanes write a key's neighbours, of several heads; 16 read one
-    // chunk of 16 keys, or neighbours.
-    static __device__ __forceinline__ uint32_t code_at(uint32_t h, uint32_t key, uint32_t ch) {
-        return ((key ^ (h & 7)) * CH + (ch ^ (key / (16 / CH) & (CH - 1)))) * 16;
+    static __device__ __forceinline__ uint32_t v_at(uint32_t key, uint32_t p) {
+        // (a row of 512 bytes: its halves meet)
+        return key * ROW + ((p ^ v_bits(key)) ^ (ROW == 512 ? p / 32 * 6 : 0)) * 8;
+    }
+    // Codes: chunk ch of key `key` of head h lies at code_at ^ ch * 16, its second half at
+    // ^ 8.  Written are half chunks of one or two keys, of several heads; read are, of one
+    // head, half a chunk of 16 keys (or of two neighbours in it), and of neighbours.
+    static __device__ __forceinline__ uint32_t code_at(uint32_t h, uint32_t key) {
+        const uint32_t k0 = key & 1, k1 = key >> 1 & 1, k2 = key >> 2 & 1, k3 = key >> 3 & 1;
+        const uint32_t h0 = h & 1, h1 = h >> 1 & 1, h2 = h >> 2 & 1;
+        uint32_t row = 0, q = 0;
+        if (CH == 2) row = h1 << 1 | h2 << 2, q = k3 * 3;
+        else if (CH == 4) row = h1 << 1 | h2, q = (k2 ^ k3) | k2 << 2;
+        else if (CH == 8) row = h1, q = k1 | k2 << 1 | k3 << 3;
+        else q = k0 | k1 << 1 | k2 << 2 | k3 << 4;
+        return (key ^ row) * (CH * 16) + (q ^ h0) * 8;
     }
 };
+__device__ __forceinline__ void put_halves(uint8_t* base, uint32_t at, u32x4 v) {
+    *reinterpret_cast<u32x2*>(base + at) = u32x2{v.x, v.y};
+    *reinterpret_cast<u32x2*>(base + (at ^ 8)) = u32x2{v.z, v.w};
+}
+__device__ __forceinline__ u32x4 get_halves(const uint8_t* base, uint32_t at) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(base + at), y = *reinterpret_cast<const u32x2*>(base + (at ^ 8));
+    return u32x4{x.x, x.y, y.x, y.y};
+}
 constexpr int kRunScales = 4096;                          // bytes of a block's scales in LDS
 constexpr int kRunKeys = 256;                             // most keys of a block's unit
 
@@ -1335,10 +1361,11 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
     auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const uint32_t key = i * key_step + ck, at = (key / kStreamKeys * nh + lh) * KB + G::code_at(lh, key % kStreamKeys, lc);
+            const uint32_t key = i * key_step + ck;
+            const uint32_t at = (key / kStreamKeys * nh + lh) * KB + (G::code_at(lh, key % kStreamKeys) ^ lc * 16);
             if (use) {
-                *reinterpret_cast<u32x4*>(kc + at) = xk[i];
-                *reinterpret_cast<u32x4*>(vc + at) = xv[i];
+                put_halves(kc, at, xk[i]);
+                put_halves(vc, at, xv[i]);
             }
         }
 #pragma unroll
@@ -1377,7 +1404,6 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
     float m, l;
     f32x4 o[DB];
     bool odd = false;                                     // V values that are not finite were taken out
-    const uint32_t zr = G::swz_v(4 * g + r / 4);
     // a head of the wave's past the last one: the last one's codes (its rows are not there)
     auto head_of = [&](int h) __attribute__((always_inline)) { return min(h0 + uint32_t(h), live - 1); };
     auto scale_at = [&](uint32_t key, uint32_t h, uint32_t block) __attribute__((always_inline)) {
@@ -1394,27 +1420,21 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
             for (int kb = 0; kb < 2; ++kb) {
                 const uint32_t key = kb * 16 + r;
                 u32x2 x[KS];                              // codes of eight values
-                // steps that a read brings
-                constexpr int STEPS = DP == 96 ? 1 : VALS / 8 < KS ? VALS / 8 : KS;
+                const uint32_t at = G::code_at(hh, key);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks += STEPS) {
-                    // (past the head's end: what was there; the queries are zeros)
+                for (int ks = 0; ks < KS; ++ks) {
+                    // (past the head's end: what is there; the queries are zeros)
                     const uint32_t d0 = value_at(ks), d = d0 < a.dim ? d0 : d0 % VALS;
-                    const uint8_t* p = codes + G::code_at(hh, key, d / VALS) + d % VALS * BITS / 8;
-                    constexpr int WORDS = STEPS * BITS / 4;
-                    uint32_t c4[4];
-                    if constexpr (WORDS == 4) {
-                        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
-                        c4[0] = v.x, c4[1] = v.y, c4[2] = v.z, c4[3] = v.w;
-                    } else if constexpr (WORDS == 2) {
+                    const uint8_t* p = codes + (at ^ d / VALS * 16 ^ d % VALS / (VALS / 2) * 8);
+                    if constexpr (BITS == 8) {
+                        x[ks] = *reinterpret_cast<const u32x2*>(p);
+                    } else if constexpr (DP == 96) {
+                        x[ks] = u32x2{*reinterpret_cast<const uint32_t*>(p + d / 8 % 2 * 4), 0};
+                    } else if (ks % 2 == 0) {             // two steps' codes
                         const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-                        c4[0] = v.x, c4[1] = v.y;
-                    } else {
-                        c4[0] = *reinterpret_cast<const uint32_t*>(p);
+                        x[ks] = u32x2{v.x, 0};
+                        x[ks + 1] = u32x2{v.y, 0};
                     }
-#pragma unroll
-                    for (int j = 0; j < STEPS; ++j)
-                        x[ks + j] = BITS == 8 ? u32x2{c4[2 * j % 4], c4[(2 * j + 1) % 4]} : u32x2{c4[j % 4], 0};
                 }
                 f32x4 y = f32x4{0, 0, 0, 0};
                 float scale = 1.0f;
@@ -1471,7 +1491,7 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
             for (int i = 0; i < CH / 2; ++i) {
                 const uint32_t idx = i * 64 + lane, key = idx / CH, ch0 = idx % CH, ch = ch0 * VALS < a.dim ? ch0 : 0u;
                 float scale = scale_at(keys + sub * kStreamKeys + key, hh, ch * VALS / kScaleBlock);
-                u32x4 x = *reinterpret_cast<const u32x4*>(codes + G::code_at(hh, key, ch));
+                u32x4 x = get_halves(codes, G::code_at(hh, key) ^ ch * 16);
                 if (scrub) {
                     const bool there = valid >> key & 1;
 #pragma unroll
@@ -1491,11 +1511,11 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
                             v[k] = y;
                         }
                     }
-                    *reinterpret_cast<u32x4*>(lv + key * G::ROW + ((ch0 * (VALS / 8) + j) ^ G::swz_v(key)) * 16) = v;
+                    put_halves(lv, G::v_at(key, ch0 * (VALS / 4)) ^ j * 16, v);
                 }
             }
         };
-        const uint8_t* v = lv + (4 * g + r / 4) * G::ROW + (r & 1) * 8;
+        const uint32_t v = G::v_at(4 * g + r / 4, r & 3);
         const bool scrub = safe || valid != 0xFFFFFFFFu;
 #pragma unroll
         for (int h = 0; h < HW; ++h) {
@@ -1509,7 +1529,7 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
             wave_order();
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const uint8_t* vd = v + ((d * 2 + ((r >> 1) & 1)) ^ zr) * 16;
+                const uint8_t* vd = lv + (v ^ (d * 32 ^ (G::ROW == 512 ? d / 8 * 48 : 0)));
                 const u32x2 x0 = lds_tr(vd), x1 = lds_tr(vd + 16 * G::ROW);
                 o[d] = mma16(u32x4{x0.x, x0.y, x1.x, x1.y}, ph, o[d], ty);
             }
