@@ -98,8 +98,14 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         const uint64_t subs = most / p.run_heads;         // times 32 keys, each with partial results of its own
         auto run_blocks = [&](uint64_t tiles, uint64_t runs) { return (tiles * runs + 7) / 8 * 8 * p.groups; };
         auto runs = [&](uint64_t tiles, uint64_t keys, uint32_t* count) {
-            // about four blocks a compute unit, 64 keys a wave of a run, 512 parts of a row
-            uint64_t n = 1024 / (tiles * p.groups);
+            // Two blocks fit a compute unit.  One request's length is known: once the
+            // card over.  Of several most are shorter than the longest, and runs that they
+            // do not have end at once: three times over.  Measured, us, by blocks (all
+            // runs counted): one request of 262144 keys, 4 bits, 80 (512), 99 (768), 104
+            // (1536); 64 of up to 8192, 8 bits, 142 (512), 122 (768), 150 (1024), 127
+            // (1536), 136 (2048); 256 of up to 4096, 4 bits, 202, 173, 188, 160, 164.  64 keys a
+            // wave of a run, 512 parts of a row.
+            uint64_t n = (B > 1 ? 1536 : 512) / (tiles * p.groups);
             if (n > keys / (64 * subs)) n = keys / (64 * subs);
             if (n > 512 / subs) n = 512 / subs;
             n = n < 1 ? 1 : n;
