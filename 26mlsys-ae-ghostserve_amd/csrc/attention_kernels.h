@@ -626,15 +626,23 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
         from_k[i] = step_k[i] ? a.pool + head_off + ck : zeros;
         from_v[i] = step_v[i] ? a.pool + a.token_bytes + head_off + cv : zeros;
     }
-    // Block scales: the lane's chunk of a key's K (from = 0) or V (token_bytes) and its
-    // scale.
+    // Block scales: the thread's chunk of a key's codes (one past the head's end is the
+    // first again: its queries are zeros, its values go nowhere) and its scale.  Keys that
+    // are not there are read from the pool's first record, and their V put as zeros.
+    uint32_t at_code[PER], at_scale[PER];
+#pragma unroll
+    for (int i = 0; i < PER && kBlocks<POOL>; ++i) {
+        const uint32_t pos = (i * kAB + tid) % CH, d = it.head * a.dim + (pos * 16 < a.dim ? pos * 16 : 0u);
+        at_code[i] = d * kBits<POOL> / 8;
+        at_scale[i] = a.scales + d / kScaleBlock;
+    }
     auto load_codes = [&](Codes16<POOL>& x, int i, uint32_t slot, uint32_t from) __attribute__((always_inline)) {
-        const uint32_t idx = i * kAB + tid, pos = idx % CH;
-        const bool in = idx / CH < uint32_t(kTileKeys) && pos * 16 < a.dim;
-        x.load(chunk_at(a, slot, from + (it.head * a.dim + pos * 16) * kBits<POOL> / 8, in));
-        x.scale = *as_global(chunk_at(a, slot, from + a.scales + (it.head * a.dim + pos * 16) / kScaleBlock, in));
+        const uint8_t* rec = a.pool + uint64_t(slot == kNoCell ? 0u : slot) * a.rec + from;
+        x.load(rec + at_code[i]);
+        x.scale = *as_global(rec + at_scale[i]);
     };
     uint32_t sl[PER];                                     // the slots that K was loaded from last
+    bool gone[kBlocks<POOL> ? PER : 1];                   // of V loaded last: its key is not there
     auto load_k = [&](uint32_t slot, uint8_t* k) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -656,6 +664,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
         for (int i = 0; i < PER; ++i) {
             if constexpr (kBlocks<POOL>) {
                 load_codes(xv[i], i, sl[i], a.token_bytes);
+                gone[i] = sl[i] == kNoCell;
                 continue;
             }
             const bool there = sl[i] != kNoCell;
@@ -674,12 +683,13 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 u32x4 w = from[CODES ? i : 0].widen(j, ty);
+                if (kBlocks<POOL> && is_v && gone[kBlocks<POOL> ? i : 0]) w = u32x4{0, 0, 0, 0};
                 if (careful) w = scrub(w);
                 *reinterpret_cast<u32x4*>(to + key * G::ROW + ((ch * 2 + j) ^ swz) * 16) = w;
             }
         }
     };
-    const uint32_t units = (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
+    const uint32_t units = kBlocks<POOL> && !a.pool_pages ? 0u : (it.k1 - it.k0 + kTileKeys - 1) / kTileKeys;
     const int32_t* const own_row = a.table + uint64_t(it.b) * a.width;
     // Of a key of the unit at `base`.  The row is chosen by lane: chosen once for the
     // unit, where its keys lie on one side of the prefix's end, the compiler lost the

@@ -6,9 +6,9 @@
 //   code = y / 2^E rounded to the nearest code (M: the largest one)
 //
 // Rows are cut into units as in norm_rotate.hip: what a rotation pairs is in one
-// lane.  A wave takes query rows, key rows or value rows of one token, not a mixture:
-// queries are computed in 32 bits, keys in 64 (which multiply and add at the rate of
-// scalar 32-bit ones here) and rounded to 32 bits before they are quantised, so that
+// lane.  A wave takes query rows or K/V rows of one token, not a mixture: queries are
+// computed in 32 bits, keys in 64 (which multiply and add at the rate of scalar 32-bit
+// ones here, and cost nothing beside the memory: 197 us with them, 195 as if V) and rounded to 32 bits before they are quantised, so that
 // a code does not hang on the noise of the sums.  A block's 32 values lie in lanes as
 // the rotation wants them, so finished rows pass through LDS (of the wave's own) and
 // come back as 16 neighbours a lane, two lanes to a block.
@@ -20,7 +20,7 @@ namespace kvec {
 struct BwArgs {
     NrArgs n;
     uint32_t half;                            // bytes of a half record
-    uint32_t q_pieces, k_pieces;              // waves of a token's queries; of its keys (as many for its values)
+    uint32_t q_pieces, k_pieces;              // waves of a token's queries; of its keys (or keys and values)
     FastDiv by_pieces;
     uint32_t items;
 };
@@ -196,10 +196,14 @@ __device__ __forceinline__ void quantise(const NrArgs& p, const float* row, uint
     if (!(sub & 1)) *as_global(half + p.kv_heads * p.dim * BITS / 8 + (r * p.dim + sub * 16) / kScaleBlock) = uint8_t(byte);
 }
 
-// QITER: query rows of a group that a wave takes.
+// QITER: query rows of a group that a wave takes.  Where that is more than one, a wave
+// takes keys and values of the same heads, too, so that the lines of a record are written
+// by one (8 bits, 32768 tokens of 32 + 2 x 8 heads of 128: 173 -> 155 us); where waves are
+// few each takes one of the two (3998 tokens 1.5 us less).
 template <class T, int BITS, int W, int NU, int QITER>
 __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
     constexpr int WAVES = kNRB / 64;
+    constexpr bool BOTH = QITER > 1;
     __shared__ Turn<double> turns[WAVES][kMaxBlockDim / 2];
     __shared__ __attribute__((aligned(16))) float rows_of[WAVES][1024];
     const NrArgs& p = g.n;
@@ -240,36 +244,50 @@ __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
     piece -= g.q_pieces;
     const int32_t slot = p.slots[t];
     if (slot < 0 || int64_t(slot) >= p.n_slots) return;
-    const bool is_v = piece >= g.k_pieces;
-    if (is_v) piece -= g.k_pieces;
-    const uint32_t r = piece * groups + group;
-    const uint8_t* from = is_v ? p.v + int64_t(t) * p.vs * int64_t(sizeof(T)) : p.k + int64_t(t) * p.ks * int64_t(sizeof(T));
-    Rows<T, W, NU, 1> x;
-    x.load(p, u, from, is_v ? p.vh : p.kh, r, 0, p.kv_heads);
-    float a[NU][W], b[NU][W];
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-        x.a[0][n].get(a[n]);
-        x.b[0][n].get(b[n]);
+    bool keys = true, values = true;
+    if (!BOTH) {
+        keys = piece < g.k_pieces;
+        values = !keys;
+        if (values) piece -= g.k_pieces;
     }
-    if (!is_v) {
+    const uint32_t r = piece * groups + group;
+    Rows<T, W, NU, 1> xk, xv;
+    if (keys) xk.load(p, u, p.k + int64_t(t) * p.ks * int64_t(sizeof(T)), p.kh, r, 0, p.kv_heads);
+    if (values) xv.load(p, u, p.v + int64_t(t) * p.vs * int64_t(sizeof(T)), p.vh, r, 0, p.kv_heads);
+    float* row = rows_of[wave] + group * p.dim;
+    uint8_t* half = p.pool + int64_t(slot) * 2 * int64_t(g.half);
+    float a[NU][W], b[NU][W];
+    if (keys) {
         Turn<double>* turn = turns[wave];
         make_turns(p, t, lane, turn);
         double c[NU][W], d[NU][W];
 #pragma unroll
-        for (int n = 0; n < NU; ++n)
+        for (int n = 0; n < NU; ++n) {
+            xk.a[0][n].get(a[n]);
+            xk.b[0][n].get(b[n]);
 #pragma unroll
             for (int j = 0; j < W; ++j) c[n][j] = double(a[n][j]), d[n][j] = double(b[n][j]);
+        }
         norm_turn<double, T, W, NU>(p, u, lanes, p.wk, turn, c, d);
 #pragma unroll
         for (int n = 0; n < NU; ++n)
 #pragma unroll
             for (int j = 0; j < W; ++j) a[n][j] = float(c[n][j]), b[n][j] = float(d[n][j]);
+        stage<W, NU>(p, u, row, a, b);
+        wave_sync();
+        quantise<T, BITS>(p, row, half, r, sub, r < p.kv_heads);
+        wave_sync();
     }
-    float* row = rows_of[wave] + group * p.dim;
-    stage<W, NU>(p, u, row, a, b);
-    wave_sync();
-    quantise<T, BITS>(p, row, p.pool + (int64_t(slot) * 2 + is_v) * int64_t(g.half), r, sub, r < p.kv_heads);
+    if (values) {
+#pragma unroll
+        for (int n = 0; n < NU; ++n) {
+            xv.a[0][n].get(a[n]);
+            xv.b[0][n].get(b[n]);
+        }
+        stage<W, NU>(p, u, row, a, b);
+        wave_sync();
+        quantise<T, BITS>(p, row, half + g.half, r, sub, r < p.kv_heads);
+    }
 }
 
 typedef void (*BwFn)(BwArgs);
@@ -296,7 +314,7 @@ int launch_block_write(const NrArgs& n, int64_t tokens, int dtype, int pool_dtyp
     const bool deep = wide && uint64_t(tokens) * (q1 + 2 * k_pieces) >= 12 * 256 * 32;
     a.q_pieces = deep ? (q1 + 3) / 4 : q1;
     a.k_pieces = k_pieces;
-    const uint64_t pieces = uint64_t(a.q_pieces) + 2 * k_pieces, items = uint64_t(tokens) * pieces;
+    const uint64_t pieces = uint64_t(a.q_pieces) + (deep ? k_pieces : 2 * k_pieces), items = uint64_t(tokens) * pieces;
     if (!launchable((items + 3) / 4, kNRB)) return set_error(KVEC_EUNSUPPORTED, "%s: too many rows for one launch", fn);
     a.by_pieces = make_fastdiv(uint32_t(pieces));
     a.items = uint32_t(items);
