@@ -198,7 +198,8 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return set_error(KVEC_EINVAL, "%s: workspace of %lld bytes, 16-byte aligned, wanted", fn, (long long)need);
     const uint64_t rec = 2 * half_bytes(s->kv_heads, s->dim, s->pool_dtype);
-    if (rec / 2 >= (uint64_t(1) << 30)) return set_error(KVEC_EUNSUPPORTED, "%s: token record too large", fn);
+    if (rec / 2 >= (block_bits(s->pool_dtype) ? kMaxBlockHalf : uint64_t(1) << 30))
+        return set_error(KVEC_EUNSUPPORTED, "%s: token record too large", fn);
     {
         auto span = [&](const void* q, int64_t st, int64_t hs, const char* name) {
             return Span{q, uint64_t((s->tokens - 1) * st + (s->heads - 1) * hs + s->dim) * 2, name, -1};

@@ -112,7 +112,7 @@ extern "C" int kvec_block_read_kv(const kvec_block_read* s, void* stream) {
     if (!aligned16(s->pool) || !aligned16(s->k) || !aligned16(s->v))
         return set_error(KVEC_EINVAL, "%s: pool, k or v not 16-byte aligned", fn);
     const uint64_t half = half_bytes(s->kv_heads, s->dim, s->pool_dtype), n = uint64_t(s->kv_heads) * uint64_t(s->dim);
-    if (half >= (uint64_t(1) << 30) || uint64_t(s->tokens) >= (uint64_t(1) << 32) ||
+    if (half >= kMaxBlockHalf || uint64_t(s->tokens) >= (uint64_t(1) << 32) ||
         uint64_t(s->tokens) * (n / 4) >= (uint64_t(1) << 32) - kBRB * kBRIter)
         return set_error(KVEC_EUNSUPPORTED, "%s: too many values for one launch", fn);
     const uint64_t out = uint64_t(s->tokens) * n * uint64_t(type_bytes(s->dtype));

@@ -312,7 +312,7 @@ int launch_block_write(const NrArgs& n, int64_t tokens, int dtype, int pool_dtyp
     BwArgs a{};
     a.n = n;
     const uint64_t half = half_bytes(int(n.kv_heads), int(n.dim), pool_dtype);
-    if (half >= (uint64_t(1) << 30)) return set_error(KVEC_EUNSUPPORTED, "%s: token record too large", fn);
+    if (half >= kMaxBlockHalf) return set_error(KVEC_EUNSUPPORTED, "%s: token record too large", fn);
     a.half = uint32_t(half);
     const uint32_t groups = 64u >> n.lg;
     const uint32_t k_pieces = (n.kv_heads + groups - 1) / groups, q1 = (n.heads + groups - 1) / groups;

@@ -149,5 +149,7 @@ inline uint64_t half_bytes(int kv_heads, int dim, int dtype) {
     const int bits = block_bits(dtype);
     return bits ? (n * uint64_t(bits) / 8 + n / kScaleBlock + 15) / 16 * 16 : n * uint64_t(type_bytes(dtype));
 }
+// Half records with block scales stay under this, so that their bits count in 32.
+constexpr uint64_t kMaxBlockHalf = uint64_t(1) << 27;
 
 }  // namespace kvec

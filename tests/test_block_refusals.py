@@ -158,3 +158,15 @@ def test_packed_read(pkg):
     assert fmt.size == C.sizeof(cls)
     s = cls.from_buffer_copy(fmt.pack(*values))
     assert [getattr(s, name) for name, _ in cls._fields_] == values
+
+
+@pytest.mark.parametrize("code, heads", [(4, 1 << 19), (5, 1 << 20)])
+def test_records_that_count_past_32_bits(pkg, no_gpu, code, heads):
+    """A token's K of 128 MiB and more: its codes' bits would not count in 32."""
+    far = {n: (i + 1) << 40 for i, n in enumerate(("q", "k", "v", "q_out", "slots", "pool"))}
+    assert norm_rotate(pkg, tokens=1, heads=1, kv_heads=heads, dim=256, q_head_stride=256, k_head_stride=256,
+                       v_head_stride=256, o_head_stride=256, pool_dtype=code, n_slots=1, **far) == -2
+    assert block_read(pkg, tokens=1, kv_heads=heads, dim=256, pool_dtype=code, n_slots=1, k=1 << 40, v=1 << 41, pool=1 << 42) == -2
+    s = dict(tokens=1, batch=1, heads=heads, kv_heads=heads, dim=256, pool_dtype=code, pool_pages=1, q_head_stride=256,
+             o_head_stride=256, q=1 << 40, out=1 << 41, pool=1 << 42)
+    assert attention(pkg, **s) == -2
