@@ -13,10 +13,12 @@
 // back, took 211 us with it and 209 with keys in 32 bits (measured when K and V still
 // had waves of their own).  A block's 32 values lie in lanes as the rotation wants them,
 // so finished rows pass through LDS (of the wave's own) and come back as 16 neighbours a
-// lane, two lanes to a block.
+// lane, two lanes to a block.  Where a piece lies in LDS is chosen so that 16 lanes meet
+// all banks (32768 tokens of 32 + 2 x 8 heads of 128, 8 bits: 165 us with rows and turns
+// in order, two thirds of them with the LDS held by conflicts; 145 so).
 //
-// Bound by memory where tokens are many (32768 of 32 + 2 x 8 heads of 128, 8 bits: 155
-// us), by the launch and the chain of loads where they are few (16 tokens: 5.4 us).
+// Bound by memory where tokens are many (those 145 us: 4.7 TB/s; 8192 tokens 41.5), by
+// the launch and the chain of loads where they are few (16 tokens: 5.0 us).
 #include "block_scale.h"
 #include "norm_rotate.h"
 
@@ -29,6 +31,8 @@ struct BwArgs {
     FastDiv by_pieces;
     uint32_t items;
 };
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr double kTwoPiHi = 6.283185307179586477;        // 2 pi rounded to 64 bits,
 constexpr double kTwoPiLo = 2.449293598294706414e-16;    // and what that leaves out
@@ -56,6 +60,21 @@ __device__ __forceinline__ double inv_root(double x) { return 1.0 / sqrt(x); }
 template <class F>
 struct Turn {
     F c, s;
+};
+
+// Where turn i lies in LDS.  Lanes read eight in a row each, 64 or 128 bytes apart; so
+// that neighbours meet other banks, places within the eight go by the lane.
+template <class F>
+__device__ __forceinline__ uint32_t turn_at(uint32_t i) {
+    return sizeof(F) == 8 ? i ^ (i >> 4 & 7) : i ^ (i >> 5 & 3) << 1;
+}
+// Where 16 bytes x of a staged row lie, in pieces of 16 bytes.  They are written one in
+// two or four, two or more rows at once (`rows`: by the row's number), and read one in
+// four: with both, 16 lanes meet all banks from rows of 256 bytes on.
+struct Place {
+    uint32_t rows;
+    __device__ __forceinline__ Place(uint32_t group, uint32_t pieces) : rows(((group & 1) * 3 ^ (group >> 1 & 1) * 10) & (pieces - 1)) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return x ^ rows ^ (x >> 4 & 3); }
 };
 
 __device__ __forceinline__ void wave_sync() {
@@ -137,7 +156,7 @@ __device__ __forceinline__ void norm_turn(const NrArgs& p, const Units<W, NU>& u
             // pairs of neighbours: the first W/2 in a, the rest in b
 #pragma unroll
             for (int j = 0; j < W / 2; ++j) {
-                const Turn<F> c0 = turn[u.pair[n] + j], c1 = turn[u.pair[n] + W / 2 + j];
+                const Turn<F> c0 = turn[turn_at<F>(u.pair[n] + j)], c1 = turn[turn_at<F>(u.pair[n] + W / 2 + j)];
                 const F x0 = a[n][2 * j], y0 = a[n][2 * j + 1], x1 = b[n][2 * j], y1 = b[n][2 * j + 1];
                 a[n][2 * j] = x0 * c0.c - y0 * c0.s;
                 a[n][2 * j + 1] = x0 * c0.s + y0 * c0.c;
@@ -147,7 +166,7 @@ __device__ __forceinline__ void norm_turn(const NrArgs& p, const Units<W, NU>& u
         } else {
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const Turn<F> c = turn[u.pair[n] + j];
+                const Turn<F> c = turn[turn_at<F>(u.pair[n] + j)];
                 const F x = a[n][j], y = b[n][j];
                 a[n][j] = x * c.c - y * c.s;
                 b[n][j] = x * c.s + y * c.c;
@@ -162,32 +181,49 @@ __device__ __forceinline__ void make_turns(const NrArgs& p, uint32_t t, uint32_t
     const uint32_t half = p.rot / 2;
     for (uint32_t i = lane; i < half; i += 64) {
         const uint32_t ax = p.axis_of ? min(uint32_t(p.axis_of[i]), p.axes - 1) : 0u;
-        turn_of(double(p.pos[int64_t(ax) * p.axis_stride + t]) * p.freqs[i], p.factor, &turn[i].c, &turn[i].s);
+        Turn<F>& to = turn[turn_at<F>(i)];
+        turn_of(double(p.pos[int64_t(ax) * p.axis_stride + t]) * p.freqs[i], p.factor, &to.c, &to.s);
     }
     wave_sync();
 }
 
 // A lane's units of a finished row as 32-bit values in LDS.
 template <int W, int NU>
-__device__ __forceinline__ void stage(const NrArgs& p, const Units<W, NU>& u, float* row, const float (*a)[W], const float (*b)[W]) {
-#pragma unroll
-    for (int n = 0; n < NU; ++n)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            if (u.a[n] < p.dim) row[u.a[n] + j] = a[n][j];
-            if (u.b[n] < p.dim) row[u.b[n] + j] = b[n][j];
+__device__ __forceinline__ void stage(const NrArgs& p, const Units<W, NU>& u, const Place& place, float* row, const float (*a)[W],
+                                      const float (*b)[W]) {
+    auto put = [&](uint32_t at, const float* x) __attribute__((always_inline)) {
+        if (at >= p.dim) return;
+        if constexpr (W == 8) {
+            f32x4* to = reinterpret_cast<f32x4*>(row);
+            to[place(at / 4)] = f32x4{x[0], x[1], x[2], x[3]};
+            to[place(at / 4 + 1)] = f32x4{x[4], x[5], x[6], x[7]};
+        } else {
+            row[place(at / 4) * 4 + at % 4] = x[0];
         }
+    };
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+        put(u.a[n], a[n]);
+        put(u.b[n], b[n]);
+    }
 }
 
 // Row `r` of a half record out of LDS: 16 neighbours a lane, two lanes a block.
 template <class T, int BITS>
-__device__ __forceinline__ void quantise(const NrArgs& p, const float* row, uint8_t* half, uint32_t r, uint32_t sub, bool live) {
+__device__ __forceinline__ void quantise(const NrArgs& p, const Place& place, const float* row, uint8_t* half, uint32_t r, uint32_t sub,
+                                         bool live) {
     const bool mine = sub * 16 < p.dim;
     float y[16];
     uint32_t top = 0;
 #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f32x4 x = {0, 0, 0, 0};
+        if (mine) x = reinterpret_cast<const f32x4*>(row)[place(sub * 4 + i)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[4 * i + j] = x[j];
+    }
+#pragma unroll
     for (int i = 0; i < 16; ++i) {
-        y[i] = mine ? row[sub * 16 + i] : 0.0f;
         top = max(top, __float_as_uint(y[i]) & 0x7FFFFFFFu);
     }
     top = max(top, uint32_t(__shfl_xor(int(top), 1, 64)));
@@ -203,13 +239,13 @@ __device__ __forceinline__ void quantise(const NrArgs& p, const float* row, uint
 
 // QITER: query rows of a group that a wave takes.  Where that is more than one, a wave
 // takes keys and values of the same heads, too, so that the lines of a record are written
-// by one (8 bits, 32768 tokens of 32 + 2 x 8 heads of 128: 173 -> 155 us); where waves are
+// by one (8 bits, 32768 tokens of 32 + 2 x 8 heads of 128: 173 -> 155 us when measured); where waves are
 // few each takes one of the two (3998 tokens 1.5 us less).
 template <class T, int BITS, int W, int NU, int QITER>
 __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
     constexpr int WAVES = kNRB / 64;
     constexpr bool BOTH = QITER > 1;
-    __shared__ Turn<double> turns[WAVES][kMaxBlockDim / 2];
+    __shared__ __attribute__((aligned(16))) Turn<double> turns[WAVES][kMaxBlockDim / 2];
     __shared__ __attribute__((aligned(16))) float rows_of[WAVES][1024];
     const NrArgs& p = g.n;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -259,7 +295,10 @@ __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
     Rows<T, W, NU, 1> xk, xv;
     if (keys) xk.load(p, u, p.k + int64_t(t) * p.ks * int64_t(sizeof(T)), p.kh, r, 0, p.kv_heads);
     if (values) xv.load(p, u, p.v + int64_t(t) * p.vs * int64_t(sizeof(T)), p.vh, r, 0, p.kv_heads);
-    float* row = rows_of[wave] + group * p.dim;
+    // a row's place in LDS: what its lanes hold, a power of two
+    const uint32_t pieces = lanes * (2 * W * NU) / 4;
+    const Place place(group, pieces);
+    float* row = rows_of[wave] + group * pieces * 4;
     uint8_t* half = p.pool + int64_t(slot) * 2 * int64_t(g.half);
     float a[NU][W], b[NU][W];
     if (keys) {
@@ -278,9 +317,9 @@ __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
         for (int n = 0; n < NU; ++n)
 #pragma unroll
             for (int j = 0; j < W; ++j) a[n][j] = float(c[n][j]), b[n][j] = float(d[n][j]);
-        stage<W, NU>(p, u, row, a, b);
+        stage<W, NU>(p, u, place, row, a, b);
         wave_sync();
-        quantise<T, BITS>(p, row, half, r, sub, r < p.kv_heads);
+        quantise<T, BITS>(p, place, row, half, r, sub, r < p.kv_heads);
         wave_sync();
     }
     if (values) {
@@ -289,9 +328,9 @@ __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
             xv.a[0][n].get(a[n]);
             xv.b[0][n].get(b[n]);
         }
-        stage<W, NU>(p, u, row, a, b);
+        stage<W, NU>(p, u, place, row, a, b);
         wave_sync();
-        quantise<T, BITS>(p, row, half + g.half, r, sub, r < p.kv_heads);
+        quantise<T, BITS>(p, place, row, half + g.half, r, sub, r < p.kv_heads);
     }
 }
 
