@@ -3,9 +3,9 @@
 //   value = code * 2^(byte - 127), rounded to the wanted type
 //
 // Nothing is computed to speak of: 33 (e4m3) or 17 (e2m1) bytes come in for 64 that
-// leave, so the kernel is bound by its stores.  A lane turns 8 neighbours into one
-// 16-byte store (two for 32-bit values), lanes side by side along a token's K and then
-// its V; it takes four such pieces, with all their loads in flight before the first
+// leave, so the kernel is bound by its stores.  A lane turns 8 neighbours (of 32
+// bits: 4) into one 16-byte store, lanes side by side along a token's K and then its V;
+// it takes four such pieces, with all their loads in flight before the first
 // is used.  32768 tokens of 8 heads of 128 from 8 bits to bf16: 35 to 37 us, 5.6 TB/s;
 // 500 tokens 3.1 us.
 #include "block_scale.h"
@@ -26,7 +26,11 @@ struct BrArgs {
     uint32_t scales;                          // where its scales start
 };
 
-// Eight codes and their scale as T in memory.
+// A piece: what makes one 16-byte store.
+template <class T>
+constexpr uint32_t kPiece = 16 / sizeof(T);
+
+// The codes of a piece and their scale as T in memory.
 template <int BITS, class T>
 __device__ __forceinline__ void put_codes(T* to, u32x2 x, float scale) {
     st16(reinterpret_cast<uint8_t*>(to), widen8<BITS>(x, scale, (T*)nullptr));
@@ -34,20 +38,23 @@ __device__ __forceinline__ void put_codes(T* to, u32x2 x, float scale) {
 template <int BITS>
 __device__ __forceinline__ void put_codes(float* to, u32x2 x, float scale) {
     typedef float f32x2v __attribute__((ext_vector_type(2)));
-    f32x2v f[4];
+    f32x2v f, g;
     if constexpr (BITS == 8) {
-        f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.x, scale, false);
-        f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.x, scale, true);
-        f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.y, scale, false);
-        f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.y, scale, true);
+        f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.x, scale, false);
+        g = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.x, scale, true);
     } else {
-        f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.x, scale, 0);
-        f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.x, scale, 1);
-        f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.x, scale, 2);
-        f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.x, scale, 3);
+        f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.x, scale, 0);
+        g = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.x, scale, 1);
     }
-    const float y[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
-    put8(to, y);
+    st16(reinterpret_cast<uint8_t*>(to), u32x4{__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(g.x), __float_as_uint(g.y)});
+}
+template <int BITS, class T>
+__device__ __forceinline__ u32x2 codes_of(const uint8_t* half, uint32_t at) {
+    constexpr uint32_t N = kPiece<T> * BITS / 8;              // bytes
+    const uint8_t* p = half + at * N;
+    if constexpr (N == 8) return *as_global(reinterpret_cast<const u32x2*>(p));
+    else if constexpr (N == 4) return u32x2{*as_global(reinterpret_cast<const uint32_t*>(p)), 0};
+    else return u32x2{*as_global(reinterpret_cast<const uint16_t*>(p)), 0};
 }
 
 template <class T, int BITS>
@@ -73,15 +80,14 @@ __global__ __launch_bounds__(kBRB) void block_read_kernel(BrArgs a) {
         byte[i] = 0;
         if (slot[i] >= 0 && int64_t(slot[i]) < a.n_slots) {
             const uint8_t* half = a.pool + (int64_t(slot[i]) * 2 + is_v[i]) * int64_t(a.half);
-            if constexpr (BITS == 8) x[i] = *as_global(reinterpret_cast<const u32x2*>(half + at[i] * 8));
-            else x[i].x = *as_global(reinterpret_cast<const uint32_t*>(half + at[i] * 4));
-            byte[i] = *as_global(half + a.scales + at[i] / (kScaleBlock / 8));
+            x[i] = codes_of<BITS, T>(half, at[i]);
+            byte[i] = *as_global(half + a.scales + at[i] / (kScaleBlock / kPiece<T>));
         }
     }
 #pragma unroll
     for (int i = 0; i < kBRIter; ++i) {
         if (first + i * kBRB >= a.pieces) break;
-        T* out = reinterpret_cast<T*>(is_v[i] ? a.v : a.k) + (uint64_t(t[i]) * a.by_half.d + at[i]) * 8;
+        T* out = reinterpret_cast<T*>(is_v[i] ? a.v : a.k) + (uint64_t(t[i]) * a.by_half.d + at[i]) * kPiece<T>;
         put_codes<BITS>(out, x[i], scale_of(byte[i]));
     }
 }
@@ -112,8 +118,9 @@ extern "C" int kvec_block_read_kv(const kvec_block_read* s, void* stream) {
     if (!aligned16(s->pool) || !aligned16(s->k) || !aligned16(s->v))
         return set_error(KVEC_EINVAL, "%s: pool, k or v not 16-byte aligned", fn);
     const uint64_t half = half_bytes(s->kv_heads, s->dim, s->pool_dtype), n = uint64_t(s->kv_heads) * uint64_t(s->dim);
+    const uint64_t piece = 16 / uint64_t(type_bytes(s->dtype));
     if (half >= kMaxBlockHalf || uint64_t(s->tokens) >= (uint64_t(1) << 32) ||
-        uint64_t(s->tokens) * (n / 4) >= (uint64_t(1) << 32) - kBRB * kBRIter)
+        uint64_t(s->tokens) * (2 * n / piece) >= (uint64_t(1) << 32) - kBRB * kBRIter)
         return set_error(KVEC_EUNSUPPORTED, "%s: too many values for one launch", fn);
     const uint64_t out = uint64_t(s->tokens) * n * uint64_t(type_bytes(s->dtype));
     {
@@ -127,9 +134,9 @@ extern "C" int kvec_block_read_kv(const kvec_block_read* s, void* stream) {
     a.k = (uint8_t*)s->k;
     a.v = (uint8_t*)s->v;
     a.n_slots = s->n_slots;
-    a.by_half = make_fastdiv(uint32_t(n / 8));
-    a.by_token = make_fastdiv(uint32_t(n / 4));
-    a.pieces = uint32_t(uint64_t(s->tokens) * (n / 4));
+    a.by_half = make_fastdiv(uint32_t(n / piece));
+    a.by_token = make_fastdiv(uint32_t(2 * n / piece));
+    a.pieces = uint32_t(uint64_t(s->tokens) * (2 * n / piece));
     a.half = uint32_t(half);
     a.scales = uint32_t(n * uint64_t(bits) / 8);
     BrFn f = s->dtype == KVEC_F32 ? pick_br<float>(bits) : s->dtype == KVEC_BF16 ? pick_br<__bf16>(bits) : pick_br<_Float16>(bits);
