@@ -1231,6 +1231,13 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
 // A weight of 0 makes NaN of a V that is not finite, so the loop runs a second time where
 // it has given a NaN: with such values taken out, and added to the rows that see them
 // afterwards.
+//
+// Bound by loads, and in 4 bits by LDS beside them.  Eight K/V heads of 128 values, four
+// query heads each: 256 requests of 4096 keys 389 us, 5.7 TB/s (8 bits), 233 us, 4.9 TB/s
+// (4 bits), where plain stream blocks over 16 bits take 788; of 64 values and of one or two
+// heads less (55 us, 5.0 TB/s for 64 requests of 64 values; 36 us, 2.1 TB/s with one head).
+// HW: two heads of 4 bits in a wave, whose rows then fill a product's 16, 241 us where one
+// took 288 (256 requests of up to 4096 keys, when measured).
 template <int DP, int BITS>
 struct RunGeom {
     static constexpr int ROW = TileGeom<DP>::ROW;         // bytes of a key's V in 16 bits

@@ -17,7 +17,7 @@
 // all banks (32768 tokens of 32 + 2 x 8 heads of 128, 8 bits: 165 us with rows and turns
 // in order, two thirds of them with the LDS held by conflicts; 145 so).
 //
-// Bound by memory where tokens are many (those 145 us: 4.7 TB/s; 8192 tokens 41.5), by
+// Bound by memory where tokens are many (those 145 us: 5.1 TB/s; 8192 tokens 41.5), by
 // the launch and the chain of loads where they are few (16 tokens: 5.0 us).
 #include "block_scale.h"
 #include "norm_rotate.h"
