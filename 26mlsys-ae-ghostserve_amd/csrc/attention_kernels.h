@@ -1676,17 +1676,33 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
     float top = -INFINITY, l = 0.0f;
     const float c = fabsf(score_factor(a));
     f32x4 o = {0, 0, 0, 0};
+#pragma unroll 4
     for (uint32_t p = tid & 63; p < parts; p += 64) top = fmaxf(top, as_global(a.ws_ml)[uint64_t(p) * rows + row].x);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-#pragma unroll 4
-    for (uint32_t p = mine; p < parts; p += each) {
-        const uint64_t at = uint64_t(p) * rows + row;
-        const f32x2 ml = as_global(a.ws_ml)[at];
-        if (ml.x == -INFINITY) continue;                  // nothing seen there
-        const float f = __builtin_amdgcn_exp2f((ml.x - top) * c);
-        l += ml.y * f;
-        if (d < a.dim) o += *as_global(reinterpret_cast<const f32x4*>(a.ws_o + at * a.dim + d)) * f;
+    // four parts at a time, so that their loads are under way together (32 rows with 512
+    // parts, eight blocks a row, 11.4 -> 8.5 us; 8192 rows with 6 parts 13.5 -> 14.3)
+    for (uint32_t p0 = mine; p0 < parts; p0 += 4 * each) {
+        f32x2 ml[4];
+        f32x4 x[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            ml[i] = f32x2{-INFINITY, 0.0f};
+            if (p0 + i * each < parts) ml[i] = as_global(a.ws_ml)[uint64_t(p0 + i * each) * rows + row];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            x[i] = f32x4{0, 0, 0, 0};
+            if (ml[i].x != -INFINITY && d < a.dim)        // (else nothing seen there, and nothing written)
+                x[i] = *as_global(reinterpret_cast<const f32x4*>(a.ws_o + (uint64_t(p0 + i * each) * rows + row) * a.dim + d));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (ml[i].x == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f((ml[i].x - top) * c);
+            l += ml[i].y * f;
+            o += x[i] * f;
+        }
     }
     lo[tid] = o;
     ll[tid] = l;
