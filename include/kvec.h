@@ -42,7 +42,8 @@ extern "C" {
  * unit_bytes, kvec_chunk_stripe has region_off and unit_bytes (0.1.0 had
  * neither).  1.1.0: kvec_hook_step added.  1.2.0: the *_kv entry points over
  * kvec_kv_bhtd added.  1.3.0: kvec_step_tables, kvec_norm_rotate_write,
- * kvec_prefix_attention added. */
+ * kvec_prefix_attention added.  1.4.0: pools with block scales (KVEC_BLOCK_*) and
+ * kvec_block_read_kv added. */
 #define KVEC_VERSION 10400
 int kvec_version(void);
 /* Static description of a KVEC_E* code. */
@@ -386,7 +387,8 @@ int kvec_gf16_tables(uint16_t* gf_exp, uint16_t* gf_log);
  * codes (e4m3 bytes; e2m1, 0 .5 1 1.5 2 3 4 6 and a sign, two to a byte, the first
  * in the low half), then a byte for each block of 32 neighbouring values of a head,
  * then up to 15 bytes, never written, to a multiple of 16.  A value is code *
- * 2^(byte - 127); byte 255: NaN, all 32.  dim: a multiple of 32 up to 256.
+ * 2^(byte - 127); byte 255: NaN, all 32.  dim: a multiple of 32 up to 256;
+ * half records of 128 MiB and more are refused.
  * Writing: byte - 127 is the smallest whole number >= -127 with which no value of
  * the block passes the largest code (448, 6), codes are the nearest ones, ties to
  * even; a block with an infinity or NaN gets 255; values that would round past the
