@@ -439,6 +439,11 @@ __device__ __forceinline__ u32x2 value4(const AttnArgs& a, uint32_t slot, uint32
     else return *as_global(reinterpret_cast<const u32x2*>(p));
 }
 
+// Whether heads of pools with block scales may have fewer values than DP: they are
+// multiples of 32, and the kernels' sizes 64, 96, 128 and 256.
+template <int POOL, int DP>
+constexpr bool kPadded = kBlocks<POOL> && (DP == 64 || DP == 256);
+
 // Sixteen codes as they lie in memory, and their scale's byte.
 template <int POOL>
 struct Codes16 {
@@ -627,7 +632,8 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
         from_v[i] = step_v[i] ? a.pool + a.token_bytes + head_off + cv : zeros;
     }
     // Block scales: the thread's chunk of a key's codes (one past the head's end is the
-    // first again: its queries are zeros, its values go nowhere) and its scale.  Keys that
+    // first again, put under the smallest scale: its queries are zeros, of which an infinity
+    // would make NaN, its values go nowhere) and its scale.  Keys that
     // are not there are read from the pool's first record, and their V put as zeros.
     uint32_t at_code[PER], at_scale[PER];
 #pragma unroll
@@ -680,9 +686,11 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             const uint32_t idx = i * kAB + tid, key = idx / CH, ch = idx % CH;
             if (kTileKeys * CH % kAB && key >= uint32_t(kTileKeys)) break;
             const uint32_t swz = is_v ? G::swz_v(key) : G::swz_k(key);
+            Codes16<POOL> x = from[CODES ? i : 0];
+            if (kPadded<POOL, DP> && ch * 16 >= a.dim) x.scale = 0;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                u32x4 w = from[CODES ? i : 0].widen(j, ty);
+                u32x4 w = x.widen(j, ty);
                 if (kBlocks<POOL> && is_v && gone[kBlocks<POOL> ? i : 0]) w = u32x4{0, 0, 0, 0};
                 if (careful) w = scrub(w);
                 *reinterpret_cast<u32x4*>(to + key * G::ROW + ((ch * 2 + j) ^ swz) * 16) = w;
@@ -1440,7 +1448,7 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
                 const uint32_t at = G::code_at(hh, key);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    // (past the head's end: what is there; the queries are zeros)
+                    // (past the head's end: the first chunk again; the queries are zeros)
                     const uint32_t d0 = value_at(ks), d = d0 < a.dim ? d0 : d0 % VALS;
                     const uint8_t* p = codes + (at ^ d / VALS * 16 ^ d % VALS / (VALS / 2) * 8);
                     if constexpr (BITS == 8) {
@@ -1458,9 +1466,12 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t d = value_at(ks);
-                    // a lane's values have one scale, or one every 32
-                    if (ks == 0 || DP == 96 || (DP == 256 && ks % 4 == 0))
+                    // a lane's values have one scale, or one every 32; past the head's end the
+                    // smallest: an infinity would make NaN of the zeros
+                    if (ks == 0 || DP == 96 || (DP == 256 && ks % 4 == 0)) {
                         scale = scale_at(sub * kStreamKeys + key, hh, d < a.dim ? d / kScaleBlock : 0u);
+                        if (kPadded<POOL, DP> && d >= a.dim) scale = scale_of(0);
+                    }
                     y = mma16(widen8<BITS>(x[ks], scale, ty), qf[ks], y, ty);
                 }
                 if (HW == 1) {
