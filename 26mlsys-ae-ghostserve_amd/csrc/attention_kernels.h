@@ -1675,7 +1675,7 @@ __global__ __launch_bounds__(kAB, DP <= 128 ? 2 : 1) void attn_kernel(AttnArgs a
 // A block takes one row, or 4 * lanes values of it: `lanes` threads a part, the parts
 // shared out to the others, so that a row's parts are read side by side.  Measured: 2048 rows of 128
 // with 12 parts 6.0 us (6.5 where the row's request is looked for), 8192 rows with 7
-// parts 12.7, 128 rows with 5 parts 3.8.
+// parts 13.5, 128 rows with 5 parts 4.0.
 template <class T>
 __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lanes) {
     __shared__ f32x4 lo[kAB];
@@ -1691,9 +1691,20 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
     for (uint32_t p = tid & 63; p < parts; p += 64) top = fmaxf(top, as_global(a.ws_ml)[uint64_t(p) * rows + row].x);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-    // four parts at a time, so that their loads are under way together (32 rows with 512
-    // parts, eight blocks a row, 11.4 -> 8.5 us; 8192 rows with 6 parts 13.5 -> 14.3)
-    for (uint32_t p0 = mine; p0 < parts; p0 += 4 * each) {
+    // Where every part has threads of its own, each takes one; otherwise four at a time, so
+    // that their loads are under way together.  Measured, us, one at a time and four: 8192
+    // rows of 6 or 7 parts and 8 places 13.6, 14.2; 2048 rows of 12 and 16 places 5.2, 5.4;
+    // of 12 and 8 places 6.1, 6.0; 1024 rows of 48 and 4 places 12.2, 10.6; 32 rows of 512
+    // and 64 places 10.3, 8.6 (2048 rows of 48 and 8 places 11.3, 11.9).
+    if (parts <= each) {
+        const uint64_t at = uint64_t(mine) * rows + row;
+        const f32x2 ml = mine < parts ? as_global(a.ws_ml)[at] : f32x2{-INFINITY, 0.0f};
+        if (ml.x != -INFINITY) {                          // (else nothing seen there, and nothing written)
+            const float f = __builtin_amdgcn_exp2f((ml.x - top) * c);
+            l = ml.y * f;
+            if (d < a.dim) o += *as_global(reinterpret_cast<const f32x4*>(a.ws_o + at * a.dim + d)) * f;
+        }
+    } else for (uint32_t p0 = mine; p0 < parts; p0 += 4 * each) {
         f32x2 ml[4];
         f32x4 x[4];
 #pragma unroll
@@ -1704,7 +1715,7 @@ __global__ __launch_bounds__(kAB) void attn_join_kernel(AttnArgs a, uint32_t lan
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             x[i] = f32x4{0, 0, 0, 0};
-            if (ml[i].x != -INFINITY && d < a.dim)        // (else nothing seen there, and nothing written)
+            if (ml[i].x != -INFINITY && d < a.dim)
                 x[i] = *as_global(reinterpret_cast<const f32x4*>(a.ws_o + (uint64_t(p0 + i * each) * rows + row) * a.dim + d));
         }
 #pragma unroll
