@@ -9,7 +9,7 @@ struct AttnPlan {
     uint32_t parts_flat, parts_own, tiles_flat, req_tiles, first;
     uint64_t rows, tiles_own, blocks_flat, blocks;
     // pools with block scales: K/V heads of a wave, groups of a block's, runs, and see AttnArgs
-    uint32_t wave_heads, run_heads, groups, run_keys, runs_flat, runs_own;
+    uint32_t wave_heads, run_heads, groups, run_keys, few_keys, runs_flat, runs_own;
     bool direct() const { return parts_flat + parts_own == 1; }
     int64_t bytes(int64_t dim) const {
         return direct() ? 0 : int64_t(uint64_t(parts_flat + parts_own) * rows * (uint64_t(dim) * 4 + 8)) + 16;
@@ -96,17 +96,18 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         while (p.run_heads < most && p.run_heads < Hk) p.run_heads *= 2;
         p.groups = uint32_t((Hk + p.run_heads - 1) / p.run_heads);
         const uint64_t subs = most / p.run_heads;         // times 32 keys, each with partial results of its own
+        p.few_keys = uint32_t(64 * subs);
         auto run_blocks = [&](uint64_t tiles, uint64_t runs) { return (tiles * runs + 7) / 8 * 8 * p.groups; };
         auto runs = [&](uint64_t tiles, uint64_t keys, uint32_t* count) {
-            // Two blocks fit a compute unit.  One request's length is known: once the
-            // card over.  Of several most are shorter than the longest, and runs that they
-            // do not have end at once: three times over.  Measured, us, by blocks (all
+            // Two blocks fit a compute unit.  One request has all its runs: once the card
+            // over.  Of several most are shorter than the longest, and runs that they do
+            // not have end at once: three times over.  Measured, us, by blocks (all
             // runs counted): one request of 262144 keys, 4 bits, 80 (512), 99 (768), 104
             // (1536); 64 of up to 8192, 8 bits, 142 (512), 122 (768), 150 (1024), 127
             // (1536), 136 (2048); 256 of up to 4096, 4 bits, 202, 173, 188, 160, 164.  64 keys a
             // wave of a run, 512 parts of a row.
             uint64_t n = (B > 1 ? 1536 : 512) / (tiles * p.groups);
-            if (n > keys / (64 * subs)) n = keys / (64 * subs);
+            if (n > keys / p.few_keys) n = keys / p.few_keys;
             if (n > 512 / subs) n = 512 / subs;
             n = n < 1 ? 1 : n;
             *count = uint32_t(n);
@@ -255,6 +256,7 @@ extern "C" int kvec_prefix_attention(const kvec_attention* s, void* workspace, i
     if (p.run_heads) {
         a.run_heads = p.run_heads;
         a.run_keys = p.run_keys;
+        a.few_keys = p.few_keys;
         a.by_groups = make_fastdiv(p.groups);
         a.by_tiles_flat = make_fastdiv(p.tiles_flat ? p.tiles_flat : 1);
         a.by_tiles_own = make_fastdiv(uint32_t(p.tiles_own));

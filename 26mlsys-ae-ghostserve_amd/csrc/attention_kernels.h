@@ -175,8 +175,9 @@ struct AttnArgs {
     FastDiv by_flat, by_own;                   // splits of each part
     FastDiv by_heads_flat, by_heads_own;       // K/V heads times splits
     // Runs (stream blocks of a pool with block scales): the K/V heads of a block, a power
-    // of two; groups of so many; row tiles and runs of each part; the fewest keys of a run
-    uint32_t run_heads, run_keys;
+    // of two; groups of so many; row tiles and runs of each part; keys of a run by max_len,
+    // and the fewest
+    uint32_t run_heads, run_keys, few_keys;
     FastDiv by_groups, by_tiles_flat, by_tiles_own, by_runs_flat, by_runs_own;
     int direct;                                // one part in all: outputs are final
     int wide_q, wide_o;                        // 16-byte rows
@@ -330,6 +331,20 @@ __device__ __forceinline__ Item make_item(const AttnArgs& a, uint32_t id) {
     return it;
 }
 
+// Tokens of the longest request, as far as a table row covers them; 256 requests are
+// asked for at a time.
+__device__ __forceinline__ uint32_t longest(const AttnArgs& a) {
+    const uint32_t lane = threadIdx.x & 63;
+    int32_t top = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 256) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) top = max(top, *as_global(a.seq_lens + min(b0 + i * 64 + lane, a.batch - 1)));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d, 64));
+    return min(uint32_t(__builtin_amdgcn_readfirstlane(top)), a.cap);
+}
+
 // A block's run of a pool with block scales.  Blocks go to the eight XCDs in turn: ids
 // eight apart are the groups of heads of the same rows and run; then come the same run of
 // the other row tiles, so that the later runs, which only long requests have, come last;
@@ -374,10 +389,25 @@ __device__ __forceinline__ Item make_run(const AttnArgs& a, uint32_t id) {
             last = seen_by(a, it.b, it.t0 + fdiv(end_row, a.by_group));
         }
     }
-    // runs of run_keys, or longer where so many do not hold them
+    // Equal shares; of own keys, runs of one length for all requests: run_keys, but where
+    // that is for more than twice the request's keys (max_len may be a table's width, or a
+    // captured step's largest) the longest request's share, and few_keys at least.
+    // Measured, 8 bits, us, by run_keys alone and so: one request of 4096 keys in a table of
+    // 262144 53, 14.6; 64 of up to 2048 in one of 32768 97, 44; with max_len right, 64 of up
+    // to 8192 128.1, 129.1, 256 of up to 4096 270.5, 274.9.
     const uint32_t n = last > first ? last - first : 0u;
-    const uint32_t steps = (n + kStreamKeys - 1) / kStreamKeys;
-    const uint32_t each = max(fdiv(steps + parts - 1, by_runs) * kStreamKeys, it.flat ? 0u : a.run_keys);
+    auto share = [&](uint32_t keys) __attribute__((always_inline)) {
+        return fdiv((keys + kStreamKeys - 1) / kStreamKeys + parts - 1, by_runs) * kStreamKeys;
+    };
+    uint32_t each = share(n);
+    if (!it.flat) {
+        uint32_t run = max(a.run_keys, a.few_keys);
+        if (run > a.few_keys && n && uint64_t(run) * parts > uint64_t(n) * 2) {
+            const uint32_t top = longest(a);
+            run = min(run, max(share(top > first ? top - first : 0u), a.few_keys));
+        }
+        each = max(each, run);
+    }
     it.k0 = first + min(uint64_t(split) * each, uint64_t(n));
     it.k1 = first + min(uint64_t(split + 1) * each, uint64_t(n));
     return it;
