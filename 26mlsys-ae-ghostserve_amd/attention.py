@@ -105,8 +105,8 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     Token t's K and V go to slot ``slots[t]`` (int32, page * page_tokens + place;
     negative or past the pool: none) of the pool's ``layer``, in the queries' type
     or, float8_e4m3fn, as value / scale, or, a :class:`.blockscale.BlockPool`, as codes
-    with their blocks' scales (K computed in 64 bits and rounded to 32 first, so that its
-    codes do not hang on how the sums were split).  The slots of a call must be distinct.
+    with their blocks' scales (K computed in 64 bits, from ``eps`` and ``factor`` rounded to
+    32, and rounded to 32 first, so that its codes do not hang on how the sums were split).  The slots of a call must be distinct.
     ``tokens`` (int32 [1] on the GPU, e.g. ``cu_new[-1:]``): tokens from that
     number on are left as they were, here and in the result.
 

@@ -7,8 +7,9 @@
 //
 // Rows are cut into units as in norm_rotate.hip: what a rotation pairs is in one
 // lane.  A wave takes query rows or K/V rows of one token, not a mixture: queries are
-// computed in 32 bits, keys in 64 and rounded to 32 before they are quantised, so that
-// a code does not hang on the noise of the sums.  64-bit arithmetic runs at the rate of
+// computed in 32 bits, keys in 64 (from eps and factor, which are 32-bit numbers) and
+// rounded to 32 before they are quantised, so that a code does not hang on the noise of
+// the sums.  64-bit arithmetic runs at the rate of
 // scalar 32-bit arithmetic here and the memory hides it: 32768 tokens, written and read
 // back, took 211 us with it and 209 with keys in 32 bits (measured when K and V still
 // had waves of their own).  A block's 32 values lie in lanes as the rotation wants them,

@@ -436,8 +436,8 @@ int kvec_step_tables(const kvec_step* step, void* stream);
  * Pair i is (x[i], x[i + rot/2]), or (x[2i], x[2i+1]) if interleaved; values
  * from rot on are not turned.  Angles in 64 bits, the rest in 32, one rounding
  * at the end.  An fp8 pool gets x / scale, values past +-448 as +-448.  For a pool
- * with block scales keys are computed in 64 bits and rounded to 32 before they are
- * quantised: a code is a decision, which the noise of 32 bits would make differently
+ * with block scales keys are computed in 64 bits (eps and factor are the 32-bit numbers
+ * given here) and rounded to 32 before they are quantised: a code is a decision, which the noise of 32 bits would make differently
  * in another kernel, and the bytes are what the codes above protect.
  * Queries go to q_out (q itself with q's strides: in place; k and v may lie
  * between its rows then, but share no values with it).  A slot outside
