@@ -16,8 +16,11 @@ byte, the first in the low half), then a scale byte for each block of 32
 neighbouring values of a head, then up to 15 bytes that nothing writes, to a multiple
 of 16.  A value is code * 2^(byte - 127); byte 255 makes all 32 NaN.  That is 8.25 or
 4.25 bits a value.  A block's scale is the smallest power of two with which no value
-passes the largest code (448 or 6), so nothing is clipped; codes are the nearest
-ones, ties to even.  A block in which a value is infinite or NaN reads back as NaN.
+passes the largest code (448 or 6); codes are the nearest ones, ties to even.  Values
+that would round past the largest of the type they come from are taken as the last that
+does not: for float16 those past 61440 (8 bits) or 49152 (4 bits, down by up to a
+quarter), for bfloat16 and float32 past 1.875 or 1.5 times 2^127.  No others are clipped.
+A block in which a value is infinite or NaN reads back as NaN.
 """
 from __future__ import annotations
 
