@@ -66,7 +66,7 @@ constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
 enum Pool { kPlain, kFp8, kBlock8, kBlock4 };
 template <int POOL>
 constexpr bool kBlocks = POOL == kBlock8 || POOL == kBlock4;
-// Bits of a value, for pools that are not plain; bytes of `n` values.
+// Bits of a value.
 template <int POOL>
 constexpr int kBits = POOL == kPlain ? 16 : POOL == kBlock4 ? 4 : 8;
 
@@ -653,8 +653,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 #pragma unroll
     for (int i = 0; i < PER && !kBlocks<POOL>; ++i) {
         const uint32_t idx = CODES ? i * kAB + tid : (wave * PER + i) * 64 + lane, key = idx / CH, pos = idx % CH;
-        constexpr uint32_t CB = POOL == kBlock4 ? 8 : 16;         // bytes of a chunk
-        const uint32_t ck = (CODES ? pos : pos ^ G::swz_k(key)) * CB, cv = (CODES ? pos : pos ^ G::swz_v(key)) * CB;
+        const uint32_t ck = (CODES ? pos : pos ^ G::swz_k(key)) * 16, cv = (CODES ? pos : pos ^ G::swz_v(key)) * 16;
         const bool in = key < uint32_t(kTileKeys);
         step_k[i] = in && ck < row_bytes ? a.rec : 0u;
         step_v[i] = in && cv < row_bytes ? a.rec : 0u;
@@ -1326,13 +1325,6 @@ constexpr int kRunKeys = 256;                             // most keys of a bloc
 __device__ __forceinline__ float max_quarters(float x) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-// What a wave wrote to LDS, before what its lanes read there from here on.
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // A barrier of the block for its LDS alone: loads on their way stay on their way.

@@ -6,8 +6,6 @@
 
 namespace kvec {
 
-typedef short s16x2 __attribute__((ext_vector_type(2)));
-
 // A scale byte as the 32-bit float that the conversions take: they read its exponent
 // bits only, so byte 0 is 2^-127 there (not 0) and byte 255 makes NaN.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }

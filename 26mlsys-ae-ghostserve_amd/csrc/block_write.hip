@@ -78,12 +78,6 @@ struct Place {
     __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return x ^ rows ^ (x >> 4 & 3); }
 };
 
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Where a lane's units lie in its row.
 template <int W, int NU>
 struct Units {
@@ -185,7 +179,7 @@ __device__ __forceinline__ void make_turns(const NrArgs& p, uint32_t t, uint32_t
         Turn<F>& to = turn[turn_at<F>(i)];
         turn_of(double(p.pos[int64_t(ax) * p.axis_stride + t]) * p.freqs[i], p.factor, &to.c, &to.s);
     }
-    wave_sync();
+    wave_order();
 }
 
 // A lane's units of a finished row as 32-bit values in LDS.
@@ -319,9 +313,9 @@ __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
 #pragma unroll
             for (int j = 0; j < W; ++j) a[n][j] = float(c[n][j]), b[n][j] = float(d[n][j]);
         stage<W, NU>(p, u, place, row, a, b);
-        wave_sync();
+        wave_order();
         quantise<T, BITS>(p, place, row, half, r, sub, r < p.kv_heads);
-        wave_sync();
+        wave_order();
     }
     if (values) {
 #pragma unroll
@@ -330,7 +324,7 @@ __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
             xv.b[0][n].get(b[n]);
         }
         stage<W, NU>(p, u, place, row, a, b);
-        wave_sync();
+        wave_order();
         quantise<T, BITS>(p, place, row, half + g.half, r, sub, r < p.kv_heads);
     }
 }

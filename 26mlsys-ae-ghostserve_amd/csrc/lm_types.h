@@ -39,6 +39,13 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(fp8_clamp(c), fp8_clamp(d), r, true));
 }
 
+// What a wave wrote to LDS, before what its lanes read there from here on.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // W values as they lie in memory.
 template <class T, int W>
 struct Raw;
