@@ -18,7 +18,7 @@
 // all banks (32768 tokens of 32 + 2 x 8 heads of 128, 8 bits: 165 us with rows and turns
 // in order, two thirds of them with the LDS held by conflicts; 145 so).
 //
-// Bound by memory where tokens are many (those 145 us: 5.1 TB/s; 8192 tokens 41.5), by
+// Bound by memory where tokens are many (those 145 us: 5.1 TB/s; 8192 tokens 37.3), by
 // the launch and the chain of loads where they are few (16 tokens: 5.0 us).
 #include "block_scale.h"
 #include "norm_rotate.h"
@@ -234,8 +234,7 @@ __device__ __forceinline__ void quantise(const NrArgs& p, const Place& place, co
 
 // QITER: query rows of a group that a wave takes.  Where that is more than one, a wave
 // takes keys and values of the same heads, too, so that the lines of a record are written
-// by one (8 bits, 32768 tokens of 32 + 2 x 8 heads of 128: 173 -> 155 us when measured); where waves are
-// few each takes one of the two (3998 tokens 1.5 us less).
+// by one; where waves are few each takes one of the two (launch_block_write).
 template <class T, int BITS, int W, int NU, int QITER>
 __global__ __launch_bounds__(kNRB) void block_write_kernel(BwArgs g) {
     constexpr int WAVES = kNRB / 64;
@@ -333,8 +332,10 @@ typedef void (*BwFn)(BwArgs);
 
 template <class T, int BITS>
 BwFn pick_bw(bool wide, bool deep) {
-    if (wide) return deep ? &block_write_kernel<T, BITS, 8, 1, 4> : &block_write_kernel<T, BITS, 8, 1, 1>;
-    return &block_write_kernel<T, BITS, 1, 2, 1>;
+    if constexpr (!__is_same(T, float)) {
+        if (deep) return &block_write_kernel<T, BITS, 8, 1, 4>;
+    }
+    return wide ? &block_write_kernel<T, BITS, 8, 1, 1> : &block_write_kernel<T, BITS, 1, 2, 1>;
 }
 template <class T>
 BwFn pick_bw_bits(int bits, bool wide, bool deep) {
@@ -350,7 +351,15 @@ int launch_block_write(const NrArgs& n, int64_t tokens, int dtype, int pool_dtyp
     a.half = uint32_t(half);
     const uint32_t groups = 64u >> n.lg;
     const uint32_t k_pieces = (n.kv_heads + groups - 1) / groups, q1 = (n.heads + groups - 1) / groups;
-    const bool deep = wide && uint64_t(tokens) * (q1 + 2 * k_pieces) >= 12 * 256 * 32;
+    // Measured, us, one query row a group and four with K and V together, 8 bits: 32 + 2 x 8
+    // heads of 128, bf16, 512 tokens 5.9, 7.2; 2048 14.6, 13.4; 8192 40.6, 37.3; 16384 90.4,
+    // 75.9; 32768 174.7, 142.2.  16 + 2 x 4 heads, 1024 tokens 5.7, 7.6; 4096 17.2, 17.5;
+    // 16384 49.8, 47.6.  64 + 2 x 8, 2048 tokens 19.8, 20.6; 16384 143.7, 123.9.  Four rows
+    // lose at any size where the heads are one row a group (8 + 2 x 2 of 64, 16384 tokens
+    // 39.0, 42.9; 65536 140, 156) and in 32 bits, whose rows take twice the registers (32 + 2
+    // x 8 of 128, 8192 tokens 63.0, 68.3; 64 + 2 x 8, 32768 423, 446).  So: 16-bit values,
+    // two rows a group or more, and waves of single rows for the card twice over.
+    const bool deep = wide && dtype != KVEC_F32 && q1 > 1 && uint64_t(tokens) * (q1 + 2 * k_pieces) >= 2 * 256 * 32;
     a.q_pieces = deep ? (q1 + 3) / 4 : q1;
     a.k_pieces = k_pieces;
     const uint64_t pieces = uint64_t(a.q_pieces) + (deep ? k_pieces : 2 * k_pieces), items = uint64_t(tokens) * pieces;
