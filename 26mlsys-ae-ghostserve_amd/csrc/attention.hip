@@ -51,6 +51,12 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
     // and many short ones the short ones go through the prefix by tiles of their
     // own: 255 requests of one token and one of 512 behind 8192 take 1125 us, in two
     // calls 160 and 106; 60 and four 538, in two calls 45 and 299.
+    // Pools with block scales, whose stream blocks are runs, go by the same: us (runs, tiles),
+    // 8 bits, 64 requests of 1024 own keys with 16 rows a K/V head 60, 61, with 24 rows 78,
+    // 61, with 64 rows 139, 61; 4 bits 50, 52; 61, 52; 111, 54; heads of 64 with 16 rows 38, 51;
+    // 64 of 4096 with 32 rows of one head 58, 35; 64 of 512 behind 4096 with 32 rows 110, 169,
+    // with 64 rows 185, 165.  It is wrong for the last, and behind 512 (32 rows 72, 51; runs
+    // are taken).
     const uint64_t own_keys = len > prefix ? len - prefix : 0;
     const uint64_t by16 = (req_rows + kStreamRows - 1) / kStreamRows, by128 = (req_rows + kTileRows - 1) / kTileRows;
     p.own_tile = 0.6 * double(own_keys) * double(by16) + double(prefix) * double(req_rows) / kTileRows >
@@ -99,13 +105,17 @@ inline AttnPlan plan_attention(const kvec_attention* s) {
         p.few_keys = uint32_t(64 * subs);
         auto run_blocks = [&](uint64_t tiles, uint64_t runs) { return (tiles * runs + 7) / 8 * 8 * p.groups; };
         auto runs = [&](uint64_t tiles, uint64_t keys, uint32_t* count) {
-            // Two blocks fit a compute unit.  One request has all its runs: once the card
-            // over.  Of several most are shorter than the longest, and runs that they do
-            // not have end at once: three times over.  Measured, us, by blocks (all
-            // runs counted): one request of 262144 keys, 4 bits, 80 (512), 99 (768), 104
-            // (1536); 64 of up to 8192, 8 bits, 142 (512), 122 (768), 150 (1024), 127
-            // (1536), 136 (2048); 256 of up to 4096, 4 bits, 202, 173, 188, 160, 164.  64 keys a
-            // wave of a run, 512 parts of a row.
+            // One request has all its runs: two blocks a compute unit, once the card over.  Of
+            // several most are shorter than the longest, and runs that they do not have end at
+            // once: three times over.  Measured, us, by blocks (512, 768, 1024, 1536; all runs
+            // counted, 32 / 8 heads of 128): one request of 262144 keys, 8 bits, 106, 124, 113,
+            // 112, 4 bits (512 parts at most) 65, 66, 64, 65; 64 of up to 8192, 8 bits, 142, 118,
+            // 149, 130, 4 bits 103, 82, 97, 86; 256 of up to 4096, 4 bits, 203, 199, 188, 160.
+            // Requests that are all equally long would have fewer: 2 of 131072, 8 bits, 105,
+            // 124, 112, 119; 64 of 4096 102, 119, 108, 115, 4 bits 62, 68, 68, 78.  So would heads
+            // of 256, of which one block fits: 16 / 4 of them, 64 of 4096, 137, 147, 155, 176, of
+            // up to 4096 123, 105, 108, 115.  (A prefix's runs are counted as several requests'.)
+            // 64 keys a wave of a run, 512 parts of a row.
             uint64_t n = (B > 1 ? 1536 : 512) / (tiles * p.groups);
             if (n > keys / p.few_keys) n = keys / p.few_keys;
             if (n > 512 / subs) n = 512 / subs;

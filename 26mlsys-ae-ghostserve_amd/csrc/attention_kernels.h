@@ -1283,8 +1283,12 @@ struct RunGeom {
     // LDS takes a load or store of 16 bytes a lane as two of 8, each at half the rate where
     // the lanes lie 16 bytes apart (1 KB: 13.5 ns; as two of 8 bytes that 32 lanes spread over
     // all banks, 6.9).  So all go by pieces of 8 bytes, and where a key's pieces lie depends
-    // on the bits of its number, and for codes of the head's, such that 32 lanes always
-    // meet 32 different places of 256 bytes.
+    // on the bits of its number, and for codes of the head's, such that 32 lanes meet 32
+    // different places of 256 bytes.  (What is left, by the addresses: codes of K for heads
+    // of 96, read by pairs; scale bytes of 4 bits, where keys lie 32 bytes or more apart, by
+    // twos and for heads of 256 fours: 32 of 776 accesses of a unit for 8 heads of 128.)  No
+    // time was gained where it came in: the loads were in the way (150, 190 and 81 us for 151,
+    // 188 and 81 before).
     //
     // V in 16 bits, 4 values a piece: piece p of a key lies at p ^ v_bits.  Written are one
     // piece of each of 32 / CH keys' chunks, read (transposed) four neighbours of 8 keys.
