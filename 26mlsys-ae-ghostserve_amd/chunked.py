@@ -30,6 +30,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .blockscale import BlockPool
 from .paged import PagedKV
 from .spec import rdp_unit_for
 
@@ -114,6 +115,7 @@ class ChunkedStripes:
         del keep
 
 
-def chunk_kv(pool: torch.Tensor, page_table: torch.Tensor, c: int, chunk_tokens: int) -> PagedKV:
-    """Descriptor of prefill chunk ``c`` (positions c*chunk_tokens ..) of every sequence."""
+def chunk_kv(pool: torch.Tensor | BlockPool, page_table: torch.Tensor, c: int, chunk_tokens: int) -> PagedKV:
+    """Descriptor of prefill chunk ``c`` (positions c*chunk_tokens ..) of every sequence; of a
+    :class:`.blockscale.BlockPool` its records (codes and scales) are coded as they are."""
     return PagedKV(pool, page_table, c * chunk_tokens, chunk_tokens)
