@@ -69,6 +69,11 @@ constexpr bool kBlocks = POOL == kBlock8 || POOL == kBlock4;
 // Bits of a value.
 template <int POOL>
 constexpr int kBits = POOL == kPlain ? 16 : POOL == kBlock4 ? 4 : 8;
+// Bytes of n values (an even number of them).
+template <int POOL>
+__device__ __forceinline__ uint32_t bytes_of(uint32_t n) {
+    return kBlocks<POOL> ? n * kBits<POOL> / 8 : n * (kBits<POOL> / 8);
+}
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -448,23 +453,23 @@ __device__ __forceinline__ f32x2 settle(float m, float l, bool sees) {
     return f32x2{sees ? top : -INFINITY, sees ? l : 0.0f};
 }
 
-// Four values of a key's V row (of K/V head `head`) from value d on, zeros where there
-// are none.
+// Four values of a key's V row (of K/V head `head`, whose values start head_off bytes into
+// it; not asked for with block scales) from value d on, zeros where there are none.
 template <class T, int POOL>
-__device__ __forceinline__ u32x2 value4(const AttnArgs& a, uint32_t slot, uint32_t head, uint32_t d) {
+__device__ __forceinline__ u32x2 value4(const AttnArgs& a, uint32_t slot, uint32_t head, uint32_t head_off, uint32_t d) {
     if constexpr (kBlocks<POOL>) {
         // (a rare path: offsets worked out anew for each, not held)
         const uint32_t at = anew(head * a.dim + d);
         const bool in = d < anew(a.dim);
         u32x2 x = {0, 0};
-        const uint8_t* p = chunk_at(a, anew(slot), a.token_bytes + at * kBits<POOL> / 8, in);
+        const uint8_t* p = chunk_at(a, anew(slot), a.token_bytes + bytes_of<POOL>(at), in);
         if constexpr (POOL == kBlock8) x.x = *as_global(reinterpret_cast<const uint32_t*>(p));
         else x.x = *as_global(reinterpret_cast<const uint16_t*>(p));
         p = chunk_at(a, anew(slot), a.token_bytes + a.scales + at / kScaleBlock, in);
         const u32x4 w = widen8<kBits<POOL>>(x, scale_of(*as_global(p)), (T*)nullptr);
         return u32x2{w.x, w.y};
     }
-    const uint8_t* p = chunk_at(a, slot, a.token_bytes + (head * a.dim + d) * kBits<POOL> / 8, d < anew(a.dim));
+    const uint8_t* p = chunk_at(a, slot, a.token_bytes + head_off + bytes_of<POOL>(d), d < anew(a.dim));
     if constexpr (POOL == kFp8) return fp8_widen(*as_global(reinterpret_cast<const uint32_t*>(p)), (T*)nullptr);
     else return *as_global(reinterpret_cast<const u32x2*>(p));
 }
@@ -629,7 +634,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
     if (tid == 0) odd = 0;
     if constexpr (CODES) __syncthreads();                   // before a value is taken out
 
-    const uint32_t row_bytes = a.dim * kBits<POOL> / 8, head_off = it.head * row_bytes;
+    const uint32_t row_bytes = bytes_of<POOL>(a.dim), head_off = it.head * row_bytes;
     // V values that are not finite become 0
     auto scrub = [&](u32x4 v) {
         const uint32_t e = exponent_bits(ty);
@@ -668,7 +673,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
 #pragma unroll
     for (int i = 0; i < PER && kBlocks<POOL>; ++i) {
         const uint32_t pos = (i * kAB + tid) % CH, d = it.head * a.dim + (pos * 16 < a.dim ? pos * 16 : 0u);
-        at_code[i] = d * kBits<POOL> / 8;
+        at_code[i] = bytes_of<POOL>(d);
         at_scale[i] = a.scales + d / kScaleBlock;
     }
     auto load_codes = [&](Codes16<POOL>& x, int i, uint32_t slot, uint32_t from) __attribute__((always_inline)) {
@@ -960,7 +965,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs& a, const Item& it, uin
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 x = not_finite(value4<T, POOL>(a, sl, it.head, uint32_t(d * 32 + 8 * i) + 4 * h), ty);
+                    const f32x4 x = not_finite(value4<T, POOL>(a, sl, it.head, head_off, uint32_t(d * 32 + 8 * i) + 4 * h), ty);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[d][4 * i + j] += x[j];
                     __builtin_amdgcn_sched_barrier(0);    // a rare path: few registers, not speed
@@ -1021,7 +1026,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
     T* const ty = nullptr;
     uint8_t* const lv = wave == 0 ? v0 : wave == 1 ? v1 : wave == 2 ? v2 : v3;
 
-    const uint32_t row_bytes = a.dim * kBits<POOL> / 8, head_off = it.head * row_bytes;
+    const uint32_t row_bytes = bytes_of<POOL>(a.dim), head_off = it.head * row_bytes;
     Codes16<POOL> xv[PER];
     u32x4 xk[2][KS];                                      // fp8: 8 bytes of each
     auto fetch = [&](uint32_t slot) {                     // slot: of the keys lane % 32
@@ -1193,7 +1198,7 @@ __device__ __forceinline__ void attn_stream(const AttnArgs& a, const Item& it, u
                 const uint32_t sl = key < limit ? key_slot(a, it, key) : kNoCell;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
-                    o[d] += not_finite(value4<T, POOL>(a, sl, it.head, uint32_t(d * 16) + 4 * g), ty);
+                    o[d] += not_finite(value4<T, POOL>(a, sl, it.head, head_off, uint32_t(d * 16) + 4 * g), ty);
             }
         }
     }
@@ -1638,7 +1643,7 @@ __device__ __forceinline__ void attn_run(const AttnArgs& a, Item it, uint8_t* kc
             for (uint32_t k = base; k < min(base + kStreamKeys, it.k1); ++k) {
                 const uint32_t sl = has && k < limit ? key_slot(a, it, k) : kNoCell;
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] += not_finite(value4<T, POOL>(a, sl, it.head + h0 + mine, uint32_t(d * 16) + 4 * g), ty);
+                for (int d = 0; d < DB; ++d) o[d] += not_finite(value4<T, POOL>(a, sl, it.head + h0 + mine, 0u, uint32_t(d * 16) + 4 * g), ty);
             }
         }
     }
