@@ -46,11 +46,9 @@ def rotary_axes(sections, device="cuda") -> torch.Tensor:
     return torch.repeat_interleave(torch.arange(len(sections), dtype=torch.uint8), n).to(device)
 
 
-def _layer(pool: torch.Tensor | BlockPool, layer: int, dtype: torch.dtype) -> tuple[int, int, int, int, int]:
-    """(address of the layer, slots, kv_heads, head_dim, KVEC_* type) of a pool beside
-    queries of ``dtype``."""
-    if isinstance(pool, BlockPool):
-        return (*pool.layer(layer), pool.kv_heads, pool.dim, pool.code)
+def _layer(pool: torch.Tensor, layer: int, dtype: torch.dtype) -> tuple[int, int, int, int, int]:
+    """(address of the layer, slots, kv_heads, head_dim, KVEC_* type) of a pool tensor
+    beside queries of ``dtype``."""
     shape = pool.shape
     if len(shape) != 6 or shape[3] != 2:
         raise ValueError("pool must be [layers, pool_pages, page_tokens, 2, heads, dim]")
@@ -65,9 +63,9 @@ def _layer(pool: torch.Tensor | BlockPool, layer: int, dtype: torch.dtype) -> tu
     return pool.data_ptr() + layer * n * 2 * H * D * pool.element_size(), n, H, D, _DTYPES[pool_dt]
 
 
-def _data(pool) -> torch.Tensor:
-    """The tensor that holds a pool."""
-    return pool.data if isinstance(pool, BlockPool) else pool
+def _block_layer(pool: BlockPool, layer: int, dtype: torch.dtype) -> tuple[int, int, int, int, int]:
+    """The same of a BlockPool."""
+    return (*pool.layer(layer), pool.kv_heads, pool.dim, pool.code)
 
 
 def _scale(t, device, what: str):
@@ -106,7 +104,8 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     negative or past the pool: none) of the pool's ``layer``, in the queries' type
     or, float8_e4m3fn, as value / scale, or, a :class:`.blockscale.BlockPool`, as codes
     with their blocks' scales (K computed in 64 bits, from ``eps`` and ``factor`` rounded to
-    32, and rounded to 32 first, so that its codes do not hang on how the sums were split).  The slots of a call must be distinct.
+    32, and rounded to 32 first, so that its codes do not hang on how the sums were split).
+    The slots of a call must be distinct.
     ``tokens`` (int32 [1] on the GPU, e.g. ``cu_new[-1:]``): tokens from that
     number on are left as they were, here and in the result.
 
@@ -117,12 +116,13 @@ def norm_rotate_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     dev, dt = q.device, q.dtype
     if dt not in _COMPUTE or k.dtype != dt or v.dtype != dt:
         raise ValueError("q, k and v must be of one type: float32, bfloat16 or float16")
-    data = _data(pool)
+    blocks = isinstance(pool, BlockPool)
+    data = pool.data if blocks else pool
     _lib.require_no_grad(q, k, v, q_weight, k_weight, data, out, what="norm_rotate_write")
     _lib.require_same_device(dev, k, v, positions, freqs, data, slots, q_weight, k_weight, axis_of, tokens, out,
                              what="norm_rotate_write tensor")
     N, Hq, D = qs
-    base, n_slots, Hk, Dp, pool_dt = _layer(pool, layer, dt)
+    base, n_slots, Hk, Dp, pool_dt = (_block_layer if blocks else _layer)(pool, layer, dt)
     if Hk != ks[1] or Dp != D:
         raise ValueError(f"pool holds {Hk} heads of {Dp}, k has {ks[1]} of {D}")
     (q0, q1, q2), (k0, k1, k2), (v0, v1, v2) = q.stride(), k.stride(), v.stride()
@@ -222,10 +222,11 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor | BlockPool, page_table
         raise ValueError(f"seq_lens must be [{B}] and cu_q int32 [{B + 1}]")
     if cu_q is None and N != B:
         raise ValueError("without cu_q there is one query token a request")
-    data = _data(pool)
+    blocks = isinstance(pool, BlockPool)
+    data = pool.data if blocks else pool
     _lib.require_no_grad(q, data, out, what="prefix_attention")
     _lib.require_same_device(dev, data, page_table, seq_lens, cu_q, prefix_pages, out, what="prefix_attention tensor")
-    base, _, Hk, Dp, pool_dt = _layer(pool, layer, dt)
+    base, _, Hk, Dp, pool_dt = (_block_layer if blocks else _layer)(pool, layer, dt)
     if Dp != D or Hq % Hk:
         raise ValueError(f"q has {Hq} heads of {D}, the pool {Hk} of {Dp}")
     for t in (page_table, seq_lens, cu_q, prefix_pages):
