@@ -63,3 +63,37 @@ def test_many_requests_in_a_long_table(pkg, gpu, bits):
         parts, out = parts_with_keys(pkg, c, 4096, 0)
         check(out, want)
         assert parts[at] >= 16 and max(parts[:at] + parts[at + 1:]) <= 4
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("prefix", [0, 45, 500])
+def test_behind_a_prefix_in_a_long_table(pkg, gpu, bits, prefix):
+    """Own keys behind a prefix, some requests with none, one idle; drafts and single tokens."""
+    for new in ([1] * 6, [2, 1, 2, 0, 1, 2]):
+        own = [900, 0, 2500, 0, 31, 32]
+        lens = [prefix + o + n if n else 0 for o, n in zip(own, new)]
+        c = case(pkg, gpu, prefix + sum(new), lens, new, 8, 4, 64, BF, bits, 16, prefix, width=8192)
+        want = reference(c)
+        for max_len in (None, max(lens), 1, 1 << 30):
+            check(run(pkg, c, max_q=max(new), max_len=max_len), want)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_a_graph_of_a_long_table(pkg, gpu, bits):
+    """Captured once for the table's width, replayed on lengths from one key to thousands."""
+    top = [6000, 300, 2000]
+    c = case(pkg, gpu, bits, top, [1] * 3, 8, 2, 64, BF, bits, 16, width=16384)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run(pkg, c)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = run(pkg, c)
+    torch.cuda.current_stream().wait_stream(s)
+    for lens in ([1, 1, 1], [6000, 1, 0], [100, 300, 2000], top, [64, 65, 63]):
+        c["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, run(pkg, c))
+        check(got, reference(c))
